@@ -604,6 +604,47 @@ int indm_timer_destroy(void* handle);
 int indm_timer_reset(void* handle, int cls_mask);
 int indm_timer_read(void* handle, float* total_ms, int* launches, double* flops);
 
+/* ---- operators of a block over tokens (csrc/token_ops.hip, csrc/window_attn.hip) ------------------------------ */
+
+/* Layer norm over the last dimension: y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps), statistics fp32 from the row
+ * in registers (mean first, then the squared differences).  x: R rows of C elements, ldx elements apart (any alignment); y dense;
+ * gamma, beta fp32 [C] or NULL (1, 0); mean, rstd [R] for the backward, or both NULL.  C <= 16384 (f32) / 32768 (bf16). */
+int indm_layernorm_fwd_f32(const float* x, long ldx, const float* gamma, const float* beta, float* y, float* mean, float* rstd,
+                           long R, int C, float eps, void* stream);
+int indm_layernorm_fwd_bf16(const void* x, long ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd, long R,
+                            int C, float eps, void* stream);
+/* Its backward: dx (dense) and, where the pointers are given, dgamma = sum_r dy xh and dbeta = sum_r dy (fp32 [C]) in one pass over
+ * dy [R, C] and x; the column sums are joined over workgroups in a fixed order through ws (indm_layernorm_bwd_ws_floats floats,
+ * elem_bytes 4 or 2; NULL when neither gradient is wanted).  R = 0 writes zeros to dgamma / dbeta. */
+long indm_layernorm_bwd_ws_floats(long R, int C, int elem_bytes);
+int indm_layernorm_bwd_f32(const float* dy, const float* x, long ldx, const float* gamma, const float* mean, const float* rstd,
+                           float* dx, float* dgamma, float* dbeta, float* ws, long R, int C, void* stream);
+int indm_layernorm_bwd_bf16(const void* dy, const void* x, long ldx, const float* gamma, const float* mean, const float* rstd,
+                            void* dx, float* dgamma, float* dbeta, float* ws, long R, int C, void* stream);
+
+/* Dropout of n dense elements, optionally onto a residual: y = (res) + keep x / (1 - p), keep = Philox uniform of (0, 1] > p; the
+ * uniform of element i is word i & 3 of counter i >> 2 under the key seed + (seed_dev ? *seed_dev : 0) -- the mask of the GroupNorm
+ * entry points above for the same seed.  A dropped element is 0 whatever x holds.  The backward is the same call on dy (res NULL).
+ * 0 <= p <= 1; y may be x or res. */
+int indm_dropout_f32(const float* x, const float* res, float* y, long n, float p, unsigned long long seed, const void* seed_dev,
+                     void* stream);
+int indm_dropout_bf16(const void* x, const void* res, void* y, long n, float p, unsigned long long seed, const void* seed_dev,
+                      void* stream);
+
+/* Rotary positions over several axes, for q [B, T, H, D] and k [B, T, Hk, D] in one launch (H or Hk may be 0): the first
+ * sum(sections) entries of a head are rotated in pairs (a, b) -> (a cos - b sin, b cos + a sin) by pos[t][axis] freqs[pair], the rest
+ * passes through.  A pair of section s (n entries at offset o) is (o + j, o + n/2 + j), interleaved: (o + 2j, o + 2j + 1).
+ * strides[6]: B, T, head strides in elements of q, then of k (D contiguous, any alignment); yq, yk dense, not the inputs.
+ * pos: [T, axes] (pos_sb = 0) or [B, T, axes] (pos_sb = T axes); pos_type 0 int32, 1 fp32, 2 int64.  freqs: fp64 [sum(sections) / 2],
+ * in the pairs' order; angles are formed and reduced in 64 bits.  sections[axes], axes <= 8: even, positive, sum <= D (HOST arrays, as strides).
+ * inverse = 1: by the negative angles (the backward pass). */
+int indm_rotary_f32(const float* q, const float* k, float* yq, float* yk, const long* strides, int B, long T, int H, int Hk, int D,
+                    const void* pos, int pos_type, long pos_sb, const double* freqs, const int* sections, int axes, int interleaved,
+                    int inverse, void* stream);
+int indm_rotary_bf16(const void* q, const void* k, void* yq, void* yk, const long* strides, int B, long T, int H, int Hk, int D,
+                     const void* pos, int pos_type, long pos_sb, const double* freqs, const int* sections, int axes, int interleaved,
+                     int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -162,6 +162,15 @@ _SIGS = {
     "indm_h16_downsample2x": [c_p, c_p, c_i, c_i, c_i, c_i, c_f, c_p],
     "indm_h16_from_f32": [c_p, c_p, c_l, c_p],
     "indm_h16_to_f32": [c_p, c_p, c_l, c_f, c_p],
+    "indm_layernorm_fwd_f32": [c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_l, c_i, c_f, c_p],
+    "indm_layernorm_fwd_bf16": [c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_l, c_i, c_f, c_p],
+    "indm_layernorm_bwd_ws_floats": [c_l, c_i, c_i],
+    "indm_layernorm_bwd_f32": [c_p, c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_l, c_i, c_p],
+    "indm_layernorm_bwd_bf16": [c_p, c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_l, c_i, c_p],
+    "indm_dropout_f32": [c_p, c_p, c_p, c_l, c_f, c_u64, c_p, c_p],
+    "indm_dropout_bf16": [c_p, c_p, c_p, c_l, c_f, c_u64, c_p, c_p],
+    "indm_rotary_f32": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
+    "indm_rotary_bf16": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
     "indm_timer_create": [c_i, c_p],
     "indm_timer_destroy": [c_p],
     "indm_timer_reset": [c_p, c_i],
@@ -170,7 +179,7 @@ _SIGS = {
 _LONG_RET = {"indm_groupnorm_ws_floats", "indm_colreduce_ws_floats", "indm_segreduce_ws_floats", "indm_rowreduce_ws_floats",
              "indm_dsm_ws_floats", "indm_sqnorm_ws_floats", "indm_ires_bwd_act_ws_floats", "indm_iresblock_ws_floats",
              "indm_pc_step_ws_floats", "indm_hutch_div_ws_floats", "indm_f16_bwd_act_ok", "indm_f16_wgrad_ws_floats",
-             "indm_h16_groupnorm_ws_floats", "indm_h16_segreduce_ws_floats"}
+             "indm_h16_groupnorm_ws_floats", "indm_h16_segreduce_ws_floats", "indm_layernorm_bwd_ws_floats"}
 
 EXPORTED_SYMBOLS = tuple(sorted(_SIGS))
 
@@ -2171,3 +2180,168 @@ def iresblock_inverse(y, cb, W1, W2T, W3, b1, b2, b3, preact, atol, rtol):
         return None
     _chk(st, "indm_iresblock_inverse")
     return x, it.value
+
+
+# --------------------------------------------------------------------------- operators of a block over tokens (csrc/token_ops.hip, window_attn.hip)
+_TOKEN_DTYPES = {torch.float32: "f32", torch.bfloat16: "bf16"}
+
+
+def _require(ok, what):
+    if not ok:
+        raise RuntimeError("indm_amd: " + what)
+
+
+def _token_suffix(op, x):
+    _require(x.dtype in _TOKEN_DTYPES, f"{op}: expected float32 or bfloat16, got {x.dtype}")
+    return _TOKEN_DTYPES[x.dtype]
+
+
+def _token_device(op, *tensors):
+    """every tensor on one GPU; -> a context in which that GPU is the current device (allocations and the launch go there)"""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError("indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback")
+            _require(t.device == dev, f"{op}: tensors on {dev} and {t.device}")
+    return _NO_TIMING if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _data(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows2d(x):
+    """(x, R, row stride) of x [..., C] as R rows with one stride and contiguous columns; a copy only where x has no such view"""
+    C = x.shape[-1]
+    R = x.numel() // C if C else 0
+    if x.is_contiguous():
+        return x, R, C
+    if x.numel() and (x.stride(-1) == 1 or C == 1):
+        try:
+            v = x.view(R, C)
+            return v, R, v.stride(0)
+        except RuntimeError:
+            pass
+    return x.contiguous(), R, C
+
+
+def _ln_check(x, gamma, beta):
+    suf = _token_suffix("layer_norm", x)
+    _require(x.dim() >= 1 and x.shape[-1] > 0, f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
+    C = x.shape[-1]
+    most = 16384 if suf == "f32" else 32768
+    _require(C <= most, f"layer_norm: rows of up to {most} {suf} elements, got {C}")
+    for name, p in (("gamma", gamma), ("beta", beta)):
+        if p is not None:
+            _require(p.dtype == torch.float32, f"layer_norm: {name} is float32, got {p.dtype}")
+            _require(tuple(p.shape) == (C,), f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
+    return suf
+
+
+def layernorm_fwd(x, gamma=None, beta=None, eps=1e-6, stats=True):
+    """x [..., C] -> y, mean [R], rstd [R] (None, None without stats)"""
+    suf = _ln_check(x, gamma, beta)
+    _require(eps >= 0.0, f"layer_norm: eps >= 0, got {eps}")
+    with _token_device("layer_norm", x, gamma, beta):
+        gamma = gamma if gamma is None or gamma.is_contiguous() else gamma.contiguous()
+        beta = beta if beta is None or beta.is_contiguous() else beta.contiguous()
+        xr, R, ldx = _rows2d(x)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = torch.empty((R,), dtype=torch.float32, device=x.device) if stats else None
+        rstd = torch.empty_like(mean) if stats else None
+        st = getattr(lib(), "indm_layernorm_fwd_" + suf)(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean),
+                                                         _data(rstd), R, x.shape[-1], eps, _stream())
+        _chk(st, "indm_layernorm_fwd_" + suf)
+    return y, mean, rstd
+
+
+def layernorm_bwd(dy, x, gamma, mean, rstd, want_gamma=True, want_beta=True):
+    """-> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its own: calls on different
+    streams, or in different captured graphs, share nothing."""
+    suf = _ln_check(x, gamma, None)
+    _require(dy.dtype == x.dtype and dy.shape == x.shape, f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    with _token_device("layer_norm", x, dy, gamma, mean, rstd):
+        C = x.shape[-1]
+        gamma = gamma if gamma is None or gamma.is_contiguous() else gamma.contiguous()
+        dy = dy if dy.is_contiguous() else dy.contiguous()
+        xr, R, ldx = _rows2d(x)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dgamma = torch.empty((C,), dtype=torch.float32, device=x.device) if want_gamma else None
+        dbeta = torch.empty((C,), dtype=torch.float32, device=x.device) if want_beta else None
+        ws = None
+        if want_gamma or want_beta:
+            ws = torch.empty((max(1, lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size())),), dtype=torch.float32, device=x.device)
+        st = getattr(lib(), "indm_layernorm_bwd_" + suf)(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean.data_ptr(), rstd.data_ptr(),
+                                                         dx.data_ptr(), _data(dgamma), _data(dbeta), _data(ws), R, C, _stream())
+        _chk(st, "indm_layernorm_bwd_" + suf)
+    return dx, dgamma, dbeta
+
+
+def dropout(x, p, seed, res=None, seed_dev=None):
+    """(res) + keep(seed + *seed_dev) x / (1 - p), the mask by x's dense (row-major) element index"""
+    suf = _token_suffix("dropout", x)
+    p = float(p)
+    _require(0.0 <= p <= 1.0, f"dropout: 0 <= p <= 1, got {p}")
+    _require(0 <= int(seed) < 1 << 64, f"dropout: the seed is a whole number of 64 bits, got {seed}")
+    if res is not None:
+        _require(res.shape == x.shape and res.dtype == x.dtype, f"dropout: res is {tuple(x.shape)} {x.dtype}, got {tuple(res.shape)} {res.dtype}")
+    if seed_dev is not None:
+        _require(seed_dev.dtype == torch.int64 and seed_dev.numel() == 1, "dropout: seed_dev is one int64 on the device")
+    with _token_device("dropout", x, res, seed_dev):
+        x = x if x.is_contiguous() else x.contiguous()
+        res = res if res is None or res.is_contiguous() else res.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        st = getattr(lib(), "indm_dropout_" + suf)(x.data_ptr(), _data(res), y.data_ptr(), x.numel(), p, int(seed), _seed_ptr(seed_dev),
+                                                   _stream())
+        _chk(st, "indm_dropout_" + suf)
+    return y
+
+
+_POS_TYPES = {torch.int32: 0, torch.float32: 1, torch.int64: 2}
+
+
+def _heads_strides(x):
+    """x [B, T, H, D] with D contiguous (a copy where it is not) and its B, T, H strides"""
+    x = x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    return x, x.stride()[:3]
+
+
+def _rotary_check(q, k, pos, freqs, sections):
+    suf = _token_suffix("rotary", q)
+    _require(q.dim() == 4, f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
+    B, T, _, D = q.shape
+    if k is not None:
+        _require(k.dtype == q.dtype and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D,
+                 f"rotary: k is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
+    A = len(sections)
+    _require(1 <= A <= 8 and all(int(n) == n and n > 0 and n % 2 == 0 for n in sections) and sum(sections) <= D,
+             f"rotary: sections are 1 to 8 even positive numbers that sum to {D} at most, got {tuple(sections)}")
+    _require(pos.dtype in _POS_TYPES, f"rotary: positions are int32, int64 or float32, got {pos.dtype}")
+    _require(tuple(pos.shape) in ((T, A), (B, T, A)), f"rotary: pos is [{T}, {A}] or [{B}, {T}, {A}], got {tuple(pos.shape)}")
+    _require(freqs.dtype == torch.float64 and tuple(freqs.shape) == (sum(sections) // 2,),
+             f"rotary: freqs is float64 [{sum(sections) // 2}], got {tuple(freqs.shape)} {freqs.dtype}")
+    return suf
+
+
+def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
+    """q [B, T, H, D], k [B, T, Hk, D] or None -> their rotated copies (dense)"""
+    suf = _rotary_check(q, k, pos, freqs, sections)
+    with _token_device("rotary", q, k, pos, freqs):
+        B, T, H, D = q.shape
+        Hk = 0 if k is None else k.shape[2]
+        q, sq = _heads_strides(q)
+        sk = (0, 0, 0)
+        yk = None
+        if k is not None:
+            k, sk = _heads_strides(k)
+            yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        pos = pos if pos.is_contiguous() else pos.contiguous()
+        freqs = freqs if freqs.is_contiguous() else freqs.contiguous()
+        st = getattr(lib(), "indm_rotary_" + suf)(q.data_ptr(), _data(k), yq.data_ptr(), _data(yk), (c_l * 6)(*sq, *sk), B, T, H, Hk, D,
+                                                  pos.data_ptr(), _POS_TYPES[pos.dtype], T * len(sections) if pos.dim() == 3 else 0,
+                                                  freqs.data_ptr(), (c_i * len(sections))(*[int(n) for n in sections]), len(sections),
+                                                  int(bool(interleaved)), int(bool(inverse)), _stream())
+        _chk(st, "indm_rotary_" + suf)
+    return yq, yk

@@ -10,6 +10,7 @@ import math
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -961,6 +962,94 @@ class _SlogdetInv(Function):
 def slogdet(w):
     """log|det w| as a [1] tensor, differentiable (d/dw = w^-T)."""
     return _SlogdetInv.apply(w)
+
+
+# ----------------------------------------------------------------------------- a block over tokens (csrc/token_ops.hip, window_attn.hip)
+def _tracked(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _LayerNorm(Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps):
+        y, mean, rstd = hip.layernorm_fwd(x, gamma, beta, eps)
+        ctx.save_for_backward(x, gamma, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma, mean, rstd = ctx.saved_tensors
+        dx, dg, db = hip.layernorm_bwd(dy, x, gamma, mean, rstd, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return dx, dg, db, None
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-6):
+    """Layer norm over the last dimension of x [..., C] (fp32 or bf16, any strides), times gamma [C], plus beta [C] (fp32; either
+    may be None).  Statistics and the sums of the parameters' gradients are fp32; the same bits on every call."""
+    if not _tracked(x, gamma, beta):
+        return hip.layernorm_fwd(x, gamma, beta, eps, stats=False)[0]
+    return _LayerNorm.apply(x, gamma, beta, float(eps))
+
+
+class _Dropout(Function):
+    @staticmethod
+    def forward(ctx, x, res, p, seed):
+        sd = hip.SEED_DEV[0] if p > 0 else None
+        ctx.cfg = (p, seed, sd)
+        return hip.dropout(x, p, seed, res, sd)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        p, seed, sd = ctx.cfg
+        dx = hip.dropout(dy, p, seed, None, sd) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x, p, seed, res=None):
+    """Dropout from a counter-based generator, onto a residual of x's shape if given: res + keep x / (1 - p).  The mask is a function
+    of (seed, element index) -- the one group_norm(drop_p=, seed=) applies for the same seed --, is regenerated in the backward pass
+    and never stored; seeds come from rng.dropout_seed().  fp32 or bf16; dropped elements are 0 whatever x holds.  A captured graph
+    replays the seed that it was captured with, unless hip.SEED_DEV holds a device offset to it (as graphed.py sets it)."""
+    return _Dropout.apply(x, res, float(p), int(seed))
+
+
+def rotary_freqs(sections, base=10000.0, device=None):
+    """The frequencies of rotary(): base ** (-2 j / n), j < n / 2, of each section of n entries, fp64 [sum(sections) / 2].  Built once
+    and kept by the module that uses it."""
+    return torch.cat([float(base) ** (-2.0 * torch.arange(int(n) // 2, dtype=torch.float64) / int(n)) for n in sections]).to(device)
+
+
+class _Rotary(Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, freqs, sections, interleaved):
+        ctx.save_for_backward(pos, freqs)
+        ctx.cfg = (sections, interleaved)
+        ctx.set_materialize_grads(False)
+        return hip.rotary(q, k, pos, freqs, sections, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        pos, freqs = ctx.saved_tensors
+        sections, interleaved = ctx.cfg
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        if dq is None:
+            if dk is not None:
+                dk = hip.rotary(dk, None, pos, freqs, sections, interleaved, inverse=True)[0]
+        else:
+            dq, dk = hip.rotary(dq, dk, pos, freqs, sections, interleaved, inverse=True)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q, k, pos, freqs, sections, interleaved=False):
+    """Rotary positions over several axes (time, height, width of image or clip tokens) -> (q', k').  q [B, T, H, D], k [B, T, Hk, D] or
+    None, fp32 or bf16, any strides (columns of one fused product).  sections: entries of a head per axis (even), the rest passes
+    through; pos [T, A] or [B, T, A] (int32, int64 or fp32), the token's coordinate on each axis; freqs from rotary_freqs().  A pair
+    (a, b) -> (a cos - b sin, b cos + a sin) of the angle pos freq; pairs are the halves of a section, or neighbours if interleaved."""
+    return _Rotary.apply(q, k, pos, freqs, tuple(int(n) for n in sections), bool(interleaved))
 
 
 INV_SQRT2 = 1.0 / math.sqrt(2.0)
