@@ -1,0 +1,731 @@
+// Attention over tokens with a sliding window and a few first tokens that stay visible ("sinks"), several heads, key / value heads
+// shared by groups of query heads, sequences of different lengths; fp32 or bf16 in HBM, fp32 softmax and accumulators.
+//
+//   o_i = sum_j P_ij v_j,  P_ij = exp(c' q_i.k_j - lse_i) over the visible j:
+//   i, j < n,  (i - left <= j <= i + right  or  j < sinks),  causal: j <= i           (a row i >= n gives zeros)
+//
+// All three kernels (FWD, DQ: the owner is a query; DKV: the owner is a key) have one shape.  A wavefront owns 32 tokens and holds
+// their vectors as matrix-instruction operands in registers; the other side streams through LDS in double-buffered tiles of BN
+// tokens that all wavefronts of the workgroup share.
+//   S^T[y][x] = sum_d Y[y][d] X[x][d]      A = rows of the tile, B = the owners: lane (l31, lhi) ends up with the owner x = l31 and
+//                                          y = 32 yb + 8 (r >> 2) + (r & 3) + 4 lhi in accumulator register r of block yb -- so a
+//                                          row's maximum and sum are in-lane work and one exchange with lane ^ 32
+//   out^T[d][x] += sum_y Z[y][d] W[y][x]   eight registers of a block, rounded to the operand type, ARE the B operand (k position t
+//                                          <-> y = 8 (t >> 2) + 4 lhi + (t & 3)); A is read transposed out of the same tile
+//                                          (ds_read_b64_tr_b16 on bf16), and out keeps the owner in the lane: rescaling is in-lane
+// On fp32 the same operands are 8 values a lane and a product is 8 v_mfma_f32_32x32x2_f32 (their k order differs from the bf16
+// instruction's, the same way on both sides).  P and dS are rounded to bf16 as operands of the second product on bf16 tensors: each
+// term is then off by half a step like the result itself, and the terms' errors average out in the sum.
+// The softmax is exp2 with a running maximum that is raised only when a new logit exceeds it by 8 (P <= 256 then: no digit is lost,
+// and the accumulators are rescaled once or twice a row instead of once a tile).
+#include "indm_common.h"
+#pragma clang diagnostic ignored "-Winline-asm"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16;
+
+__device__ __attribute__((aligned(16))) const unsigned zero16[4] = {0u, 0u, 0u, 0u};   // what a chunk outside a tensor reads
+
+struct WAttnArgs {
+  const void *q, *k, *v;            // [B, T, heads, D], D contiguous, 16-byte rows; strides in elements
+  long qb, qt, qh, kb, kt, kh, vb, vt, vh;
+  const void *o, *dO;               // dense [B, T, H, D] (backward)
+  void *out, *dq, *dk, *dv;         // dense
+  float* lse;                       // [B, H, T]: log2 of the sum of exponentials, in units of the exp2 argument
+  float* delta;                     // [B, H, T]: <dO, o>
+  float* part;                      // sink partials [B Hk][chunks][32 key blocks][2][D]
+  const int* lengths;               // [B] or NULL
+  int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks;
+  float c, scale;                   // scale * log2(e), scale
+};
+
+constexpr int pow2_ceil(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
+
+template <typename T, int DP>
+struct Geo {
+  static constexpr int EPC = 16 / (int)sizeof(T);                  // elements of a 16-byte chunk
+  static constexpr int CH = DP / EPC, NCH = pow2_ceil(CH);         // chunks of a row, and with padding to a power of two
+  static constexpr int RB = NCH * 16;                              // bytes of a row in LDS
+  static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NY = BN / 32;   // streamed tokens a tile
+  static constexpr int TILE = BN * RB;
+  static constexpr int KK = DP / 16, DB = DP / 32;
+  // LDS address of chunk c of row r: c ^ swz(r).  16 successive rows at one chunk (the row-wise operand reads) and four
+  // successive rows at one 64-byte unit (the transposed ones) then fall on different banks.
+  static __device__ __forceinline__ int swz(int r) {
+    return NCH == 4 ? (r >> 2) & 3 : NCH == 8 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+  }
+};
+
+template <typename T> struct Op;
+template <> struct Op<u16> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ frag zero() {
+    const u32x4 z = {0u, 0u, 0u, 0u};
+    return __builtin_bit_cast(frag, z);
+  }
+  static __device__ __forceinline__ frag global(const u16* p) { return *(const bf16x8*)p; }
+  static __device__ __forceinline__ frag pack(const f32x16& s, int o) {
+    return indm_pack_bf16x8(s[o], s[o + 1], s[o + 2], s[o + 3], s[o + 4], s[o + 5], s[o + 6], s[o + 7]);
+  }
+  static __device__ __forceinline__ float get(const frag& f, int i) { return (float)f[i]; }
+};
+struct f32frag {
+  f32x4 a, b;
+};
+template <> struct Op<float> {
+  typedef f32frag frag;
+  static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.a[i], b.a[i], c, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.b[i], b.b[i], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ frag zero() {
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    return {z, z};
+  }
+  static __device__ __forceinline__ frag global(const float* p) { return {*(const f32x4*)p, *(const f32x4*)(p + 4)}; }
+  static __device__ __forceinline__ frag pack(const f32x16& s, int o) {
+    const f32x4 a = {s[o], s[o + 1], s[o + 2], s[o + 3]}, b = {s[o + 4], s[o + 5], s[o + 6], s[o + 7]};
+    return {a, b};
+  }
+  static __device__ __forceinline__ float get(const frag& f, int i) { return i < 4 ? f.a[i] : f.b[i - 4]; }
+};
+
+template <typename T> using Frag = typename Op<T>::frag;
+
+// value of the other half of the wavefront combined with this one's: x over lanes l31 and l31 + 32
+__device__ __forceinline__ float half_max(float x) {
+  const unsigned u = __float_as_uint(x);
+  const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const unsigned u = __float_as_uint(x);
+  const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// the lane's places in a tile, computed once
+template <typename T, int DP>
+struct Lane {
+  using G = Geo<T, DP>;
+  int l31, lhi, row, tr0, tr1, x, t0, t1;
+  __device__ __forceinline__ Lane(int lane) {
+    l31 = lane & 31;
+    lhi = lane >> 5;
+    row = l31 * G::RB;                       // row-wise operand: row l31, chunk (.. + lhi) ^ x
+    x = G::swz(l31);
+    if constexpr (sizeof(T) == 2) {
+      const int jj = (lane & 15) >> 2, g1 = (lane >> 4) & 1, c4 = lane & 3, r = 4 * lhi + jj;
+      tr0 = r * G::RB + (c4 & 1) * 8;        // transposed operand: rows r and r + 8 of a 16-row group
+      tr1 = tr0 + 8 * G::RB;
+      t0 = (2 * g1 + (c4 >> 1)) ^ G::swz(r);
+      t1 = (2 * g1 + (c4 >> 1)) ^ G::swz(r + 8);
+    } else {
+      tr0 = 4 * lhi * G::RB + (l31 & 3) * 4;
+      tr1 = t0 = t1 = 0;
+    }
+  }
+  // elements 16 kk + 8 lhi .. + 7 of row 32 yb + l31
+  __device__ __forceinline__ typename Op<T>::frag rowwise(const char* tile, int yb, int kk) const {
+    const char* p = tile + row + yb * 32 * G::RB;
+    if constexpr (sizeof(T) == 2) {
+      return *(const bf16x8*)(p + (((2 * kk + lhi) ^ x) << 4));
+    } else {
+      return {*(const f32x4*)(p + (((4 * kk + 2 * lhi) ^ x) << 4)), *(const f32x4*)(p + (((4 * kk + 2 * lhi + 1) ^ x) << 4))};
+    }
+  }
+  // element d = 32 db + l31 of the eight rows r0 + 8 (t >> 2) + 4 lhi + (t & 3), r0 a multiple of 16
+  __device__ __forceinline__ typename Op<T>::frag transposed(const char* tile, int r0, int db) const {
+    if constexpr (sizeof(T) == 2) {
+      const char* p = tile + r0 * G::RB;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(p + tr0 + (((db * 4) ^ t0) << 4)));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(p + tr1 + (((db * 4) ^ t1) << 4)));
+      const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(bf16x8, v);
+    } else {
+      const char* p = tile + r0 * G::RB + tr0;
+      const int chunk = db * 8 + (l31 >> 2);
+      f32frag f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int r = 8 * (t >> 2) + (t & 3);
+        const float v = *(const float*)(p + r * G::RB + ((chunk ^ G::swz(r + 4 * lhi)) << 4));
+        if (t < 4) f.a[t] = v; else f.b[t - 4] = v;
+      }
+      return f;
+    }
+  }
+};
+
+// rows first .. first + BN - 1 of a head -> a tile in LDS, by direct copies of 16 bytes a lane (1 KB a wave-instruction, the swizzle is
+// on the source side).  Rows from n on and chunks from D on read zeros: what lies behind a sequence never enters a product.
+template <typename T, int DP, int WV>
+__device__ __forceinline__ void stage(char* tile, const T* src, long stride, int first, int n, int D, int wave, int lane) {
+  using G = Geo<T, DP>;
+  constexpr int COPIES = G::BN * G::NCH / 64;
+#pragma unroll
+  for (int i = 0; i < (COPIES + WV - 1) / WV; ++i) {
+    const int w = wave + i * WV;
+    if (COPIES % WV == 0 || w < COPIES) {
+      const int slot = w * 64 + lane, r = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(r);
+      const bool in = first + r < n && c * G::EPC < D;
+      const void* s = in ? (const void*)(src + (long)(first + r) * stride + c * G::EPC) : (const void*)zero16;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
+                                       (__attribute__((address_space(3))) void*)(tile + w * 1024), 16, 0, 0);
+    }
+  }
+}
+__device__ __forceinline__ void staged() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// the owner's row as operands (rows from n on: zeros)
+template <typename T, int DP>
+__device__ __forceinline__ void load_owner(const T* row, bool live, int D, int lhi, Frag<T> (&f)[Geo<T, DP>::KK]) {
+#pragma unroll
+  for (int kk = 0; kk < Geo<T, DP>::KK; ++kk)
+    f[kk] = live && 16 * kk + 8 * lhi < D ? Op<T>::global(row + 16 * kk + 8 * lhi) : Op<T>::zero();
+}
+
+// out^T in the accumulators -> the owner's row: 16 bytes a lane and store.  (bf16: the halves trade, so that lane l31 holds elements
+// 0 .. 7 and lane l31 + 32 elements 8 .. 15 of each 16.)
+template <typename T, int DP>
+__device__ __forceinline__ void store_owner(T* row, const f32x16 (&acc)[Geo<T, DP>::DB], float f, bool live, int D, int lhi) {
+#pragma unroll
+  for (int db = 0; db < Geo<T, DP>::DB; ++db) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int a = 0; a < 4; a += 2) {
+        unsigned w[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const f32x2 v = {acc[db][4 * (a + h) + 2 * e] * f, acc[db][4 * (a + h) + 2 * e + 1] * f};
+            w[h][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+          }
+        const u32x2 s0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false));
+        const u32x2 s1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false));
+        const u32x4 o = {s0[0], s1[0], s0[1], s1[1]};
+        const int d = 32 * db + 8 * a + 8 * lhi;
+        if (live && d < D) *(u32x4*)(row + d) = o;
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 o = {acc[db][4 * a] * f, acc[db][4 * a + 1] * f, acc[db][4 * a + 2] * f, acc[db][4 * a + 3] * f};
+        const int d = 32 * db + 8 * a + 4 * lhi;
+        if (live && d < D) *(f32x4*)(row + d) = o;
+      }
+    }
+  }
+}
+
+// workgroup -> work item, so that neighbouring items (which share most of their tiles) run on one XCD's L2
+__device__ __forceinline__ int xcd_item(int id, int total) {
+  const int x = id & 7, per = total >> 3, rem = total & 7;
+  return x * per + (x < rem ? x : rem) + (id >> 3);
+}
+
+__device__ __forceinline__ int seq_len(const WAttnArgs& p, int b) {
+  if (p.lengths == nullptr) return p.T;
+  const int n = p.lengths[b];
+  return n < 0 ? 0 : n < p.T ? n : p.T;
+}
+
+// tiles of keys that queries q0 .. q1 of a sequence of n see: [0, ns) and [t0, t1]
+struct KeyTiles {
+  int ns, t0, count;
+};
+__device__ __forceinline__ KeyTiles key_tiles(const WAttnArgs& p, int q0, int q1, int n, int BN) {
+  if (q0 >= n) return {0, 0, 0};
+  if (q1 > n - 1) q1 = n - 1;
+  int lo = q0 - p.left, hi = p.causal ? q1 : q1 + p.right;
+  lo = lo < 0 ? 0 : lo;
+  hi = hi > n - 1 ? n - 1 : hi;
+  int s = p.sinks < n ? p.sinks : n;
+  if (p.causal && s > q1 + 1) s = q1 + 1;
+  const int st = (s + BN - 1) / BN;
+  int t0 = lo / BN, t1 = hi / BN;
+  if (st >= t0) {
+    t0 = s > 0 ? 0 : t0;
+    if (st - 1 > t1) t1 = st - 1;
+    return {0, t0, t1 - t0 + 1};
+  }
+  return {st, t0, st + t1 - t0 + 1};
+}
+
+// ---------------------------------------------------------------------------------------------- owner = queries: forward, dq
+template <typename T, int DP, int WV, bool BWD>
+__global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
+  using G = Geo<T, DP>;
+  using O = Op<T>;
+  typedef typename O::frag frag;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][K tile, V tile]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Lane<T, DP> at(lane);
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.H, b = bh / p.H;
+  const int n = seq_len(p, b);
+  const int q0 = tile * (WV * 32), qw = q0 + wave * 32, i = qw + at.l31;
+  const int hk = h / (p.H / p.Hk);
+  const T* K = (const T*)p.k + b * p.kb + hk * p.kh;
+  const T* V = (const T*)p.v + b * p.vb + hk * p.vh;
+  const long orow = (((long)b * p.T + i) * p.H + h) * p.D, srow = ((long)b * p.H + h) * p.T + i;
+  const bool live = i < n;
+  const KeyTiles kt = key_tiles(p, q0, q0 + WV * 32 - 1, n, G::BN);
+  auto first_of = [&](int it) { return (it < kt.ns ? it : kt.t0 + it - kt.ns) * G::BN; };
+  auto fetch = [&](int it) {
+    char* buf = smem + (it & 1) * 2 * G::TILE;
+    stage<T, DP, WV>(buf, K, p.kt, first_of(it), n, p.D, wave, lane);
+    stage<T, DP, WV>(buf + G::TILE, V, p.vt, first_of(it), n, p.D, wave, lane);
+  };
+  if (kt.count > 0) fetch(0);
+
+  frag qf[G::KK], df[BWD ? G::KK : 1];
+  load_owner<T, DP>((const T*)p.q + b * p.qb + (long)i * p.qt + h * p.qh, live, p.D, at.lhi, qf);
+  float lse = INFINITY, delta = 0.f;
+  if constexpr (BWD) {
+    load_owner<T, DP>((const T*)p.dO + orow, live, p.D, at.lhi, df);
+    frag of[G::KK];
+    load_owner<T, DP>((const T*)p.o + orow, live, p.D, at.lhi, of);
+#pragma unroll
+    for (int kk = 0; kk < G::KK; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta += O::get(df[kk], e) * O::get(of[kk], e);
+    delta = half_sum(delta);
+    if (live) lse = p.lse[srow];
+    if (i < p.T && at.lhi == 0) p.delta[srow] = delta;
+  }
+  // the lane's visible keys: lo .. hi, and those below sk
+  const int lo = i - p.left;
+  int hi = p.causal ? i : i + p.right, sk = p.sinks;
+  if (hi > n - 1) hi = n - 1;
+  if (p.causal && sk > i + 1) sk = i + 1;
+  if (sk > n) sk = n;
+  if (!live) {
+    hi = lo - 1;
+    sk = 0;
+  }
+
+  f32x16 acc[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float m = -INFINITY, sum = 0.f;   // running maximum in use (units of the exp2 argument), this lane's half of the sum
+  const int qa = qw, qb = qw + 31 < n - 1 ? qw + 31 : n - 1;
+
+  if (kt.count > 0) staged();
+  for (int it = 0; it < kt.count; ++it) {
+    if (it + 1 < kt.count) fetch(it + 1);
+    const char* kb = smem + (it & 1) * 2 * G::TILE;
+    const char* vb = kb + G::TILE;
+    const int k0 = first_of(it), k1 = k0 + G::BN - 1;
+    // (wave-uniform) does any of this wavefront's queries see any of the tile's keys?  all of all?
+    const bool any = qa < n && k0 < n && (k0 < p.sinks || (k1 >= qa - p.left && (p.causal || k0 <= qb + p.right))) && (!p.causal || k0 <= qb);
+    const bool all = k1 < n && (k1 < p.sinks || (k0 >= qa + 31 - p.left && (p.causal || k1 <= qa + p.right))) && (!p.causal || k1 <= qa);
+    if (any) {
+      f32x16 S[G::NY];
+#pragma unroll
+      for (int y = 0; y < G::NY; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[y][r] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < G::KK; ++kk)
+#pragma unroll
+        for (int y = 0; y < G::NY; ++y) S[y] = O::mma(at.rowwise(kb, y, kk), qf[kk], S[y]);
+      if (!all) {
+#pragma unroll
+        for (int y = 0; y < G::NY; ++y)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = k0 + 32 * y + 8 * (r >> 2) + (r & 3) + 4 * at.lhi;
+            S[y][r] = (j >= lo && j <= hi) || j < sk ? S[y][r] : -INFINITY;
+          }
+      }
+      if constexpr (!BWD) {
+        float top = S[0][0];
+#pragma unroll
+        for (int y = 0; y < G::NY; ++y)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, S[y][r]);
+        top = half_max(top) * p.c;
+        if (__any(top > m + 8.f)) {   // (-inf + 8 = -inf: the first visible key always raises it)
+          const float up = fmaxf(m, top);
+          const float f = up > -INFINITY ? __builtin_amdgcn_exp2f(m - up) : 1.f;
+          m = up;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        }
+        const float mm = m > -INFINITY ? m : 0.f;
+#pragma unroll
+        for (int y = 0; y < G::NY; ++y)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            S[y][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[y][r], p.c, -mm));
+            sum += S[y][r];
+          }
+      } else {
+#pragma unroll
+        for (int y = 0; y < G::NY; ++y) {
+          f32x16 dP;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dP[r] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < G::KK; ++kk) dP = O::mma(at.rowwise(vb, y, kk), df[kk], dP);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            S[y][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[y][r], p.c, -lse)) * (dP[r] - delta);   // dS / scale
+        }
+      }
+      const char* zb = BWD ? kb : vb;
+#pragma unroll
+      for (int y = 0; y < G::NY; ++y)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const frag w = O::pack(S[y], 8 * a);
+#pragma unroll
+          for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
+        }
+    }
+    staged();
+  }
+
+  if (!live) {   // (also where a visible key's values were infinite: 0 times that is not 0)
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  }
+  if constexpr (!BWD) {
+    sum = half_sum(sum);
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    store_owner<T, DP>((T*)p.out + orow, acc, inv, i < p.T, p.D, at.lhi);
+    if (p.lse != nullptr && i < p.T && at.lhi == 0) p.lse[srow] = live ? m + __log2f(sum) : INFINITY;
+  } else {
+    store_owner<T, DP>((T*)p.dq + orow, acc, p.scale, i < p.T, p.D, at.lhi);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- owner = keys: dk, dv
+// The queries of every head of the group stream past the key.  SINK = false: the window's part of all keys.  SINK = true: what the sink
+// keys get from queries whose window they are outside of -- a few keys against all queries, so the queries are split over p.chunks
+// workgroups whose fp32 partial sums the first kind adds up in order (no atomics).
+template <typename T, int DP, int WV, bool SINK>
+__global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
+  using G = Geo<T, DP>;
+  using O = Op<T>;
+  typedef typename O::frag frag;
+  constexpr int BUF = 2 * G::TILE + 2 * G::BN * (int)sizeof(float);
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile, dO tile, lse, delta]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Lane<T, DP> at(lane);
+  const int item = xcd_item(blockIdx.x, gridDim.x);
+  const int per = SINK ? p.tiles * p.chunks : p.tiles;
+  const int bh = item / per, hk = bh % p.Hk, b = bh / p.Hk;
+  const int chunk = SINK ? item % per % p.chunks : 0, tile = SINK ? item % per / p.chunks : item % per;
+  const int n = seq_len(p, b), group = p.H / p.Hk;
+  const int j0 = tile * (WV * 32), jw = j0 + wave * 32, j = jw + at.l31;
+  const bool live = j < n;
+  // tiles of queries: i0 .. i1 of each head of the group, one after the other (SINK: this chunk's share of all of them)
+  int i0, i1;
+  if constexpr (SINK) {
+    i0 = p.causal ? j0 : 0;
+    i1 = n - 1;
+  } else {
+    i0 = p.causal ? j0 : j0 - p.right;
+    i1 = j0 + WV * 32 - 1 + p.left;
+    i0 = i0 < 0 ? 0 : i0;
+    i1 = i1 > n - 1 ? n - 1 : i1;
+  }
+  const int t0 = i0 / G::BN, nt = j0 < n && i1 >= i0 ? i1 / G::BN - t0 + 1 : 0;
+  int from = 0, to = nt * group;
+  if constexpr (SINK) {
+    from = (int)((long)to * chunk / p.chunks);
+    to = (int)((long)to * (chunk + 1) / p.chunks);
+  }
+  float hold[2];
+  auto fetch = [&](int it) {
+    const int h = hk * group + it / nt, first = (t0 + it % nt) * G::BN;
+    char* buf = smem + (it & 1) * BUF;
+    stage<T, DP, WV>(buf, (const T*)p.q + b * p.qb + h * p.qh, p.qt, first, n, p.D, wave, lane);
+    stage<T, DP, WV>(buf + G::TILE, (const T*)p.dO + ((long)b * p.T * p.H + h) * p.D, (long)p.H * p.D, first, n, p.D, wave, lane);
+    const int i = first + lane;
+    if (wave == 0 && lane < G::BN) {
+      const long s = ((long)b * p.H + h) * p.T + i;
+      hold[0] = i < n ? p.lse[s] : INFINITY;
+      hold[1] = i < n ? p.delta[s] : 0.f;
+    }
+  };
+  auto put = [&](int it) {   // (the row statistics go through registers: written once the tile's reads are on their way)
+    if (wave == 0 && lane < G::BN) {
+      float* st = (float*)(smem + (it & 1) * BUF + 2 * G::TILE);
+      st[lane] = hold[0];
+      st[G::BN + lane] = hold[1];
+    }
+  };
+  if (from < to) fetch(from);
+
+  frag kf[G::KK], vf[G::KK];
+  load_owner<T, DP>((const T*)p.k + b * p.kb + (long)j * p.kt + hk * p.kh, live, p.D, at.lhi, kf);
+  load_owner<T, DP>((const T*)p.v + b * p.vb + (long)j * p.vt + hk * p.vh, live, p.D, at.lhi, vf);
+  // the lane's queries.  window: lo .. hi.  sinks: up to last, outside of lo .. hi
+  int lo = p.causal ? j : j - p.right, hi = j + p.left, last = n - 1;
+  if constexpr (SINK) {
+    if (p.causal) lo = -(1 << 30);
+    if (j >= p.sinks || !live) last = -1;
+  } else {
+    if (hi > n - 1) hi = n - 1;
+    if (!live) hi = lo - 1;
+  }
+
+  f32x16 dk[G::DB], dv[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+
+  if (from < to) {
+    put(from);
+    staged();
+  }
+  for (int it = from; it < to; ++it) {
+    if (it + 1 < to) fetch(it + 1);
+    const char* qb = smem + (it & 1) * BUF;
+    const char* db = qb + G::TILE;
+    const float* st = (const float*)(db + G::TILE);
+    const int first = (t0 + it % nt) * G::BN;
+#pragma unroll
+    for (int y = 0; y < G::NY; ++y) {
+      const int ia = first + 32 * y, ib = ia + 31;   // (wave-uniform tests, as in the other kernel)
+      bool any, all;
+      if constexpr (SINK) {
+        any = jw < p.sinks && jw < n && ia < n && (ib > jw + p.left || (!p.causal && ia < jw + 31 - p.right));
+        all = false;
+      } else {
+        any = jw < n && ia < n && ia <= jw + 31 + p.left && ib >= (p.causal ? jw : jw - p.right);
+        all = jw + 31 < n && ib < n && ib <= jw + p.left && ia >= (p.causal ? jw + 31 : jw + 31 - p.right);
+      }
+      if (!any) continue;
+      f32x16 S, dP;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = dP[r] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < G::KK; ++kk) {
+        S = O::mma(at.rowwise(qb, y, kk), kf[kk], S);
+        dP = O::mma(at.rowwise(db, y, kk), vf[kk], dP);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 l4 = *(const f32x4*)(st + 32 * y + 8 * a + 4 * at.lhi), d4 = *(const f32x4*)(st + G::BN + 32 * y + 8 * a + 4 * at.lhi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * a + e, i = ia + 8 * a + 4 * at.lhi + e;
+          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, -l4[e]));
+          if constexpr (SINK) w = i <= last && (i < lo || i > hi) ? w : 0.f;
+          else if (!all) w = i >= lo && i <= hi ? w : 0.f;
+          S[r] = w;
+          dP[r] = w * (dP[r] - d4[e]);
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const frag w = O::pack(S, 8 * a), z = O::pack(dP, 8 * a);
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d) {
+          dv[d] = O::mma(at.transposed(db, 32 * y + 16 * a, d), w, dv[d]);
+          dk[d] = O::mma(at.transposed(qb, 32 * y + 16 * a, d), z, dk[d]);
+        }
+      }
+    }
+    if (it + 1 < to) put(it + 1);
+    staged();
+  }
+
+  if constexpr (SINK) {
+    // part[bh][chunk][key of the sink tiles][dk, dv][D]
+    float* row = p.part + ((((long)bh * p.chunks + chunk) * p.tiles * (WV * 32) + j) * 2) * p.D;
+    store_owner<float, DP>(row, dk, 1.f, true, p.D, at.lhi);
+    store_owner<float, DP>(row + p.D, dv, 1.f, true, p.D, at.lhi);
+  } else {
+    if (!live) {
+#pragma unroll
+      for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+    }
+    const int sp = (p.sinks + 31) / 32 * 32;
+    if (p.chunks > 0 && jw < sp && live) {   // add what the sink kernel gathered
+      for (int c = 0; c < p.chunks; ++c) {
+        const float* row = p.part + ((((long)bh * p.chunks + c) * sp + j) * 2) * p.D;
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const int dd = 32 * d + 8 * a + 4 * at.lhi;
+            if (dd < p.D) {
+              const f32x4 u = *(const f32x4*)(row + dd), w = *(const f32x4*)(row + p.D + dd);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                dk[d][4 * a + e] += u[e];
+                dv[d][4 * a + e] += w[e];
+              }
+            }
+          }
+      }
+    }
+    const long orow = (((long)b * p.T + j) * p.Hk + hk) * p.D;
+    store_owner<T, DP>((T*)p.dk + orow, dk, p.scale, j < p.T, p.D, at.lhi);
+    store_owner<T, DP>((T*)p.dv + orow, dv, 1.f, j < p.T, p.D, at.lhi);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+template <auto Kernel>
+int launch(const WAttnArgs& p, long groups, int threads, size_t lds, hipStream_t st) {
+  if (groups > 0x7fffffffL) return INDM_E_SHAPE;
+  if (indm_lds_optin<Kernel>(lds) != INDM_OK) return INDM_E_LAUNCH;
+  hipLaunchKernelGGL((*Kernel), dim3((unsigned)groups), dim3(threads), lds, st, p);
+  return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
+}
+
+template <typename T, int DP, int WV, bool BWD>
+int run_query(WAttnArgs p, hipStream_t st) {
+  p.tiles = cdiv(p.T, WV * 32);
+  return launch<wattn_query_kernel<T, DP, WV, BWD>>(p, (long)p.tiles * p.H * p.B, WV * 64, 4 * (size_t)Geo<T, DP>::TILE, st);
+}
+template <typename T, int DP, int WV, bool SINK>
+int run_key(WAttnArgs p, hipStream_t st) {
+  using G = Geo<T, DP>;
+  p.tiles = SINK ? cdiv(p.sinks, 32) : cdiv(p.T, WV * 32);
+  return launch<wattn_key_kernel<T, DP, WV, SINK>>(p, (long)p.tiles * (SINK ? p.chunks : 1) * p.Hk * p.B, WV * 64,
+                                                   2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
+}
+
+// do the sinks reach queries outside of the window?  (sinks are clamped to T before)
+inline bool sinks_matter(int T, int left, int right, int sinks, int causal) {
+  return sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right));
+}
+inline int sink_chunks(int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
+  if (!sinks_matter(T, left, right, sinks, causal)) return 0;
+  const long rows = (long)B * Hk * cdiv(sinks, 32), units = (long)(H / Hk) * cdiv(T, 64);   // of at least one tile each
+  long c = 1024 / rows;
+  c = c < 1 ? 1 : c;
+  return (int)(c < units ? c : units);
+}
+
+#define WA_DISPATCH(CALL)                 \
+  if (p.D <= 32) return CALL(32);         \
+  if (p.D <= 64) return CALL(64);         \
+  if (p.D <= 96) return CALL(96);         \
+  return CALL(128);
+
+template <typename T>
+int check(const WAttnArgs& p, const long* strides) {
+  if (p.B < 0 || p.T < 0 || p.T > (1 << 28) || p.H <= 0 || p.Hk <= 0 || p.H % p.Hk || p.D <= 0 || p.D > 128 || p.D % 8) return INDM_E_SHAPE;
+  if (p.left < 0 || p.right < 0 || p.sinks < 0 || strides == nullptr || !(p.scale > 0.f && p.scale < INFINITY)) return INDM_E_ARG;
+  if (p.B == 0 || p.T == 0) return INDM_OK;
+  if (p.q == nullptr || p.k == nullptr || p.v == nullptr || (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15)) return INDM_E_ARG;
+  for (int i = 0; i < 9; ++i)
+    if (strides[i] % (16 / (long)sizeof(T))) return INDM_E_ARG;
+  return 1;
+}
+WAttnArgs pack_args(const void* q, const void* k, const void* v, const long* s, const int* lengths, int B, int T, int H, int Hk, int D,
+                    int left, int right, int sinks, int causal, float scale) {
+  WAttnArgs p = {};
+  p.q = q; p.k = k; p.v = v; p.lengths = lengths;
+  if (s != nullptr) {
+    p.qb = s[0]; p.qt = s[1]; p.qh = s[2]; p.kb = s[3]; p.kt = s[4]; p.kh = s[5]; p.vb = s[6]; p.vt = s[7]; p.vh = s[8];
+  }
+  p.B = B; p.T = T; p.H = H; p.Hk = Hk; p.D = D; p.causal = causal != 0;
+  p.left = left < T ? left : T; p.right = right < T ? right : T; p.sinks = sinks < T ? sinks : T;   // (no further than T: no overflow)
+  p.scale = scale; p.c = scale * 1.44269504088896340736f;
+  return p;
+}
+
+template <typename T>
+int fwd(WAttnArgs p, const long* strides, void* o, float* lse, hipStream_t st) {
+  const int r = check<T>(p, strides);
+  if (r <= 0) return r;
+  if (o == nullptr || ((uintptr_t)o & 15)) return INDM_E_ARG;
+  p.out = o; p.lse = lse;
+#define WA_FWD(DP) run_query<T, DP, 4, false>(p, st)
+  WA_DISPATCH(WA_FWD)
+}
+
+template <typename T, int DP>
+int bwd_dp(const WAttnArgs& p, hipStream_t st) {
+  int r = run_query<T, DP, 4, true>(p, st);   // dq, and delta for the others
+  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, 1, true>(p, st);
+  if (r == INDM_OK) r = run_key<T, DP, 4, false>(p, st);
+  return r;
+}
+template <typename T>
+int bwd(WAttnArgs p, const long* strides, const void* o, const void* dO, const float* lse, void* dq, void* dk, void* dv, float* ws,
+        hipStream_t st) {
+  const int r = check<T>(p, strides);
+  if (r <= 0) return r;
+  if (o == nullptr || dO == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || ws == nullptr ||
+      (((uintptr_t)o | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
+  p.o = o; p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
+  p.delta = ws;
+  p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
+  p.chunks = sink_chunks(p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
+#define WA_BWD(DP) bwd_dp<T, DP>(p, st)
+  WA_DISPATCH(WA_BWD)
+}
+
+}  // namespace
+
+INDM_API int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, float* lse,
+                                const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal,
+                                float scale, void* stream) {
+  return fwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, lse,
+                    (hipStream_t)stream);
+}
+INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, const long* strides, void* o, float* lse,
+                                 const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal,
+                                 float scale, void* stream) {
+  return fwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, lse,
+                  (hipStream_t)stream);
+}
+
+INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal) {
+  if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
+  sinks = sinks < T ? sinks : T;
+  const long chunks = sink_chunks(B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal);
+  return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * chunks * cdiv(sinks, 32) * 32 * 2 * D;
+}
+INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const float* dO,
+                                const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,
+                                int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream) {
+  return bwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, dO, lse, dq, dk,
+                    dv, ws, (hipStream_t)stream);
+}
+INDM_API int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, const long* strides, const void* o, const void* dO,
+                                 const float* lse, const int* lengths, void* dq, void* dk, void* dv, float* ws, int B, int T, int H,
+                                 int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream) {
+  return bwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, dO, lse, dq, dk, dv,
+                  ws, (hipStream_t)stream);
+}

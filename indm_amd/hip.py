@@ -171,6 +171,11 @@ _SIGS = {
     "indm_dropout_bf16": [c_p, c_p, c_p, c_l, c_f, c_u64, c_p, c_p],
     "indm_rotary_f32": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
     "indm_rotary_bf16": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
+    "indm_wattn_fwd_f32": [c_p] * 7 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_fwd_bf16": [c_p] * 7 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_bwd_ws_floats": [c_i] * 9,
+    "indm_wattn_bwd_f32": [c_p] * 12 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_bwd_bf16": [c_p] * 12 + [c_i] * 9 + [c_f, c_p],
     "indm_timer_create": [c_i, c_p],
     "indm_timer_destroy": [c_p],
     "indm_timer_reset": [c_p, c_i],
@@ -179,7 +184,8 @@ _SIGS = {
 _LONG_RET = {"indm_groupnorm_ws_floats", "indm_colreduce_ws_floats", "indm_segreduce_ws_floats", "indm_rowreduce_ws_floats",
              "indm_dsm_ws_floats", "indm_sqnorm_ws_floats", "indm_ires_bwd_act_ws_floats", "indm_iresblock_ws_floats",
              "indm_pc_step_ws_floats", "indm_hutch_div_ws_floats", "indm_f16_bwd_act_ok", "indm_f16_wgrad_ws_floats",
-             "indm_h16_groupnorm_ws_floats", "indm_h16_segreduce_ws_floats", "indm_layernorm_bwd_ws_floats"}
+             "indm_h16_groupnorm_ws_floats", "indm_h16_segreduce_ws_floats", "indm_layernorm_bwd_ws_floats",
+             "indm_wattn_bwd_ws_floats"}
 
 EXPORTED_SYMBOLS = tuple(sorted(_SIGS))
 
@@ -2186,13 +2192,13 @@ def iresblock_inverse(y, cb, W1, W2T, W3, b1, b2, b3, preact, atol, rtol):
 _TOKEN_DTYPES = {torch.float32: "f32", torch.bfloat16: "bf16"}
 
 
-def _require(ok, what):
-    if not ok:
-        raise RuntimeError("indm_amd: " + what)
+def _refuse(what):
+    raise RuntimeError("indm_amd: " + what)
 
 
 def _token_suffix(op, x):
-    _require(x.dtype in _TOKEN_DTYPES, f"{op}: expected float32 or bfloat16, got {x.dtype}")
+    if x.dtype not in _TOKEN_DTYPES:
+        _refuse(f"{op}: expected float32 or bfloat16, got {x.dtype}")
     return _TOKEN_DTYPES[x.dtype]
 
 
@@ -2203,12 +2209,17 @@ def _token_device(op, *tensors):
         if t is not None:
             if not t.is_cuda:
                 raise RuntimeError("indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback")
-            _require(t.device == dev, f"{op}: tensors on {dev} and {t.device}")
+            if t.device != dev:
+                _refuse(f"{op}: tensors on {dev} and {t.device}")
     return _NO_TIMING if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _data(t):
     return None if t is None else t.data_ptr()
+
+
+def _contig(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _rows2d(x):
@@ -2226,32 +2237,39 @@ def _rows2d(x):
     return x.contiguous(), R, C
 
 
+_LN_MAX_C = {"f32": 16384, "bf16": 32768}
+
+
 def _ln_check(x, gamma, beta):
     suf = _token_suffix("layer_norm", x)
-    _require(x.dim() >= 1 and x.shape[-1] > 0, f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        _refuse(f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
     C = x.shape[-1]
-    most = 16384 if suf == "f32" else 32768
-    _require(C <= most, f"layer_norm: rows of up to {most} {suf} elements, got {C}")
+    if C > _LN_MAX_C[suf]:
+        _refuse(f"layer_norm: rows of up to {_LN_MAX_C[suf]} {suf} elements, got {C}")
     for name, p in (("gamma", gamma), ("beta", beta)):
         if p is not None:
-            _require(p.dtype == torch.float32, f"layer_norm: {name} is float32, got {p.dtype}")
-            _require(tuple(p.shape) == (C,), f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
+            if p.dtype != torch.float32:
+                _refuse(f"layer_norm: {name} is float32, got {p.dtype}")
+            if p.shape != (C,):
+                _refuse(f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
     return suf
 
 
 def layernorm_fwd(x, gamma=None, beta=None, eps=1e-6, stats=True):
     """x [..., C] -> y, mean [R], rstd [R] (None, None without stats)"""
     suf = _ln_check(x, gamma, beta)
-    _require(eps >= 0.0, f"layer_norm: eps >= 0, got {eps}")
+    if not eps >= 0.0:
+        _refuse(f"layer_norm: eps >= 0, got {eps}")
     with _token_device("layer_norm", x, gamma, beta):
-        gamma = gamma if gamma is None or gamma.is_contiguous() else gamma.contiguous()
-        beta = beta if beta is None or beta.is_contiguous() else beta.contiguous()
+        gamma, beta = _contig(gamma), _contig(beta)
         xr, R, ldx = _rows2d(x)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = torch.empty((R,), dtype=torch.float32, device=x.device) if stats else None
-        rstd = torch.empty_like(mean) if stats else None
-        st = getattr(lib(), "indm_layernorm_fwd_" + suf)(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean),
-                                                         _data(rstd), R, x.shape[-1], eps, _stream())
+        mean = rstd = None
+        if stats:
+            mean, rstd = torch.empty((2, R), dtype=torch.float32, device=x.device).unbind(0)
+        fn = lib().indm_layernorm_fwd_f32 if suf == "f32" else lib().indm_layernorm_fwd_bf16
+        st = fn(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean), _data(rstd), R, x.shape[-1], eps, _stream())
         _chk(st, "indm_layernorm_fwd_" + suf)
     return y, mean, rstd
 
@@ -2260,11 +2278,11 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, want_gamma=True, want_beta=True):
     """-> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its own: calls on different
     streams, or in different captured graphs, share nothing."""
     suf = _ln_check(x, gamma, None)
-    _require(dy.dtype == x.dtype and dy.shape == x.shape, f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    if dy.dtype != x.dtype or dy.shape != x.shape:
+        _refuse(f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     with _token_device("layer_norm", x, dy, gamma, mean, rstd):
         C = x.shape[-1]
-        gamma = gamma if gamma is None or gamma.is_contiguous() else gamma.contiguous()
-        dy = dy if dy.is_contiguous() else dy.contiguous()
+        gamma, dy = _contig(gamma), _contig(dy)
         xr, R, ldx = _rows2d(x)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dgamma = torch.empty((C,), dtype=torch.float32, device=x.device) if want_gamma else None
@@ -2272,8 +2290,9 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, want_gamma=True, want_beta=True):
         ws = None
         if want_gamma or want_beta:
             ws = torch.empty((max(1, lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size())),), dtype=torch.float32, device=x.device)
-        st = getattr(lib(), "indm_layernorm_bwd_" + suf)(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean.data_ptr(), rstd.data_ptr(),
-                                                         dx.data_ptr(), _data(dgamma), _data(dbeta), _data(ws), R, C, _stream())
+        fn = lib().indm_layernorm_bwd_f32 if suf == "f32" else lib().indm_layernorm_bwd_bf16
+        st = fn(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _data(dgamma),
+                _data(dbeta), _data(ws), R, C, _stream())
         _chk(st, "indm_layernorm_bwd_" + suf)
     return dx, dgamma, dbeta
 
@@ -2281,46 +2300,41 @@ def layernorm_bwd(dy, x, gamma, mean, rstd, want_gamma=True, want_beta=True):
 def dropout(x, p, seed, res=None, seed_dev=None):
     """(res) + keep(seed + *seed_dev) x / (1 - p), the mask by x's dense (row-major) element index"""
     suf = _token_suffix("dropout", x)
-    p = float(p)
-    _require(0.0 <= p <= 1.0, f"dropout: 0 <= p <= 1, got {p}")
-    _require(0 <= int(seed) < 1 << 64, f"dropout: the seed is a whole number of 64 bits, got {seed}")
-    if res is not None:
-        _require(res.shape == x.shape and res.dtype == x.dtype, f"dropout: res is {tuple(x.shape)} {x.dtype}, got {tuple(res.shape)} {res.dtype}")
-    if seed_dev is not None:
-        _require(seed_dev.dtype == torch.int64 and seed_dev.numel() == 1, "dropout: seed_dev is one int64 on the device")
+    if not 0.0 <= p <= 1.0:
+        _refuse(f"dropout: 0 <= p <= 1, got {p}")
+    if not 0 <= seed < 1 << 64:
+        _refuse(f"dropout: the seed is a whole number of 64 bits, got {seed}")
+    if res is not None and (res.shape != x.shape or res.dtype != x.dtype):
+        _refuse(f"dropout: res is {tuple(x.shape)} {x.dtype}, got {tuple(res.shape)} {res.dtype}")
+    if seed_dev is not None and (seed_dev.dtype != torch.int64 or seed_dev.numel() != 1):
+        _refuse("dropout: seed_dev is one int64 on the device")
     with _token_device("dropout", x, res, seed_dev):
-        x = x if x.is_contiguous() else x.contiguous()
-        res = res if res is None or res.is_contiguous() else res.contiguous()
+        x, res = _contig(x), _contig(res)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        st = getattr(lib(), "indm_dropout_" + suf)(x.data_ptr(), _data(res), y.data_ptr(), x.numel(), p, int(seed), _seed_ptr(seed_dev),
-                                                   _stream())
-        _chk(st, "indm_dropout_" + suf)
+        fn = lib().indm_dropout_f32 if suf == "f32" else lib().indm_dropout_bf16
+        _chk(fn(x.data_ptr(), _data(res), y.data_ptr(), x.numel(), p, seed, _seed_ptr(seed_dev), _stream()), "indm_dropout_" + suf)
     return y
 
 
 _POS_TYPES = {torch.int32: 0, torch.float32: 1, torch.int64: 2}
 
 
-def _heads_strides(x):
-    """x [B, T, H, D] with D contiguous (a copy where it is not) and its B, T, H strides"""
-    x = x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-    return x, x.stride()[:3]
-
-
 def _rotary_check(q, k, pos, freqs, sections):
     suf = _token_suffix("rotary", q)
-    _require(q.dim() == 4, f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
+    if q.dim() != 4:
+        _refuse(f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
     B, T, _, D = q.shape
-    if k is not None:
-        _require(k.dtype == q.dtype and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D,
-                 f"rotary: k is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
-    A = len(sections)
-    _require(1 <= A <= 8 and all(int(n) == n and n > 0 and n % 2 == 0 for n in sections) and sum(sections) <= D,
-             f"rotary: sections are 1 to 8 even positive numbers that sum to {D} at most, got {tuple(sections)}")
-    _require(pos.dtype in _POS_TYPES, f"rotary: positions are int32, int64 or float32, got {pos.dtype}")
-    _require(tuple(pos.shape) in ((T, A), (B, T, A)), f"rotary: pos is [{T}, {A}] or [{B}, {T}, {A}], got {tuple(pos.shape)}")
-    _require(freqs.dtype == torch.float64 and tuple(freqs.shape) == (sum(sections) // 2,),
-             f"rotary: freqs is float64 [{sum(sections) // 2}], got {tuple(freqs.shape)} {freqs.dtype}")
+    if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D):
+        _refuse(f"rotary: k is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
+    A, R = len(sections), sum(sections)
+    if not 1 <= A <= 8 or R > D or any(n < 2 or n % 2 for n in sections):
+        _refuse(f"rotary: sections are 1 to 8 even positive numbers that sum to {D} at most, got {tuple(sections)}")
+    if pos.dtype not in _POS_TYPES:
+        _refuse(f"rotary: positions are int32, int64 or float32, got {pos.dtype}")
+    if pos.shape != (T, A) and pos.shape != (B, T, A):
+        _refuse(f"rotary: pos is [{T}, {A}] or [{B}, {T}, {A}], got {tuple(pos.shape)}")
+    if freqs.dtype != torch.float64 or freqs.shape != (R // 2,):
+        _refuse(f"rotary: freqs is float64 [{R // 2}], got {tuple(freqs.shape)} {freqs.dtype}")
     return suf
 
 
@@ -2329,19 +2343,87 @@ def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
     suf = _rotary_check(q, k, pos, freqs, sections)
     with _token_device("rotary", q, k, pos, freqs):
         B, T, H, D = q.shape
-        Hk = 0 if k is None else k.shape[2]
-        q, sq = _heads_strides(q)
-        sk = (0, 0, 0)
-        yk = None
+        Hk, sk, yk = 0, (0, 0, 0), None
+        q = q if q.stride(3) == 1 or D == 1 else q.contiguous()
         if k is not None:
-            k, sk = _heads_strides(k)
+            k = k if k.stride(3) == 1 or D == 1 else k.contiguous()
+            Hk, sk = k.shape[2], k.stride()[:3]
             yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        pos = pos if pos.is_contiguous() else pos.contiguous()
-        freqs = freqs if freqs.is_contiguous() else freqs.contiguous()
-        st = getattr(lib(), "indm_rotary_" + suf)(q.data_ptr(), _data(k), yq.data_ptr(), _data(yk), (c_l * 6)(*sq, *sk), B, T, H, Hk, D,
-                                                  pos.data_ptr(), _POS_TYPES[pos.dtype], T * len(sections) if pos.dim() == 3 else 0,
-                                                  freqs.data_ptr(), (c_i * len(sections))(*[int(n) for n in sections]), len(sections),
-                                                  int(bool(interleaved)), int(bool(inverse)), _stream())
+        pos, freqs, A = _contig(pos), _contig(freqs), len(sections)
+        fn = lib().indm_rotary_f32 if suf == "f32" else lib().indm_rotary_bf16
+        st = fn(q.data_ptr(), _data(k), yq.data_ptr(), _data(yk), (c_l * 6)(*q.stride()[:3], *sk), B, T, H, Hk, D, pos.data_ptr(),
+                _POS_TYPES[pos.dtype], T * A if pos.dim() == 3 else 0, freqs.data_ptr(), (c_i * A)(*sections), A, int(interleaved),
+                int(inverse), _stream())
         _chk(st, "indm_rotary_" + suf)
     return yq, yk
+
+
+def _aligned_rows(x):
+    """x [B, T, heads, D] with D contiguous and every row on 16 bytes; a copy where it is not so"""
+    s, e = x.stride(), 16 // x.element_size()
+    if s[3] == 1 and s[0] % e == 0 and s[1] % e == 0 and s[2] % e == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
+    suf = _token_suffix("window_attention", q)
+    if q.dim() != 4:
+        _refuse(f"window_attention: q is [B, T, H, D], got {tuple(q.shape)}")
+    B, T, H, D = q.shape
+    for name, x in (("k", k), ("v", v)):
+        if x.dtype != q.dtype or x.dim() != 4 or x.shape[:2] != q.shape[:2] or x.shape[3] != D or x.shape != k.shape:
+            _refuse(f"window_attention: {name} is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(x.shape)} {x.dtype}")
+    Hk = k.shape[2]
+    if H < 1 or Hk < 1 or H % Hk:
+        _refuse(f"window_attention: the {H} heads of q are a multiple of the {Hk} of k and v")
+    if D % 8 or not 8 <= D <= 128:
+        _refuse(f"window_attention: heads of 8, 16, ... 128 entries, got {D}")
+    if T > 1 << 28:
+        _refuse(f"window_attention: up to {1 << 28} tokens, got {T}")
+    if left < 0 or right < 0 or sinks < 0:
+        _refuse(f"window_attention: window and sinks >= 0, got ({left}, {right}), {sinks}")
+    if not 0.0 < scale < float("inf"):
+        _refuse(f"window_attention: scale > 0, got {scale}")
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
+        _refuse(f"window_attention: lengths is int32 [{B}], got {tuple(lengths.shape)} {lengths.dtype}")
+    return suf
+
+
+def wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats=True):
+    """-> o [B, T, H, D], lse [B, H, T] (None without stats), q, k, v as the kernel read them (copies where rows were not on 16 bytes)"""
+    suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
+    with _token_device("window_attention", q, k, v, lengths):
+        q, k, v, lengths = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v), _contig(lengths)
+        B, T, H, D = q.shape
+        o = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device) if stats else None
+        fn = lib().indm_wattn_fwd_f32 if suf == "f32" else lib().indm_wattn_fwd_bf16
+        st = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), o.data_ptr(),
+                _data(lse), _data(lengths), B, T, H, k.shape[2], D, min(left, T), min(right, T), min(sinks, T), int(causal), scale, _stream())
+        _chk(st, "indm_wattn_fwd_" + suf)
+    return o, lse, q, k, v
+
+
+def wattn_bwd(q, k, v, o, lse, do, left, right, sinks, causal, lengths, scale):
+    """-> dq, dk, dv (dense).  q, k, v, o, lse: wattn_fwd's.  The scratch is an allocation of its own."""
+    suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
+    if do.dtype != q.dtype or do.shape != q.shape:
+        _refuse(f"window_attention: do is {tuple(q.shape)} {q.dtype}, got {tuple(do.shape)} {do.dtype}")
+    with _token_device("window_attention", q, k, v, o, lse, do, lengths):
+        do, lengths = _contig(do), _contig(lengths)
+        if do.data_ptr() % 16:
+            do = do.clone()
+        B, T, H, D = q.shape
+        Hk, left, right, sinks = k.shape[2], min(left, T), min(right, T), min(sinks, T)
+        dq = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        ws = torch.empty((max(1, lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, int(causal))),), dtype=torch.float32,
+                         device=q.device)
+        fn = lib().indm_wattn_bwd_f32 if suf == "f32" else lib().indm_wattn_bwd_bf16
+        st = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), o.data_ptr(),
+                do.data_ptr(), lse.data_ptr(), _data(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H, Hk, D,
+                left, right, sinks, int(causal), scale, _stream())
+        _chk(st, "indm_wattn_bwd_" + suf)
+    return dq, dk, dv

@@ -1052,4 +1052,36 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     return _Rotary.apply(q, k, pos, freqs, tuple(int(n) for n in sections), bool(interleaved))
 
 
+class _WindowAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, left, right, sinks, causal, lengths, scale):
+        o, lse, q, k, v = hip.wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale)
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.cfg = (left, right, sinks, causal, scale)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        left, right, sinks, causal, scale = ctx.cfg
+        dq, dk, dv = hip.wattn_bwd(q, k, v, o, lse, do, left, right, sinks, causal, lengths, scale)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, scale=None):
+    """Attention over tokens with a sliding window and a few first tokens that stay visible: o [B, T, H, D] of q [B, T, H, D] and
+    k, v [B, T, Hk, D] (H a multiple of Hk: groups of heads share a key head; fp32 or bf16, any strides, D a multiple of 8 up to 128).
+    Token j is visible to token i when i - left <= j <= i + right or j < sinks, and, if causal, j <= i.  window: (left, right), one
+    number for both sides, or None; None for a side: no limit.  lengths: int32 [B], tokens from lengths[b] on belong to no sequence --
+    they are visible to nobody, whatever they hold, and their rows of o and of the gradients are zeros.  scale: default D ** -0.5."""
+    left, right = window if isinstance(window, (tuple, list)) else (window, window)
+    far = q.shape[1] if q.dim() > 1 else 0
+    left, right = far if left is None else int(left), far if right is None else int(right)
+    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
+    if not _tracked(q, k, v):
+        return hip.wattn_fwd(q, k, v, left, right, int(sinks), bool(causal), lengths, scale, stats=False)[0]
+    return _WindowAttention.apply(q, k, v, left, right, int(sinks), bool(causal), lengths, scale)
+
+
 INV_SQRT2 = 1.0 / math.sqrt(2.0)
