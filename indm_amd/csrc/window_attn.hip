@@ -38,6 +38,7 @@ struct WAttnArgs {
   const void *q, *k, *v;            // [B, T, heads, D], D contiguous, 16-byte rows; strides in elements
   long qb, qt, qh, kb, kt, kh, vb, vt, vh;
   const void *o, *dO;               // dense [B, T, H, D] (backward)
+  void* olo;                        // bf16: what rounding o left, rounded itself (written by the forward pass, read by the backward), or NULL
   void *out, *dq, *dk, *dv;         // dense
   float* lse;                       // [B, H, T]: log2 of the sum of exponentials, in units of the exp2 argument
   float* delta;                     // [B, H, T]: <dO, o>
@@ -46,6 +47,8 @@ struct WAttnArgs {
   int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks;
   float c, scale;                   // scale * log2(e), scale
 };
+
+constexpr long MAX_STRIDE = 1 << 22;   // elements between tokens: a tile's byte offsets stay below 2^31
 
 constexpr int pow2_ceil(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
@@ -63,6 +66,12 @@ struct Geo {
     return NCH == 4 ? (r >> 2) & 3 : NCH == 8 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
   }
 };
+
+// wavefronts a SIMD that the register allocation aims at (kind 0: forward, 1: dq, 2: dk / dv).  512 registers a SIMD lane over 4, 3, 2 or
+// 1: what fits without spilling
+constexpr int waves_per_simd(int size, int DP, int kind) {
+  return size == 2 ? (DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : 2) : DP <= 32 ? 3 : DP <= 64 ? (kind == 0 ? 3 : 2) : DP <= 96 && kind == 0 ? 2 : 1;
+}
 
 template <typename T> struct Op;
 template <> struct Op<u16> {
@@ -174,23 +183,41 @@ struct Lane {
 };
 
 // rows first .. first + BN - 1 of a head -> a tile in LDS, by direct copies of 16 bytes a lane (1 KB a wave-instruction, the swizzle is
-// on the source side).  Rows from n on and chunks from D on read zeros: what lies behind a sequence never enters a product.
+// on the source side).  A whole tile of whole rows needs no vector arithmetic in the loop: a scalar base plus the lane's byte offsets,
+// which are computed once (the swizzle repeats every 16 rows: PER of them).  Otherwise rows from n on and chunks from D on read
+// zeros: what lies behind a sequence never enters a product.
 template <typename T, int DP, int WV>
-__device__ __forceinline__ void stage(char* tile, const T* src, long stride, int first, int n, int D, int wave, int lane) {
+struct Stager {
   using G = Geo<T, DP>;
-  constexpr int COPIES = G::BN * G::NCH / 64;
+  static constexpr int COPIES = G::BN * G::NCH / 64, N = (COPIES + WV - 1) / WV;
+  static constexpr int R = WV * 64 / G::NCH;                  // rows from one of a wavefront's copies to its next
+  static constexpr int PER = R >= 16 ? 1 : 16 / R < N ? 16 / R : N;
+  unsigned off[PER];
+  __device__ __forceinline__ Stager(long stride, int wave, int lane) {
 #pragma unroll
-  for (int i = 0; i < (COPIES + WV - 1) / WV; ++i) {
-    const int w = wave + i * WV;
-    if (COPIES % WV == 0 || w < COPIES) {
-      const int slot = w * 64 + lane, r = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(r);
-      const bool in = first + r < n && c * G::EPC < D;
-      const void* s = in ? (const void*)(src + (long)(first + r) * stride + c * G::EPC) : (const void*)zero16;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
-                                       (__attribute__((address_space(3))) void*)(tile + w * 1024), 16, 0, 0);
+    for (int i = 0; i < PER; ++i) {
+      const int slot = (wave + i * WV) * 64 + lane, r = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(r);
+      off[i] = (unsigned)(r * (int)stride + c * G::EPC) * (unsigned)sizeof(T);   // (the host keeps strides up to 2^22 elements)
     }
   }
-}
+  __device__ __forceinline__ void fetch(char* tile, const T* src, long stride, int first, int n, int D, int wave, int lane) const {
+    const bool whole = first + G::BN <= n && D == DP && G::CH == G::NCH;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int w = wave + i * WV;
+      if (COPIES % WV == 0 || w < COPIES) {
+        char* dst = tile + w * 1024;
+        const char* s = (const char*)(src + (long)(first + i / PER * (PER * R)) * stride) + off[i % PER];
+        if (!whole) {
+          const int slot = w * 64 + lane, r = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(r);
+          if (!(first + r < n && c * G::EPC < D)) s = (const char*)zero16;
+        }
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)s,
+                                         (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+      }
+    }
+  }
+};
 __device__ __forceinline__ void staged() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -274,7 +301,7 @@ __device__ __forceinline__ KeyTiles key_tiles(const WAttnArgs& p, int q0, int q1
 
 // ---------------------------------------------------------------------------------------------- owner = queries: forward, dq
 template <typename T, int DP, int WV, bool BWD>
-__global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0)) void wattn_query_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
@@ -292,10 +319,11 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
   const bool live = i < n;
   const KeyTiles kt = key_tiles(p, q0, q0 + WV * 32 - 1, n, G::BN);
   auto first_of = [&](int it) { return (it < kt.ns ? it : kt.t0 + it - kt.ns) * G::BN; };
+  const Stager<T, DP, WV> ks(p.kt, wave, lane), vs(p.vt, wave, lane);
   auto fetch = [&](int it) {
     char* buf = smem + (it & 1) * 2 * G::TILE;
-    stage<T, DP, WV>(buf, K, p.kt, first_of(it), n, p.D, wave, lane);
-    stage<T, DP, WV>(buf + G::TILE, V, p.vt, first_of(it), n, p.D, wave, lane);
+    ks.fetch(buf, K, p.kt, first_of(it), n, p.D, wave, lane);
+    vs.fetch(buf + G::TILE, V, p.vt, first_of(it), n, p.D, wave, lane);
   };
   if (kt.count > 0) fetch(0);
 
@@ -310,18 +338,26 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
     for (int kk = 0; kk < G::KK; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta += O::get(df[kk], e) * O::get(of[kk], e);
+    if (sizeof(T) == 2 && p.olo != nullptr) {
+      load_owner<T, DP>((const T*)p.olo + orow, live, p.D, at.lhi, of);
+#pragma unroll
+      for (int kk = 0; kk < G::KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta += O::get(df[kk], e) * O::get(of[kk], e);
+    }
     delta = half_sum(delta);
     if (live) lse = p.lse[srow];
     if (i < p.T && at.lhi == 0) p.delta[srow] = delta;
   }
-  // the lane's visible keys: lo .. hi, and those below sk
-  const int lo = i - p.left;
-  int hi = p.causal ? i : i + p.right, sk = p.sinks;
+  // the lane's visible keys: lo .. lo + span, and those below sk (a row behind the sequence: none)
+  int lo = i - p.left, hi = p.causal ? i : i + p.right, sk = p.sinks;
   if (hi > n - 1) hi = n - 1;
   if (p.causal && sk > i + 1) sk = i + 1;
   if (sk > n) sk = n;
+  unsigned span = (unsigned)(hi - lo);
   if (!live) {
-    hi = lo - 1;
+    lo = 0x7fffffff;
+    span = 0;
     sk = 0;
   }
 
@@ -338,37 +374,39 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
     if (it + 1 < kt.count) fetch(it + 1);
     const char* kb = smem + (it & 1) * 2 * G::TILE;
     const char* vb = kb + G::TILE;
-    const int k0 = first_of(it), k1 = k0 + G::BN - 1;
-    // (wave-uniform) does any of this wavefront's queries see any of the tile's keys?  all of all?
-    const bool any = qa < n && k0 < n && (k0 < p.sinks || (k1 >= qa - p.left && (p.causal || k0 <= qb + p.right))) && (!p.causal || k0 <= qb);
-    const bool all = k1 < n && (k1 < p.sinks || (k0 >= qa + 31 - p.left && (p.causal || k1 <= qa + p.right))) && (!p.causal || k1 <= qa);
-    if (any) {
-      f32x16 S[G::NY];
 #pragma unroll
-      for (int y = 0; y < G::NY; ++y)
+    for (int y = 0; y < G::NY; ++y) {
+      const int k0 = first_of(it) + 32 * y, k1 = k0 + 31;
+      // (wave-uniform) does any of this wavefront's queries see any of these 32 keys?  all of all?
+      const bool any = qa < n && k0 < n && (k0 < p.sinks || (k1 >= qa - p.left && (p.causal || k0 <= qb + p.right))) && (!p.causal || k0 <= qb);
+      const bool all = qa + 31 < n && k1 < n && (k1 < p.sinks || (k0 >= qa + 31 - p.left && (p.causal || k1 <= qa + p.right))) && (!p.causal || k1 <= qa);
+      if (!any) continue;
+      f32x16 S;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) S[y][r] = 0.f;
+      for (int r = 0; r < 16; ++r) S[r] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < G::KK; ++kk)
-#pragma unroll
-        for (int y = 0; y < G::NY; ++y) S[y] = O::mma(at.rowwise(kb, y, kk), qf[kk], S[y]);
+      for (int kk = 0; kk < G::KK; ++kk) S = O::mma(at.rowwise(kb, y, kk), qf[kk], S);
       if (!all) {
-#pragma unroll
-        for (int y = 0; y < G::NY; ++y)
+        const unsigned from = (unsigned)(k0 + 4 * at.lhi - lo);
+        if (k0 < p.sinks) {
+          const int left = sk - k0 - 4 * at.lhi;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int j = k0 + 32 * y + 8 * (r >> 2) + (r & 3) + 4 * at.lhi;
-            S[y][r] = (j >= lo && j <= hi) || j < sk ? S[y][r] : -INFINITY;
+            const int j = 8 * (r >> 2) + (r & 3);
+            S[r] = from + j <= span || j < left ? S[r] : -INFINITY;
           }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[r] = from + 8 * (r >> 2) + (r & 3) <= span ? S[r] : -INFINITY;
+        }
       }
       if constexpr (!BWD) {
-        float top = S[0][0];
+        float top = S[0];
 #pragma unroll
-        for (int y = 0; y < G::NY; ++y)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, S[y][r]);
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
         top = half_max(top) * p.c;
         if (__any(top > m + 8.f)) {   // (-inf + 8 = -inf: the first visible key always raises it)
+          asm volatile("" ::: "memory");   // (keeps the rescaling behind the branch)
           const float up = fmaxf(m, top);
           const float f = up > -INFINITY ? __builtin_amdgcn_exp2f(m - up) : 1.f;
           m = up;
@@ -380,34 +418,27 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
         }
         const float mm = m > -INFINITY ? m : 0.f;
 #pragma unroll
-        for (int y = 0; y < G::NY; ++y)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            S[y][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[y][r], p.c, -mm));
-            sum += S[y][r];
-          }
-      } else {
-#pragma unroll
-        for (int y = 0; y < G::NY; ++y) {
-          f32x16 dP;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dP[r] = 0.f;
-#pragma unroll
-          for (int kk = 0; kk < G::KK; ++kk) dP = O::mma(at.rowwise(vb, y, kk), df[kk], dP);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            S[y][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[y][r], p.c, -lse)) * (dP[r] - delta);   // dS / scale
+        for (int r = 0; r < 16; ++r) {
+          S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, -mm));
+          sum += S[r];
         }
+      } else {
+        f32x16 dP;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dP[r] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < G::KK; ++kk) dP = O::mma(at.rowwise(vb, y, kk), df[kk], dP);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, -lse)) * (dP[r] - delta);   // dS / scale
       }
       const char* zb = BWD ? kb : vb;
 #pragma unroll
-      for (int y = 0; y < G::NY; ++y)
+      for (int a = 0; a < 2; ++a) {
+        const frag w = O::pack(S, 8 * a);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const frag w = O::pack(S[y], 8 * a);
-#pragma unroll
-          for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
-        }
+        for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
+      }
     }
     staged();
   }
@@ -422,6 +453,18 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
     sum = half_sum(sum);
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     store_owner<T, DP>((T*)p.out + orow, acc, inv, i < p.T, p.D, at.lhi);
+    if constexpr (sizeof(T) == 2) {
+      if (p.olo != nullptr) {
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float v = acc[d][r] * inv;
+            acc[d][r] = v - (float)(__bf16)v;
+          }
+        store_owner<T, DP>((T*)p.olo + orow, acc, 1.f, i < p.T, p.D, at.lhi);
+      }
+    }
     if (p.lse != nullptr && i < p.T && at.lhi == 0) p.lse[srow] = live ? m + __log2f(sum) : INFINITY;
   } else {
     store_owner<T, DP>((T*)p.dq + orow, acc, p.scale, i < p.T, p.D, at.lhi);
@@ -433,7 +476,7 @@ __global__ __launch_bounds__(WV * 64) void wattn_query_kernel(WAttnArgs p) {
 // keys get from queries whose window they are outside of -- a few keys against all queries, so the queries are split over p.chunks
 // workgroups whose fp32 partial sums the first kind adds up in order (no atomics).
 template <typename T, int DP, int WV, bool SINK>
-__global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wattn_key_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
@@ -465,12 +508,13 @@ __global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
     from = (int)((long)to * chunk / p.chunks);
     to = (int)((long)to * (chunk + 1) / p.chunks);
   }
+  const Stager<T, DP, WV> qs(p.qt, wave, lane), ds((long)p.H * p.D, wave, lane);
   float hold[2];
   auto fetch = [&](int it) {
     const int h = hk * group + it / nt, first = (t0 + it % nt) * G::BN;
     char* buf = smem + (it & 1) * BUF;
-    stage<T, DP, WV>(buf, (const T*)p.q + b * p.qb + h * p.qh, p.qt, first, n, p.D, wave, lane);
-    stage<T, DP, WV>(buf + G::TILE, (const T*)p.dO + ((long)b * p.T * p.H + h) * p.D, (long)p.H * p.D, first, n, p.D, wave, lane);
+    qs.fetch(buf, (const T*)p.q + b * p.qb + h * p.qh, p.qt, first, n, p.D, wave, lane);
+    ds.fetch(buf + G::TILE, (const T*)p.dO + ((long)b * p.T * p.H + h) * p.D, (long)p.H * p.D, first, n, p.D, wave, lane);
     const int i = first + lane;
     if (wave == 0 && lane < G::BN) {
       const long s = ((long)b * p.H + h) * p.T + i;
@@ -497,8 +541,12 @@ __global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
     if (j >= p.sinks || !live) last = -1;
   } else {
     if (hi > n - 1) hi = n - 1;
-    if (!live) hi = lo - 1;
+    if (!live) {
+      lo = 0x7fffffff;
+      hi = lo;
+    }
   }
+  const unsigned span = (unsigned)(hi - lo);
 
   f32x16 dk[G::DB], dv[G::DB];
 #pragma unroll
@@ -528,35 +576,43 @@ __global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
         all = jw + 31 < n && ib < n && ib <= jw + p.left && ia >= (p.causal ? jw + 31 : jw + 31 - p.right);
       }
       if (!any) continue;
-      f32x16 S, dP;
+      f32x16 P, dP;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[r] = dP[r] = 0.f;
+      for (int r = 0; r < 16; ++r) P[r] = dP[r] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < G::KK; ++kk) {
-        S = O::mma(at.rowwise(qb, y, kk), kf[kk], S);
-        dP = O::mma(at.rowwise(db, y, kk), vf[kk], dP);
-      }
+      for (int kk = 0; kk < G::KK; ++kk) P = O::mma(at.rowwise(qb, y, kk), kf[kk], P);
+      const unsigned at0 = (unsigned)(ia + 4 * at.lhi - lo);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const f32x4 l4 = *(const f32x4*)(st + 32 * y + 8 * a + 4 * at.lhi), d4 = *(const f32x4*)(st + G::BN + 32 * y + 8 * a + 4 * at.lhi);
+        const f32x4 l4 = *(const f32x4*)(st + 32 * y + 8 * a + 4 * at.lhi);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * a + e, i = ia + 8 * a + 4 * at.lhi + e;
-          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, -l4[e]));
-          if constexpr (SINK) w = i <= last && (i < lo || i > hi) ? w : 0.f;
-          else if (!all) w = i >= lo && i <= hi ? w : 0.f;
-          S[r] = w;
-          dP[r] = w * (dP[r] - d4[e]);
+          const int r = 4 * a + e;
+          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r], p.c, -l4[e]));
+          if constexpr (SINK) w = ia + 4 * at.lhi + 8 * a + e <= last && at0 + 8 * a + e > span ? w : 0.f;
+          else if (!all) w = at0 + 8 * a + e <= span ? w : 0.f;
+          P[r] = w;
         }
       }
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        const frag w = O::pack(S, 8 * a), z = O::pack(dP, 8 * a);
+        const frag w = O::pack(P, 8 * a);
 #pragma unroll
-        for (int d = 0; d < G::DB; ++d) {
-          dv[d] = O::mma(at.transposed(db, 32 * y + 16 * a, d), w, dv[d]);
-          dk[d] = O::mma(at.transposed(qb, 32 * y + 16 * a, d), z, dk[d]);
-        }
+        for (int d = 0; d < G::DB; ++d) dv[d] = O::mma(at.transposed(db, 32 * y + 16 * a, d), w, dv[d]);
+      }
+#pragma unroll
+      for (int kk = 0; kk < G::KK; ++kk) dP = O::mma(at.rowwise(db, y, kk), vf[kk], dP);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 d4 = *(const f32x4*)(st + G::BN + 32 * y + 8 * a + 4 * at.lhi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) P[4 * a + e] *= dP[4 * a + e] - d4[e];
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const frag w = O::pack(P, 8 * a);
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d) dk[d] = O::mma(at.transposed(qb, 32 * y + 16 * a, d), w, dk[d]);
       }
     }
     if (it + 1 < to) put(it + 1);
@@ -577,28 +633,40 @@ __global__ __launch_bounds__(WV * 64) void wattn_key_kernel(WAttnArgs p) {
     }
     const int sp = (p.sinks + 31) / 32 * 32;
     if (p.chunks > 0 && jw < sp && live) {   // add what the sink kernel gathered
-      for (int c = 0; c < p.chunks; ++c) {
-        const float* row = p.part + ((((long)bh * p.chunks + c) * sp + j) * 2) * p.D;
+      const float* row = p.part + ((long)bh * p.chunks * sp + j) * 2 * p.D;
 #pragma unroll
-        for (int d = 0; d < G::DB; ++d)
+      for (int d = 0; d < G::DB; ++d)
 #pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const int dd = 32 * d + 8 * a + 4 * at.lhi;
-            if (dd < p.D) {
-              const f32x4 u = *(const f32x4*)(row + dd), w = *(const f32x4*)(row + p.D + dd);
+        for (int a = 0; a < 4; ++a) {
+          const int dd = 32 * d + 8 * a + 4 * at.lhi;
+          if (dd < p.D) {
+            const f32x4 u = *(const f32x4*)(row + dd), w = *(const f32x4*)(row + p.D + dd);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                dk[d][4 * a + e] += u[e];
-                dv[d][4 * a + e] += w[e];
-              }
+            for (int e = 0; e < 4; ++e) {
+              dk[d][4 * a + e] += u[e];
+              dv[d][4 * a + e] += w[e];
             }
           }
-      }
+        }
     }
     const long orow = (((long)b * p.T + j) * p.Hk + hk) * p.D;
     store_owner<T, DP>((T*)p.dk + orow, dk, p.scale, j < p.T, p.D, at.lhi);
     store_owner<T, DP>((T*)p.dv + orow, dv, 1.f, j < p.T, p.D, at.lhi);
   }
+}
+
+// the sink partials of each (sequence, key head) added up over the chunks, in order, into chunk 0: a workgroup's lanes own 64 columns
+// of the n = key blocks x 2 D values, its wavefronts a quarter of the chunks each
+__global__ __launch_bounds__(256) void wattn_join_kernel(float* part, int chunks, int n) {
+  __shared__ float sh[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;   // (n is a multiple of 64 x 8)
+  float* base = part + (long)blockIdx.y * chunks * n + col;
+  float s = 0.f;
+#pragma unroll 4
+  for (int c = chunks * wave / 4; c < chunks * (wave + 1) / 4; ++c) s += base[(long)c * n];
+  sh[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0) base[0] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -621,6 +689,13 @@ int run_key(WAttnArgs p, hipStream_t st) {
   p.tiles = SINK ? cdiv(p.sinks, 32) : cdiv(p.T, WV * 32);
   return launch<wattn_key_kernel<T, DP, WV, SINK>>(p, (long)p.tiles * (SINK ? p.chunks : 1) * p.Hk * p.B, WV * 64,
                                                    2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
+}
+
+inline int run_join(const WAttnArgs& p, hipStream_t st) {
+  const int n = cdiv(p.sinks, 32) * 64 * p.D;
+  if ((long)p.B * p.Hk > 65535) return INDM_E_SHAPE;
+  hipLaunchKernelGGL(wattn_join_kernel, dim3(n / 64, p.B * p.Hk), dim3(256), 0, st, p.part, p.chunks, n);
+  return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
 // do the sinks reach queries outside of the window?  (sinks are clamped to T before)
@@ -648,7 +723,8 @@ int check(const WAttnArgs& p, const long* strides) {
   if (p.B == 0 || p.T == 0) return INDM_OK;
   if (p.q == nullptr || p.k == nullptr || p.v == nullptr || (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15)) return INDM_E_ARG;
   for (int i = 0; i < 9; ++i)
-    if (strides[i] % (16 / (long)sizeof(T))) return INDM_E_ARG;
+    if (strides[i] < 0 || strides[i] % (16 / (long)sizeof(T))) return INDM_E_ARG;
+  if (p.qt > MAX_STRIDE || p.kt > MAX_STRIDE || p.vt > MAX_STRIDE || (long)p.H * p.D > MAX_STRIDE) return INDM_E_SHAPE;
   return 1;
 }
 WAttnArgs pack_args(const void* q, const void* k, const void* v, const long* s, const int* lengths, int B, int T, int H, int Hk, int D,
@@ -665,11 +741,11 @@ WAttnArgs pack_args(const void* q, const void* k, const void* v, const long* s, 
 }
 
 template <typename T>
-int fwd(WAttnArgs p, const long* strides, void* o, float* lse, hipStream_t st) {
+int fwd(WAttnArgs p, const long* strides, void* o, void* olo, float* lse, hipStream_t st) {
   const int r = check<T>(p, strides);
   if (r <= 0) return r;
-  if (o == nullptr || ((uintptr_t)o & 15)) return INDM_E_ARG;
-  p.out = o; p.lse = lse;
+  if (o == nullptr || (((uintptr_t)o | (uintptr_t)olo) & 15)) return INDM_E_ARG;
+  p.out = o; p.olo = olo; p.lse = lse;
 #define WA_FWD(DP) run_query<T, DP, 4, false>(p, st)
   WA_DISPATCH(WA_FWD)
 }
@@ -678,17 +754,18 @@ template <typename T, int DP>
 int bwd_dp(const WAttnArgs& p, hipStream_t st) {
   int r = run_query<T, DP, 4, true>(p, st);   // dq, and delta for the others
   if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, 1, true>(p, st);
+  if (r == INDM_OK && p.chunks > 1) r = run_join(p, st);
   if (r == INDM_OK) r = run_key<T, DP, 4, false>(p, st);
   return r;
 }
 template <typename T>
-int bwd(WAttnArgs p, const long* strides, const void* o, const void* dO, const float* lse, void* dq, void* dk, void* dv, float* ws,
+int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const void* dO, const float* lse, void* dq, void* dk, void* dv, float* ws,
         hipStream_t st) {
   const int r = check<T>(p, strides);
   if (r <= 0) return r;
   if (o == nullptr || dO == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || ws == nullptr ||
-      (((uintptr_t)o | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
-  p.o = o; p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
+      (((uintptr_t)o | (uintptr_t)olo | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
+  p.o = o; p.olo = const_cast<void*>(olo); p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = ws;
   p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
   p.chunks = sink_chunks(p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
@@ -701,13 +778,13 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* dO, const f
 INDM_API int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, float* lse,
                                 const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal,
                                 float scale, void* stream) {
-  return fwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, lse,
+  return fwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, nullptr, lse,
                     (hipStream_t)stream);
 }
-INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, const long* strides, void* o, float* lse,
+INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, const long* strides, void* o, void* o_lo, float* lse,
                                  const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal,
                                  float scale, void* stream) {
-  return fwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, lse,
+  return fwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, o_lo, lse,
                   (hipStream_t)stream);
 }
 
@@ -720,12 +797,12 @@ INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int l
 INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const float* dO,
                                 const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,
                                 int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream) {
-  return bwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, dO, lse, dq, dk,
-                    dv, ws, (hipStream_t)stream);
+  return bwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, nullptr, dO, lse, dq,
+                    dk, dv, ws, (hipStream_t)stream);
 }
-INDM_API int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, const long* strides, const void* o, const void* dO,
-                                 const float* lse, const int* lengths, void* dq, void* dk, void* dv, float* ws, int B, int T, int H,
+INDM_API int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, const long* strides, const void* o, const void* o_lo,
+                                 const void* dO, const float* lse, const int* lengths, void* dq, void* dk, void* dv, float* ws, int B, int T, int H,
                                  int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream) {
-  return bwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, dO, lse, dq, dk, dv,
-                  ws, (hipStream_t)stream);
+  return bwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, o_lo, dO, lse, dq, dk,
+                  dv, ws, (hipStream_t)stream);
 }

@@ -172,10 +172,10 @@ _SIGS = {
     "indm_rotary_f32": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
     "indm_rotary_bf16": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
     "indm_wattn_fwd_f32": [c_p] * 7 + [c_i] * 9 + [c_f, c_p],
-    "indm_wattn_fwd_bf16": [c_p] * 7 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_fwd_bf16": [c_p] * 8 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_bwd_ws_floats": [c_i] * 9,
     "indm_wattn_bwd_f32": [c_p] * 12 + [c_i] * 9 + [c_f, c_p],
-    "indm_wattn_bwd_bf16": [c_p] * 12 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_bwd_bf16": [c_p] * 13 + [c_i] * 9 + [c_f, c_p],
     "indm_timer_create": [c_i, c_p],
     "indm_timer_destroy": [c_p],
     "indm_timer_reset": [c_p, c_i],
@@ -2360,9 +2360,9 @@ def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
 
 
 def _aligned_rows(x):
-    """x [B, T, heads, D] with D contiguous and every row on 16 bytes; a copy where it is not so"""
+    """x [B, T, heads, D] with D contiguous, every row on 16 bytes and tokens at most 2^22 elements apart; a copy where it is not so"""
     s, e = x.stride(), 16 // x.element_size()
-    if s[3] == 1 and s[0] % e == 0 and s[1] % e == 0 and s[2] % e == 0 and x.data_ptr() % 16 == 0:
+    if s[3] == 1 and s[0] % e == 0 and s[1] % e == 0 and s[2] % e == 0 and s[1] <= 1 << 22 and x.data_ptr() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -2380,8 +2380,8 @@ def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
         _refuse(f"window_attention: the {H} heads of q are a multiple of the {Hk} of k and v")
     if D % 8 or not 8 <= D <= 128:
         _refuse(f"window_attention: heads of 8, 16, ... 128 entries, got {D}")
-    if T > 1 << 28:
-        _refuse(f"window_attention: up to {1 << 28} tokens, got {T}")
+    if T > 1 << 28 or H * D > 1 << 22:
+        _refuse(f"window_attention: up to {1 << 28} tokens of {1 << 22} entries, got {T} of {H * D}")
     if left < 0 or right < 0 or sinks < 0:
         _refuse(f"window_attention: window and sinks >= 0, got ({left}, {right}), {sinks}")
     if not 0.0 < scale < float("inf"):
@@ -2392,22 +2392,28 @@ def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
 
 
 def wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats=True):
-    """-> o [B, T, H, D], lse [B, H, T] (None without stats), q, k, v as the kernel read them (copies where rows were not on 16 bytes)"""
+    """-> o [B, T, H, D]; with stats for the backward: what rounding o to bf16 left (None for float32) and lse [B, H, T]; and q, k, v as
+    the kernel read them (copies where rows were not on 16 bytes)"""
     suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
     with _token_device("window_attention", q, k, v, lengths):
         q, k, v, lengths = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v), _contig(lengths)
         B, T, H, D = q.shape
+        strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         o = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
         lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device) if stats else None
-        fn = lib().indm_wattn_fwd_f32 if suf == "f32" else lib().indm_wattn_fwd_bf16
-        st = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), o.data_ptr(),
-                _data(lse), _data(lengths), B, T, H, k.shape[2], D, min(left, T), min(right, T), min(sinks, T), int(causal), scale, _stream())
+        rest = (_data(lengths), B, T, H, k.shape[2], D, min(left, T), min(right, T), min(sinks, T), int(causal), scale, _stream())
+        if suf == "f32":
+            olo = None
+            st = lib().indm_wattn_fwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(lse), *rest)
+        else:
+            olo = torch.empty_like(o) if stats else None
+            st = lib().indm_wattn_fwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(olo), _data(lse), *rest)
         _chk(st, "indm_wattn_fwd_" + suf)
-    return o, lse, q, k, v
+    return o, olo, lse, q, k, v
 
 
-def wattn_bwd(q, k, v, o, lse, do, left, right, sinks, causal, lengths, scale):
-    """-> dq, dk, dv (dense).  q, k, v, o, lse: wattn_fwd's.  The scratch is an allocation of its own."""
+def wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale):
+    """-> dq, dk, dv (dense).  q, k, v, o, olo, lse: wattn_fwd's.  The scratch is an allocation of its own."""
     suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
     if do.dtype != q.dtype or do.shape != q.shape:
         _refuse(f"window_attention: do is {tuple(q.shape)} {q.dtype}, got {tuple(do.shape)} {do.dtype}")
@@ -2421,9 +2427,12 @@ def wattn_bwd(q, k, v, o, lse, do, left, right, sinks, causal, lengths, scale):
         dk, dv = (torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
         ws = torch.empty((max(1, lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, int(causal))),), dtype=torch.float32,
                          device=q.device)
-        fn = lib().indm_wattn_bwd_f32 if suf == "f32" else lib().indm_wattn_bwd_bf16
-        st = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), o.data_ptr(),
-                do.data_ptr(), lse.data_ptr(), _data(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H, Hk, D,
+        strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        rest = (do.data_ptr(), lse.data_ptr(), _data(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H, Hk, D,
                 left, right, sinks, int(causal), scale, _stream())
+        if suf == "f32":
+            st = lib().indm_wattn_bwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), *rest)
+        else:
+            st = lib().indm_wattn_bwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(olo), *rest)
         _chk(st, "indm_wattn_bwd_" + suf)
     return dq, dk, dv

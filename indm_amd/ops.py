@@ -1055,17 +1055,17 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
 class _WindowAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, left, right, sinks, causal, lengths, scale):
-        o, lse, q, k, v = hip.wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        o, olo, lse, q, k, v = hip.wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale)
+        ctx.save_for_backward(q, k, v, o, olo, lse, lengths)
         ctx.cfg = (left, right, sinks, causal, scale)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, olo, lse, lengths = ctx.saved_tensors
         left, right, sinks, causal, scale = ctx.cfg
-        dq, dk, dv = hip.wattn_bwd(q, k, v, o, lse, do, left, right, sinks, causal, lengths, scale)
+        dq, dk, dv = hip.wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale)
         return dq, dk, dv, None, None, None, None, None, None
 
 
