@@ -87,6 +87,16 @@ template <> struct Op<u16> {
   static __device__ __forceinline__ frag pack(const f32x16& s, int o) {
     return indm_pack_bf16x8(s[o], s[o + 1], s[o + 2], s[o + 3], s[o + 4], s[o + 5], s[o + 6], s[o + 7]);
   }
+  static __device__ __forceinline__ frag pack_rest(const f32x16& s, const frag& w, int o) {   // what pack's rounding left
+    const u32x4 u = __builtin_bit_cast(u32x4, w);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = s[o + 2 * i] - __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = s[o + 2 * i + 1] - __uint_as_float(u[i] & 0xffff0000u);
+    }
+    return indm_pack_bf16x8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+  }
   static __device__ __forceinline__ float get(const frag& f, int i) { return (float)f[i]; }
 };
 struct f32frag {
@@ -436,8 +446,17 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0)
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const frag w = O::pack(S, 8 * a);
+        if constexpr (!BWD && sizeof(T) == 2) {
+          const frag rest = O::pack_rest(S, w, 8 * a);
 #pragma unroll
-        for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
+          for (int d = 0; d < G::DB; ++d) {
+            const frag z = at.transposed(zb, 32 * y + 16 * a, d);
+            acc[d] = O::mma(z, rest, O::mma(z, w, acc[d]));
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
+        }
       }
     }
     staged();
