@@ -2204,14 +2204,18 @@ def _token_suffix(op, x):
 
 def _token_device(op, *tensors):
     """every tensor on one GPU; -> a context in which that GPU is the current device (allocations and the launch go there)"""
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None:
-            if not t.is_cuda:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            if not (t.is_cuda and tensors[0].is_cuda):
                 raise RuntimeError("indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback")
-            if t.device != dev:
-                _refuse(f"{op}: tensors on {dev} and {t.device}")
-    return _NO_TIMING if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+            _refuse(f"{op}: tensors on {tensors[0].device} and {t.device}")
+    return _NO_TIMING if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
+def _like(x):
+    """a dense tensor of x's shape, type and device"""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _data(t):
@@ -2257,42 +2261,42 @@ def _ln_check(x, gamma, beta):
 
 
 def layernorm_fwd(x, gamma=None, beta=None, eps=1e-6, stats=True):
-    """x [..., C] -> y, mean [R], rstd [R] (None, None without stats)"""
+    """x [..., C] -> y, the rows' statistics for the backward (fp32 [2 R]: means, then rstds; None without stats)"""
     suf = _ln_check(x, gamma, beta)
     if not eps >= 0.0:
         _refuse(f"layer_norm: eps >= 0, got {eps}")
     with _token_device("layer_norm", x, gamma, beta):
         gamma, beta = _contig(gamma), _contig(beta)
         xr, R, ldx = _rows2d(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = rstd = None
-        if stats:
-            mean, rstd = torch.empty((2, R), dtype=torch.float32, device=x.device).unbind(0)
+        y = _like(x)
+        mean = torch.empty((2 * R,), dtype=torch.float32, device=x.device) if stats else None   # the means, then the rstds
         fn = lib().indm_layernorm_fwd_f32 if suf == "f32" else lib().indm_layernorm_fwd_bf16
-        st = fn(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean), _data(rstd), R, x.shape[-1], eps, _stream())
+        st = fn(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean), mean.data_ptr() + 4 * R if stats else None,
+                R, x.shape[-1], eps, _stream())
         _chk(st, "indm_layernorm_fwd_" + suf)
-    return y, mean, rstd
+    return y, mean
 
 
-def layernorm_bwd(dy, x, gamma, mean, rstd, want_gamma=True, want_beta=True):
+def layernorm_bwd(dy, x, gamma, stats, want_gamma=True, want_beta=True):
     """-> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its own: calls on different
     streams, or in different captured graphs, share nothing."""
     suf = _ln_check(x, gamma, None)
     if dy.dtype != x.dtype or dy.shape != x.shape:
         _refuse(f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    with _token_device("layer_norm", x, dy, gamma, mean, rstd):
+    with _token_device("layer_norm", x, dy, gamma, stats):
         C = x.shape[-1]
         gamma, dy = _contig(gamma), _contig(dy)
         xr, R, ldx = _rows2d(x)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _like(x)
         dgamma = torch.empty((C,), dtype=torch.float32, device=x.device) if want_gamma else None
         dbeta = torch.empty((C,), dtype=torch.float32, device=x.device) if want_beta else None
         ws = None
         if want_gamma or want_beta:
             ws = torch.empty((max(1, lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size())),), dtype=torch.float32, device=x.device)
         fn = lib().indm_layernorm_bwd_f32 if suf == "f32" else lib().indm_layernorm_bwd_bf16
-        st = fn(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _data(dgamma),
-                _data(dbeta), _data(ws), R, C, _stream())
+        mean = stats.data_ptr()
+        st = fn(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean, mean + 4 * R, dx.data_ptr(), _data(dgamma), _data(dbeta),
+                _data(ws), R, C, _stream())
         _chk(st, "indm_layernorm_bwd_" + suf)
     return dx, dgamma, dbeta
 
@@ -2310,7 +2314,7 @@ def dropout(x, p, seed, res=None, seed_dev=None):
         _refuse("dropout: seed_dev is one int64 on the device")
     with _token_device("dropout", x, res, seed_dev):
         x, res = _contig(x), _contig(res)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _like(x)
         fn = lib().indm_dropout_f32 if suf == "f32" else lib().indm_dropout_bf16
         _chk(fn(x.data_ptr(), _data(res), y.data_ptr(), x.numel(), p, seed, _seed_ptr(seed_dev), _stream()), "indm_dropout_" + suf)
     return y
@@ -2348,8 +2352,8 @@ def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
         if k is not None:
             k = k if k.stride(3) == 1 or D == 1 else k.contiguous()
             Hk, sk = k.shape[2], k.stride()[:3]
-            yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            yk = _like(k)
+        yq = _like(q)
         pos, freqs, A = _contig(pos), _contig(freqs), len(sections)
         fn = lib().indm_rotary_f32 if suf == "f32" else lib().indm_rotary_bf16
         st = fn(q.data_ptr(), _data(k), yq.data_ptr(), _data(yk), (c_l * 6)(*q.stride()[:3], *sk), B, T, H, Hk, D, pos.data_ptr(),
@@ -2399,7 +2403,7 @@ def wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats=True):
         q, k, v, lengths = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v), _contig(lengths)
         B, T, H, D = q.shape
         strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-        o = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+        o = _like(q)
         lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device) if stats else None
         rest = (_data(lengths), B, T, H, k.shape[2], D, min(left, T), min(right, T), min(sinks, T), int(causal), scale, _stream())
         if suf == "f32":
@@ -2423,8 +2427,7 @@ def wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, sca
             do = do.clone()
         B, T, H, D = q.shape
         Hk, left, right, sinks = k.shape[2], min(left, T), min(right, T), min(sinks, T)
-        dq = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device) for _ in range(2))
+        dq, dk, dv = _like(q), _like(k), _like(v)
         ws = torch.empty((max(1, lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, int(causal))),), dtype=torch.float32,
                          device=q.device)
         strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])

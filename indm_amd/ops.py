@@ -969,18 +969,29 @@ def _tracked(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable, whose bookkeeping (some microseconds) is only needed where the backward pass is itself recorded"""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 class _LayerNorm(Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps):
-        y, mean, rstd = hip.layernorm_fwd(x, gamma, beta, eps)
-        ctx.save_for_backward(x, gamma, mean, rstd)
+        y, stats = hip.layernorm_fwd(x, gamma, beta, eps)
+        ctx.save_for_backward(x, gamma, stats)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, gamma, mean, rstd = ctx.saved_tensors
-        dx, dg, db = hip.layernorm_bwd(dy, x, gamma, mean, rstd, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        x, gamma, stats = ctx.saved_tensors
+        _, want_gamma, want_beta, _ = ctx.needs_input_grad
+        dx, dg, db = hip.layernorm_bwd(dy, x, gamma, stats, want_gamma, want_beta)
         return dx, dg, db, None
 
 
@@ -1000,7 +1011,7 @@ class _Dropout(Function):
         return hip.dropout(x, p, seed, res, sd)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         p, seed, sd = ctx.cfg
         dx = hip.dropout(dy, p, seed, None, sd) if ctx.needs_input_grad[0] else None
@@ -1030,7 +1041,7 @@ class _Rotary(Function):
         return hip.rotary(q, k, pos, freqs, sections, interleaved)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dq, dk):
         pos, freqs = ctx.saved_tensors
         sections, interleaved = ctx.cfg
@@ -1061,7 +1072,7 @@ class _WindowAttention(Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         q, k, v, o, olo, lse, lengths = ctx.saved_tensors
         left, right, sinks, causal, scale = ctx.cfg
