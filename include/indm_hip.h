@@ -650,18 +650,18 @@ int indm_rotary_bf16(const void* q, const void* k, void* yq, void* yk, const lon
  * clamped to 0 .. T; NULL: T).  Rows i >= n of o and of the gradients are zeros, and what q, k, v hold there is never used.
  * q [B, T, H, D], k, v [B, T, Hk, D] (H a multiple of Hk: head h reads h / (H / Hk)), strides[9]: B, T, head strides in elements of
  * q, k, v (a HOST array); D contiguous, D % 8 == 0, D <= 128; rows on 16 bytes (bases and strides),
- * strides not negative, token strides and H D up to 2^22.  o dense.  o_lo (bf16, as o, or NULL): what rounding o to bf16 left; the
- * backward's <dO, o> then is as exact as its other terms.  lse fp32 [B, H, T] for
+ * strides not negative, token strides and H D up to 2^22.  o dense.  o_lo (bf16, as o, or NULL; fp32: not used): what rounding o to bf16
+ * left; the backward's <dO, o> then is as exact as its other terms.  lse fp32 [B, H, T] for
  * the backward (log2 of the sum of exponentials; +inf for rows >= n), or NULL.  left, right, sinks >= 0, scale > 0.
  * Backward: dq, dk, dv dense from dense o, dO and lse; ws: indm_wattn_bwd_ws_floats floats, 16-byte aligned.  The queries' heads that
  * share a key are summed in a fixed order, the sinks' long sums are split over workgroups and joined in a fixed order. */
-int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, float* lse, const int* lengths,
-                       int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream);
+int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, void* o_lo, float* lse,
+                       const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream);
 int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, const long* strides, void* o, void* o_lo, float* lse,
                         const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream);
 long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal);
-int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const float* dO,
-                       const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H, int Hk,
+int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const void* o_lo,
+                       const float* dO, const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H, int Hk,
                        int D, int left, int right, int sinks, int causal, float scale, void* stream);
 int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, const long* strides, const void* o, const void* o_lo, const void* dO,
                         const float* lse, const int* lengths, void* dq, void* dk, void* dv, float* ws, int B, int T, int H, int Hk,

@@ -794,7 +794,7 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
 
 }  // namespace
 
-INDM_API int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, float* lse,
+INDM_API int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, void*, float* lse,
                                 const int* lengths, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal,
                                 float scale, void* stream) {
   return fwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, nullptr, lse,
@@ -813,8 +813,8 @@ INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int l
   const long chunks = sink_chunks(B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal);
   return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * chunks * cdiv(sinks, 32) * 32 * 2 * D;
 }
-INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const float* dO,
-                                const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,
+INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const void*,
+                                const float* dO, const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,
                                 int Hk, int D, int left, int right, int sinks, int causal, float scale, void* stream) {
   return bwd<float>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, nullptr, dO, lse, dq,
                     dk, dv, ws, (hipStream_t)stream);

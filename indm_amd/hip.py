@@ -171,10 +171,10 @@ _SIGS = {
     "indm_dropout_bf16": [c_p, c_p, c_p, c_l, c_f, c_u64, c_p, c_p],
     "indm_rotary_f32": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
     "indm_rotary_bf16": [c_p, c_p, c_p, c_p, c_p, c_i, c_l, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_i, c_i, c_i, c_p],
-    "indm_wattn_fwd_f32": [c_p] * 7 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_fwd_f32": [c_p] * 8 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_fwd_bf16": [c_p] * 8 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_bwd_ws_floats": [c_i] * 9,
-    "indm_wattn_bwd_f32": [c_p] * 12 + [c_i] * 9 + [c_f, c_p],
+    "indm_wattn_bwd_f32": [c_p] * 13 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_bwd_bf16": [c_p] * 13 + [c_i] * 9 + [c_f, c_p],
     "indm_timer_create": [c_i, c_p],
     "indm_timer_destroy": [c_p],
@@ -2189,28 +2189,36 @@ def iresblock_inverse(y, cb, W1, W2T, W3, b1, b2, b3, preact, atol, rtol):
 
 
 # --------------------------------------------------------------------------- operators of a block over tokens (csrc/token_ops.hip, window_attn.hip)
+# A call of these costs more host time than GPU time on small tensors: the checks build their messages only when they refuse, nothing is
+# looked up by a name that has to be put together first, and a tensor's scratch is one allocation.
 _TOKEN_DTYPES = {torch.float32: "f32", torch.bfloat16: "bf16"}
+_token_fns = {}
+
+
+def _token_fn(op, dtype):
+    """the entry point indm_<op>_<type> of the library"""
+    fn = _token_fns.get((op, dtype))
+    if fn is None:
+        if dtype not in _TOKEN_DTYPES:
+            _refuse(f"{op}: expected float32 or bfloat16, got {dtype}")
+        fn = _token_fns[op, dtype] = getattr(lib(), f"indm_{op}_{_TOKEN_DTYPES[dtype]}")
+    return fn
 
 
 def _refuse(what):
     raise RuntimeError("indm_amd: " + what)
 
 
-def _token_suffix(op, x):
-    if x.dtype not in _TOKEN_DTYPES:
-        _refuse(f"{op}: expected float32 or bfloat16, got {x.dtype}")
-    return _TOKEN_DTYPES[x.dtype]
-
-
 def _token_device(op, *tensors):
-    """every tensor on one GPU; -> a context in which that GPU is the current device (allocations and the launch go there)"""
+    """None if every tensor is on the current GPU; if all are on another one, a context in which that one is current (allocations and the
+    launch belong there)"""
     dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != dev or dev < 0):
             if not (t.is_cuda and tensors[0].is_cuda):
                 raise RuntimeError("indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback")
             _refuse(f"{op}: tensors on {tensors[0].device} and {t.device}")
-    return _NO_TIMING if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+    return None if torch.cuda.current_device() == dev else torch.cuda.device(dev)
 
 
 def _like(x):
@@ -2218,21 +2226,13 @@ def _like(x):
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _data(t):
-    return None if t is None else t.data_ptr()
-
-
-def _contig(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
 def _rows2d(x):
     """(x, R, row stride) of x [..., C] as R rows with one stride and contiguous columns; a copy only where x has no such view"""
     C = x.shape[-1]
-    R = x.numel() // C if C else 0
+    R = x.numel() // C
     if x.is_contiguous():
         return x, R, C
-    if x.numel() and (x.stride(-1) == 1 or C == 1):
+    if R and (x.stride(-1) == 1 or C == 1):
         try:
             v = x.view(R, C)
             return v, R, v.stride(0)
@@ -2241,69 +2241,85 @@ def _rows2d(x):
     return x.contiguous(), R, C
 
 
-_LN_MAX_C = {"f32": 16384, "bf16": 32768}
+_LN_MAX_C = {torch.float32: 16384, torch.bfloat16: 32768}
 
 
-def _ln_check(x, gamma, beta):
-    suf = _token_suffix("layer_norm", x)
+def _ln_check(x, gamma, beta, eps):
+    if x.dtype not in _TOKEN_DTYPES:
+        _refuse(f"layer_norm: expected float32 or bfloat16, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         _refuse(f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
     C = x.shape[-1]
-    if C > _LN_MAX_C[suf]:
-        _refuse(f"layer_norm: rows of up to {_LN_MAX_C[suf]} {suf} elements, got {C}")
-    for name, p in (("gamma", gamma), ("beta", beta)):
-        if p is not None:
+    if C > _LN_MAX_C[x.dtype]:
+        _refuse(f"layer_norm: rows of up to {_LN_MAX_C[x.dtype]} {x.dtype} elements, got {C}")
+    for p in (gamma, beta):
+        if p is not None and (p.dtype != torch.float32 or p.shape != (C,)):
+            name = "gamma" if p is gamma else "beta"
             if p.dtype != torch.float32:
                 _refuse(f"layer_norm: {name} is float32, got {p.dtype}")
-            if p.shape != (C,):
-                _refuse(f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
-    return suf
+            _refuse(f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
+    if not eps >= 0.0:
+        _refuse(f"layer_norm: eps >= 0, got {eps}")
 
 
 def layernorm_fwd(x, gamma=None, beta=None, eps=1e-6, stats=True):
     """x [..., C] -> y, the rows' statistics for the backward (fp32 [2 R]: means, then rstds; None without stats)"""
-    suf = _ln_check(x, gamma, beta)
-    if not eps >= 0.0:
-        _refuse(f"layer_norm: eps >= 0, got {eps}")
-    with _token_device("layer_norm", x, gamma, beta):
-        gamma, beta = _contig(gamma), _contig(beta)
-        xr, R, ldx = _rows2d(x)
-        y = _like(x)
-        mean = torch.empty((2 * R,), dtype=torch.float32, device=x.device) if stats else None   # the means, then the rstds
-        fn = lib().indm_layernorm_fwd_f32 if suf == "f32" else lib().indm_layernorm_fwd_bf16
-        st = fn(xr.data_ptr(), ldx, _data(gamma), _data(beta), y.data_ptr(), _data(mean), mean.data_ptr() + 4 * R if stats else None,
-                R, x.shape[-1], eps, _stream())
-        _chk(st, "indm_layernorm_fwd_" + suf)
+    _ln_check(x, gamma, beta, eps)
+    away = _token_device("layer_norm", x, gamma, beta)
+    if away is not None:
+        with away:
+            return layernorm_fwd(x, gamma, beta, eps, stats)
+    if gamma is not None and not gamma.is_contiguous():
+        gamma = gamma.contiguous()
+    if beta is not None and not beta.is_contiguous():
+        beta = beta.contiguous()
+    xr, R, ldx = _rows2d(x)
+    y = _like(x)
+    mean = torch.empty((2 * R,), dtype=torch.float32, device=x.device) if stats else None
+    m = mean.data_ptr() if stats else 0
+    st = _token_fn("layernorm_fwd", x.dtype)(
+        xr.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), y.data_ptr(),
+        m, m + 4 * R if stats else 0, R, x.shape[-1], eps, _stream())
+    if st:
+        _chk(st, "indm_layernorm_fwd")
     return y, mean
 
 
 def layernorm_bwd(dy, x, gamma, stats, want_gamma=True, want_beta=True):
-    """-> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its own: calls on different
-    streams, or in different captured graphs, share nothing."""
-    suf = _ln_check(x, gamma, None)
+    """x, gamma, stats: layernorm_fwd's -> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its
+    own: calls on different streams, or in different captured graphs, share nothing."""
     if dy.dtype != x.dtype or dy.shape != x.shape:
         _refuse(f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    with _token_device("layer_norm", x, dy, gamma, stats):
-        C = x.shape[-1]
-        gamma, dy = _contig(gamma), _contig(dy)
-        xr, R, ldx = _rows2d(x)
-        dx = _like(x)
-        dgamma = torch.empty((C,), dtype=torch.float32, device=x.device) if want_gamma else None
-        dbeta = torch.empty((C,), dtype=torch.float32, device=x.device) if want_beta else None
-        ws = None
-        if want_gamma or want_beta:
-            ws = torch.empty((max(1, lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size())),), dtype=torch.float32, device=x.device)
-        fn = lib().indm_layernorm_bwd_f32 if suf == "f32" else lib().indm_layernorm_bwd_bf16
-        mean = stats.data_ptr()
-        st = fn(dy.data_ptr(), xr.data_ptr(), ldx, _data(gamma), mean, mean + 4 * R, dx.data_ptr(), _data(dgamma), _data(dbeta),
-                _data(ws), R, C, _stream())
-        _chk(st, "indm_layernorm_bwd_" + suf)
+    away = _token_device("layer_norm", x, dy, gamma, stats)
+    if away is not None:
+        with away:
+            return layernorm_bwd(dy, x, gamma, stats, want_gamma, want_beta)
+    C = x.shape[-1]
+    if gamma is not None and not gamma.is_contiguous():
+        gamma = gamma.contiguous()
+    if not dy.is_contiguous():
+        dy = dy.contiguous()
+    xr, R, ldx = _rows2d(x)
+    dx, dgamma, dbeta, ws = _like(x), None, None, None
+    if want_gamma:
+        dgamma = torch.empty((C,), dtype=torch.float32, device=x.device)
+    if want_beta:
+        dbeta = torch.empty((C,), dtype=torch.float32, device=x.device)
+    if want_gamma or want_beta:
+        ws = torch.empty((lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size()) or 1,), dtype=torch.float32, device=x.device)
+    m = stats.data_ptr()
+    st = _token_fn("layernorm_bwd", x.dtype)(
+        dy.data_ptr(), xr.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(), m, m + 4 * R, dx.data_ptr(),
+        None if dgamma is None else dgamma.data_ptr(), None if dbeta is None else dbeta.data_ptr(), None if ws is None else ws.data_ptr(),
+        R, C, _stream())
+    if st:
+        _chk(st, "indm_layernorm_bwd")
     return dx, dgamma, dbeta
 
 
 def dropout(x, p, seed, res=None, seed_dev=None):
     """(res) + keep(seed + *seed_dev) x / (1 - p), the mask by x's dense (row-major) element index"""
-    suf = _token_suffix("dropout", x)
+    fn = _token_fn("dropout", x.dtype)
     if not 0.0 <= p <= 1.0:
         _refuse(f"dropout: 0 <= p <= 1, got {p}")
     if not 0 <= seed < 1 << 64:
@@ -2312,11 +2328,18 @@ def dropout(x, p, seed, res=None, seed_dev=None):
         _refuse(f"dropout: res is {tuple(x.shape)} {x.dtype}, got {tuple(res.shape)} {res.dtype}")
     if seed_dev is not None and (seed_dev.dtype != torch.int64 or seed_dev.numel() != 1):
         _refuse("dropout: seed_dev is one int64 on the device")
-    with _token_device("dropout", x, res, seed_dev):
-        x, res = _contig(x), _contig(res)
-        y = _like(x)
-        fn = lib().indm_dropout_f32 if suf == "f32" else lib().indm_dropout_bf16
-        _chk(fn(x.data_ptr(), _data(res), y.data_ptr(), x.numel(), p, seed, _seed_ptr(seed_dev), _stream()), "indm_dropout_" + suf)
+    away = _token_device("dropout", x, res, seed_dev)
+    if away is not None:
+        with away:
+            return dropout(x, p, seed, res, seed_dev)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if res is not None and not res.is_contiguous():
+        res = res.contiguous()
+    y = torch.empty_like(x)
+    st = fn(x.data_ptr(), None if res is None else res.data_ptr(), y.data_ptr(), x.numel(), p, seed, _seed_ptr(seed_dev), _stream())
+    if st:
+        _chk(st, "indm_dropout")
     return y
 
 
@@ -2324,7 +2347,8 @@ _POS_TYPES = {torch.int32: 0, torch.float32: 1, torch.int64: 2}
 
 
 def _rotary_check(q, k, pos, freqs, sections):
-    suf = _token_suffix("rotary", q)
+    if q.dtype not in _TOKEN_DTYPES:
+        _refuse(f"rotary: expected float32 or bfloat16, got {q.dtype}")
     if q.dim() != 4:
         _refuse(f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
     B, T, _, D = q.shape
@@ -2339,27 +2363,36 @@ def _rotary_check(q, k, pos, freqs, sections):
         _refuse(f"rotary: pos is [{T}, {A}] or [{B}, {T}, {A}], got {tuple(pos.shape)}")
     if freqs.dtype != torch.float64 or freqs.shape != (R // 2,):
         _refuse(f"rotary: freqs is float64 [{R // 2}], got {tuple(freqs.shape)} {freqs.dtype}")
-    return suf
 
 
 def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
     """q [B, T, H, D], k [B, T, Hk, D] or None -> their rotated copies (dense)"""
-    suf = _rotary_check(q, k, pos, freqs, sections)
-    with _token_device("rotary", q, k, pos, freqs):
-        B, T, H, D = q.shape
-        Hk, sk, yk = 0, (0, 0, 0), None
-        q = q if q.stride(3) == 1 or D == 1 else q.contiguous()
-        if k is not None:
-            k = k if k.stride(3) == 1 or D == 1 else k.contiguous()
-            Hk, sk = k.shape[2], k.stride()[:3]
-            yk = _like(k)
-        yq = _like(q)
-        pos, freqs, A = _contig(pos), _contig(freqs), len(sections)
-        fn = lib().indm_rotary_f32 if suf == "f32" else lib().indm_rotary_bf16
-        st = fn(q.data_ptr(), _data(k), yq.data_ptr(), _data(yk), (c_l * 6)(*q.stride()[:3], *sk), B, T, H, Hk, D, pos.data_ptr(),
-                _POS_TYPES[pos.dtype], T * A if pos.dim() == 3 else 0, freqs.data_ptr(), (c_i * A)(*sections), A, int(interleaved),
-                int(inverse), _stream())
-        _chk(st, "indm_rotary_" + suf)
+    _rotary_check(q, k, pos, freqs, sections)
+    away = _token_device("rotary", q, k, pos, freqs)
+    if away is not None:
+        with away:
+            return rotary(q, k, pos, freqs, sections, interleaved, inverse)
+    B, T, H, D = q.shape
+    if q.stride(3) != 1 and D > 1:
+        q = q.contiguous()
+    sq, A = q.stride(), len(sections)
+    yq = _like(q)
+    if k is None:
+        Hk, pk, pyk, sk, yk = 0, None, None, sq, None
+    else:
+        if k.stride(3) != 1 and D > 1:
+            k = k.contiguous()
+        yk = _like(k)
+        Hk, pk, pyk, sk = k.shape[2], k.data_ptr(), yk.data_ptr(), k.stride()
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
+    if not freqs.is_contiguous():
+        freqs = freqs.contiguous()
+    st = _token_fn("rotary", q.dtype)(
+        q.data_ptr(), pk, yq.data_ptr(), pyk, (c_l * 6)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2]), B, T, H, Hk, D, pos.data_ptr(),
+        _POS_TYPES[pos.dtype], T * A if pos.dim() == 3 else 0, freqs.data_ptr(), (c_i * A)(*sections), A, interleaved, inverse, _stream())
+    if st:
+        _chk(st, "indm_rotary")
     return yq, yk
 
 
@@ -2372,13 +2405,14 @@ def _aligned_rows(x):
 
 
 def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
-    suf = _token_suffix("window_attention", q)
+    if q.dtype not in _TOKEN_DTYPES:
+        _refuse(f"window_attention: expected float32 or bfloat16, got {q.dtype}")
     if q.dim() != 4:
         _refuse(f"window_attention: q is [B, T, H, D], got {tuple(q.shape)}")
     B, T, H, D = q.shape
-    for name, x in (("k", k), ("v", v)):
+    for x in (k, v):
         if x.dtype != q.dtype or x.dim() != 4 or x.shape[:2] != q.shape[:2] or x.shape[3] != D or x.shape != k.shape:
-            _refuse(f"window_attention: {name} is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(x.shape)} {x.dtype}")
+            _refuse(f"window_attention: {'k' if x is k else 'v'} is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(x.shape)} {x.dtype}")
     Hk = k.shape[2]
     if H < 1 or Hk < 1 or H % Hk:
         _refuse(f"window_attention: the {H} heads of q are a multiple of the {Hk} of k and v")
@@ -2392,50 +2426,60 @@ def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
         _refuse(f"window_attention: scale > 0, got {scale}")
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
         _refuse(f"window_attention: lengths is int32 [{B}], got {tuple(lengths.shape)} {lengths.dtype}")
-    return suf
 
 
 def wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats=True):
     """-> o [B, T, H, D]; with stats for the backward: what rounding o to bf16 left (None for float32) and lse [B, H, T]; and q, k, v as
     the kernel read them (copies where rows were not on 16 bytes)"""
-    suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
-    with _token_device("window_attention", q, k, v, lengths):
-        q, k, v, lengths = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v), _contig(lengths)
-        B, T, H, D = q.shape
-        strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-        o = _like(q)
-        lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device) if stats else None
-        rest = (_data(lengths), B, T, H, k.shape[2], D, min(left, T), min(right, T), min(sinks, T), int(causal), scale, _stream())
-        if suf == "f32":
-            olo = None
-            st = lib().indm_wattn_fwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(lse), *rest)
-        else:
-            olo = torch.empty_like(o) if stats else None
-            st = lib().indm_wattn_fwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(olo), _data(lse), *rest)
-        _chk(st, "indm_wattn_fwd_" + suf)
+    _wattn_check(q, k, v, left, right, sinks, lengths, scale)
+    away = _token_device("window_attention", q, k, v, lengths)
+    if away is not None:
+        with away:
+            return wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats)
+    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+    if lengths is not None and not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    B, T, H, D = q.shape
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    strides = (c_l * 9)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
+    o, olo, lse = _like(q), None, None
+    if stats:
+        lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device)
+        if q.dtype == torch.bfloat16:
+            olo = torch.empty_like(o)
+    st = _token_fn("wattn_fwd", q.dtype)(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), None if olo is None else olo.data_ptr(),
+        None if lse is None else lse.data_ptr(), None if lengths is None else lengths.data_ptr(), B, T, H, k.shape[2], D, min(left, T),
+        min(right, T), min(sinks, T), causal, scale, _stream())
+    if st:
+        _chk(st, "indm_wattn_fwd")
     return o, olo, lse, q, k, v
 
 
 def wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale):
-    """-> dq, dk, dv (dense).  q, k, v, o, olo, lse: wattn_fwd's.  The scratch is an allocation of its own."""
-    suf = _wattn_check(q, k, v, left, right, sinks, lengths, scale)
+    """-> dq, dk, dv (dense).  q, k, v, o, olo, lse: wattn_fwd's, which checked the arguments.  The scratch is an allocation of its own."""
     if do.dtype != q.dtype or do.shape != q.shape:
         _refuse(f"window_attention: do is {tuple(q.shape)} {q.dtype}, got {tuple(do.shape)} {do.dtype}")
-    with _token_device("window_attention", q, k, v, o, lse, do, lengths):
-        do, lengths = _contig(do), _contig(lengths)
-        if do.data_ptr() % 16:
-            do = do.clone()
-        B, T, H, D = q.shape
-        Hk, left, right, sinks = k.shape[2], min(left, T), min(right, T), min(sinks, T)
-        dq, dk, dv = _like(q), _like(k), _like(v)
-        ws = torch.empty((max(1, lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, int(causal))),), dtype=torch.float32,
-                         device=q.device)
-        strides = (c_l * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-        rest = (do.data_ptr(), lse.data_ptr(), _data(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H, Hk, D,
-                left, right, sinks, int(causal), scale, _stream())
-        if suf == "f32":
-            st = lib().indm_wattn_bwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), *rest)
-        else:
-            st = lib().indm_wattn_bwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), _data(olo), *rest)
-        _chk(st, "indm_wattn_bwd_" + suf)
+    away = _token_device("window_attention", q, k, v, o, lse, do, lengths)
+    if away is not None:
+        with away:
+            return wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale)
+    if not do.is_contiguous():
+        do = do.contiguous()
+    if do.data_ptr() % 16:
+        do = do.clone()
+    if lengths is not None and not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    B, T, H, D = q.shape
+    Hk, left, right, sinks = k.shape[2], min(left, T), min(right, T), min(sinks, T)
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    strides = (c_l * 9)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    ws = torch.empty((lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, causal) or 1,), dtype=torch.float32, device=q.device)
+    st = _token_fn("wattn_bwd", q.dtype)(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), None if olo is None else olo.data_ptr(), do.data_ptr(),
+        lse.data_ptr(), None if lengths is None else lengths.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H,
+        Hk, D, left, right, sinks, causal, scale, _stream())
+    if st:
+        _chk(st, "indm_wattn_bwd")
     return dq, dk, dv

@@ -1060,7 +1060,7 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     None, fp32 or bf16, any strides (columns of one fused product).  sections: entries of a head per axis (even), the rest passes
     through; pos [T, A] or [B, T, A] (int32, int64 or fp32), the token's coordinate on each axis; freqs from rotary_freqs().  A pair
     (a, b) -> (a cos - b sin, b cos + a sin) of the angle pos freq; pairs are the halves of a section, or neighbours if interleaved."""
-    return _Rotary.apply(q, k, pos, freqs, tuple(int(n) for n in sections), bool(interleaved))
+    return _Rotary.apply(q, k, pos, freqs, sections, bool(interleaved))
 
 
 class _WindowAttention(Function):

@@ -54,10 +54,10 @@ def test_c_entry_points_refuse_and_ignore_empty_work():
         ok = (ctypes.c_long * 9)(*[64] * 9)
 
         def f(q=p, s=ok, o=p, B=1, T=4, H=2, Hk=1, D=16, l=1, r=1, sinks=0, scale=1.0):
-            return fwd(q, p, p, s, o, *([None] if suf == "bf16" else []), None, None, B, T, H, Hk, D, l, r, sinks, 0, scale, None)
+            return fwd(q, p, p, s, o, None, None, None, B, T, H, Hk, D, l, r, sinks, 0, scale, None)
 
         def g(ws=p, o=p, D=16, T=4):
-            return bwd(p, p, p, ok, o, *([None] if suf == "bf16" else []), p, p, None, p, p, p, ws, 1, T, 2, 1, D, 1, 1, 0, 0, 1.0, None)
+            return bwd(p, p, p, ok, o, None, p, p, None, p, p, p, ws, 1, T, 2, 1, D, 1, 1, 0, 0, 1.0, None)
 
         assert f(H=3, Hk=2) == f(D=12) == f(D=136) == f(D=0) == f(B=-1) == f(T=-1) == f(T=(1 << 28) + 1) == f(H=0) == f(Hk=0) == -1
         assert f(l=-1) == f(r=-1) == f(sinks=-1) == f(scale=0.0) == f(scale=float("nan")) == f(scale=float("inf")) == -4
