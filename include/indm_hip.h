@@ -608,7 +608,7 @@ int indm_timer_read(void* handle, float* total_ms, int* launches, double* flops)
 
 /* Layer norm over the last dimension: y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(var + eps), statistics fp32 from the row
  * in registers (mean first, then the squared differences).  x: R rows of C elements, ldx elements apart (any alignment); y dense;
- * gamma, beta fp32 [C] or NULL (1, 0); mean, rstd [R] for the backward, or both NULL.  C <= 16384 (f32) / 32768 (bf16). */
+ * gamma, beta fp32 [C] or NULL (1, 0); mean, rstd [R] for the backward, or both NULL.  C <= 16384. */
 int indm_layernorm_fwd_f32(const float* x, long ldx, const float* gamma, const float* beta, float* y, float* mean, float* rstd,
                            long R, int C, float eps, void* stream);
 int indm_layernorm_fwd_bf16(const void* x, long ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd, long R,
@@ -636,7 +636,7 @@ int indm_dropout_bf16(const void* x, const void* res, void* y, long n, float p, 
  * passes through.  A pair of section s (n entries at offset o) is (o + j, o + n/2 + j), interleaved: (o + 2j, o + 2j + 1).
  * strides[6]: B, T, head strides in elements of q, then of k (D contiguous, any alignment); yq, yk dense, not the inputs.
  * pos: [T, axes] (pos_sb = 0) or [B, T, axes] (pos_sb = T axes); pos_type 0 int32, 1 fp32, 2 int64.  freqs: fp64 [sum(sections) / 2],
- * in the pairs' order; angles are formed and reduced in 64 bits.  sections[axes], axes <= 8: even, positive, sum <= D (HOST arrays, as strides).
+ * in the pairs' order; angles are formed and reduced in 64 bits.  sections[axes], axes <= 8: even, positive, sum <= D <= 4096 (HOST arrays, as strides).
  * inverse = 1: by the negative angles (the backward pass). */
 int indm_rotary_f32(const float* q, const float* k, float* yq, float* yk, const long* strides, int B, long T, int H, int Hk, int D,
                     const void* pos, int pos_type, long pos_sb, const double* freqs, const int* sections, int axes, int interleaved,

@@ -11,8 +11,7 @@ namespace {
 
 typedef unsigned u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x2t __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2t __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ unsigned short to_bits16(float v) {
   const __bf16 h = (__bf16)v;   // round to nearest even
@@ -59,13 +58,26 @@ template <> struct Row<unsigned short> {   // bf16
 
 // the vector at p, of which n elements (any n) exist; the others read as 0
 template <typename T>
-__device__ __forceinline__ void load_part(const T* p, int n, float (&v)[Row<T>::V]) {
+__device__ __forceinline__ typename Row<T>::raw load_raw(const T* p, int n) {
+  typename Row<T>::raw w = {0u, 0u, 0u, 0u};
   if (n >= Row<T>::V) {
-    Row<T>::unpack(Row<T>::load(p), v);
-  } else {
+    w = Row<T>::load(p);
+  } else if (n > 0) {
 #pragma unroll
-    for (int i = 0; i < Row<T>::V; ++i) v[i] = i < n ? Row<T>::get(p + i) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        if (i < n) w[i] = __float_as_uint(p[i]);
+      } else {
+        const unsigned lo = 2 * i < n ? p[2 * i] : 0u, hi = 2 * i + 1 < n ? p[2 * i + 1] : 0u;
+        w[i] = lo | hi << 16;
+      }
+    }
   }
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void load_part(const T* p, int n, float (&v)[Row<T>::V]) {
+  Row<T>::unpack(load_raw<T>(p, n), v);
 }
 template <typename T>
 __device__ __forceinline__ void store_part(T* p, int n, const float (&v)[Row<T>::V]) {
@@ -99,16 +111,38 @@ __device__ __forceinline__ void load_param(const float* p, int n, float fill, fl
 // ------------------------------------------------------------------------------------------------ layer norm
 // A team of L lanes owns a row and keeps it in registers (NV vectors a lane), so the statistics are the two-pass ones -- the
 // mean, then the sum of squared differences from it -- and x is read from HBM once.  L < 64: several rows a wavefront.
-// Sum over the team; every lane gets it.  L > 64: the team is the whole workgroup.
+// Sum over the team; every lane gets the same bits (each step adds a pair, whichever order).  Within a wavefront all steps are
+// vector instructions: lanes 1, 2, then mirrored quads and halves of a row of 16, then rows and halves of the wavefront traded.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  const int i = __float_as_int(v);
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
 template <int L>
 __device__ __forceinline__ float team_sum(float v, float* sh) {
-  if constexpr (L <= 64) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-  } else {
-    return block_sum(v, sh);
+  v = dpp_add<0xB1>(v);    // quad_perm [1, 0, 3, 2]
+  v = dpp_add<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+  v = dpp_add<0x141>(v);   // row_half_mirror
+  v = dpp_add<0x140>(v);   // row_mirror
+  if constexpr (L >= 32) {
+    const unsigned u = __float_as_uint(v);
+    const u32x2t r = __builtin_bit_cast(u32x2t, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
+  if constexpr (L >= 64) {
+    const unsigned u = __float_as_uint(v);
+    const u32x2t r = __builtin_bit_cast(u32x2t, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L > 64) {   // the team is the whole workgroup
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < L / 64; ++i) v += sh[i];
+  }
+  return v;
 }
 
 // y = (x - mean) rstd gamma + beta;  R rows of C, x's rows ldx elements apart.  RPT rows a team at once: their loads are all in
@@ -188,7 +222,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_fwd_kernel(const 
 // dx = rstd (h - mean(h) - xh mean(h xh)),  h = dy gamma,  xh = (x - mean) rstd;  per-workgroup partial sums of
 // dgamma = sum dy xh and dbeta = sum dy in registers over the workgroup's rows, folded over its teams in a fixed order and
 // written to part[workgroup][2][C] (layernorm_param_kernel adds those up: no atomics, the same bits every time).
-template <typename T, int L, int NV>
+template <typename T, int L, int NV, int RPT>
 __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                                            long ldx, const float* __restrict__ gamma,
                                                                            const float* __restrict__ mean,
@@ -207,40 +241,54 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < V; ++i) dg[j][i] = db[j][i] = 0.f;
   }
-  const long step = (long)gridDim.x * TEAMS;
+  const long step = (long)gridDim.x * TEAMS * RPT;
   // (the loop's trip count is the same for every team of a workgroup: team_sum's barriers are reached by all)
-  for (long rb = (long)blockIdx.x * TEAMS; rb < R; rb += step) {
-    const long r = rb + team;
-    const bool live = r < R;
-    float d[NV][V], xh[NV][V];
+  for (long rb = (long)blockIdx.x * TEAMS * RPT; rb < R; rb += step) {
+    float d[RPT][NV][V], xh[RPT][NV][V], m[RPT], rs[RPT], s1[RPT], s2[RPT];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * L + lane) * V;
-      load_part<T>(x + r * ldx + c, live ? C - c : 0, xh[j]);
-      load_part<T>(dy + r * C + c, live ? C - c : 0, d[j]);
-    }
-    const float m = live ? mean[r] : 0.f, rs = live ? rstd[r] : 0.f;
-    float s1 = 0.f, s2 = 0.f;
+    for (int k = 0; k < RPT; ++k) {
+      const long r = rb + k * TEAMS + team;
+      const bool live = r < R;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        xh[j][i] = (xh[j][i] - m) * rs;   // (places behind the row have d = 0: they add nothing below)
-        const float h = d[j][i] * g[j][i];
-        dg[j][i] += d[j][i] * xh[j][i];
-        db[j][i] += d[j][i];
-        s1 += h;
-        s2 += h * xh[j][i];
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * L + lane) * V;
+        load_part<T>(x + r * ldx + c, live ? C - c : 0, xh[k][j]);
+        load_part<T>(dy + r * C + c, live ? C - c : 0, d[k][j]);
       }
-    s1 = team_sum<L>(s1, sh) * inv;
-    s2 = team_sum<L>(s2, sh) * inv;
+      m[k] = live ? mean[r] : 0.f;
+      rs[k] = live ? rstd[r] : 0.f;
+    }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * L + lane) * V;
-      float o[V];
+    for (int k = 0; k < RPT; ++k) {
+      s1[k] = s2[k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = rs * (d[j][i] * g[j][i] - s1 - xh[j][i] * s2);
-      store_part<T>(dx + r * C + c, live ? C - c : 0, o);
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          xh[k][j][i] = (xh[k][j][i] - m[k]) * rs[k];   // (places behind the row have d = 0: they add nothing below)
+          const float h = d[k][j][i] * g[j][i];
+          dg[j][i] += d[k][j][i] * xh[k][j][i];
+          db[j][i] += d[k][j][i];
+          s1[k] += h;
+          s2[k] += h * xh[k][j][i];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      s1[k] = team_sum<L>(s1[k], sh) * inv;
+      s2[k] = team_sum<L>(s2[k], sh) * inv;
+    }
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const long r = rb + k * TEAMS + team;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * L + lane) * V;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = rs[k] * (d[k][j][i] * g[j][i] - s1[k] - xh[k][j][i] * s2[k]);
+        store_part<T>(dx + r * C + c, r < R ? C - c : 0, o);
+      }
     }
   }
   if (part == nullptr) return;
@@ -300,27 +348,63 @@ __global__ __launch_bounds__(1024) void layernorm_param_kernel(const float* __re
   }
 }
 
-template <typename T> constexpr int ln_max_c() { return 4096 * Row<T>::V; }   // 1024 lanes x 4 vectors
+// The team that owns rows of n vectors.  Forward: the fewest lanes that hold one with 32 elements a lane, so that rows up to 2048
+// elements need no barrier (fp32, 4099 rows of 1153: 64 lanes x 6 vectors 10 us, 256 lanes x 2 13 us).  Backward: a lane holds five
+// values of each of its columns, so from 128 vectors on fewer of them on more lanes win (fp32, 16384 rows of 2048: 64 lanes x 8 97 us,
+// 256 lanes x 2 83 us) -- and below, one wavefront does (fp32, 87381 rows of 384: 64 x 2 83 us, 256 x 1 122 us).
+constexpr int LN_MAX_C = 16384;
+#define LN_DISPATCH_FWD(CALL)                                    \
+  const int n = cdiv(C, Row<T>::V);                              \
+  if (n <= 16) return CALL(16, 1);                               \
+  if (n <= 32) return CALL(32, 1);                               \
+  if (n <= 64) return CALL(64, 1);                               \
+  if (n <= 128) return CALL(64, 2);                              \
+  if (n <= 192) return CALL(64, 3);                              \
+  if (n <= 256) return CALL(64, 4);                              \
+  if constexpr (Row<T>::V == 4) {                                \
+    if (n <= 384) return CALL(64, 6);                            \
+    if (n <= 512) return CALL(64, 8);                            \
+    if (n <= 1024) return CALL(256, 4);                          \
+    if (n <= 2048) return CALL(1024, 2);                         \
+    return CALL(1024, 4);                                        \
+  } else {                                                       \
+    if (n <= 512) return CALL(256, 2);                           \
+    if (n <= 1024) return CALL(256, 4);                          \
+    return CALL(1024, 2);                                        \
+  }
+#define LN_DISPATCH_BWD(CALL)                                    \
+  const int n = cdiv(C, Row<T>::V);                              \
+  if (n <= 16) return CALL(16, 1);                               \
+  if (n <= 32) return CALL(32, 1);                               \
+  if (n <= 64) return CALL(64, 1);                               \
+  if (n <= 128) return CALL(64, 2);                              \
+  if (n <= 256) return CALL(256, 1);                             \
+  if (n <= 512) return CALL(256, 2);                             \
+  if (n <= 1024) return CALL(512, 2);                            \
+  if constexpr (Row<T>::V == 4) {                                \
+    if (n <= 2048) return CALL(512, 4);                          \
+    return CALL(1024, 4);                                        \
+  } else {                                                       \
+    return CALL(1024, 2);                                        \
+  }
 
-// teams (rows in flight) of a workgroup for rows of C elements, V a vector
-inline int ln_teams(int C, int V) {
-  const int n = cdiv(C, V);
-  return n <= 16 ? 16 : n <= 32 ? 8 : n <= 256 ? 4 : 1;
-}
-// workgroups of the backward pass: enough to fill the chip, but no more than keeps the partial sums small next to the rows
-inline int ln_bwd_blocks(long R, int C, int V) {
-  const int teams = ln_teams(C, V);
+// rows a team takes at once: up to 32 elements a lane in flight
+constexpr int ln_rpt(int V, int NV, int L) { return L > 256 ? 1 : NV * V <= 8 ? 4 : NV * V <= 16 ? 2 : 1; }
+constexpr int ln_bwd_rpt(int V, int NV, int L) { return L <= 64 && NV * V <= 8 ? 2 : 1; }
+
+// workgroups of the backward pass: enough to fill the chip, but few enough that the partial sums (16 C bytes a workgroup, written and
+// read) stay a sixth of the rows' 3 R C elem bytes
+inline int ln_bwd_blocks(long R, int teams, int elem) {
   const long rows = (R + teams - 1) / teams;
-  long nb = rows / 4;
+  long nb = R * elem / 32;
   if (nb > 1024) nb = 1024;
   if (nb < 256) nb = 256;
   return (int)(nb < rows ? nb : rows);
 }
-
 template <typename T, int L, int NV>
 int launch_ln_fwd(const T* x, long ldx, const float* gamma, const float* beta, T* y, float* mean, float* rstd, long R, int C,
                   float eps, hipStream_t st) {
-  constexpr int BLOCK = L > 256 ? L : 256, TEAMS = BLOCK / L, RPT = NV == 1 ? 4 : NV == 2 && L <= 256 ? 2 : 1;
+  constexpr int BLOCK = L > 256 ? L : 256, TEAMS = BLOCK / L, RPT = ln_rpt(Row<T>::V, NV, L);
   if (RPT > 1 && R >= 512L * TEAMS * RPT) {
     const long nb = (R + TEAMS * RPT - 1) / (TEAMS * RPT);
     if (nb > 0x7fffffffL) return INDM_E_SHAPE;
@@ -338,12 +422,16 @@ int launch_ln_fwd(const T* x, long ldx, const float* gamma, const float* beta, T
 template <typename T, int L, int NV>
 int launch_ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const float* mean, const float* rstd, T* dx, float* dgamma,
                   float* dbeta, float* part, long R, int C, hipStream_t st) {
-  constexpr int BLOCK = L > 256 ? L : 256;
-  const int nb = ln_bwd_blocks(R, C, Row<T>::V);
+  constexpr int BLOCK = L > 256 ? L : 256, TEAMS = BLOCK / L, RPT = ln_bwd_rpt(Row<T>::V, NV, L);
+  const int nb = ln_bwd_blocks(R, TEAMS, sizeof(T));
   const bool params = dgamma != nullptr || dbeta != nullptr;
   const size_t lds = params && L < 256 ? 2 * (size_t)C * sizeof(float) : 0;   // (at most 2 x 2048 floats: four teams of 64 lanes)
-  hipLaunchKernelGGL((layernorm_bwd_kernel<T, L, NV>), dim3(nb), dim3(BLOCK), lds, st, dy, x, ldx, gamma, mean, rstd, dx,
-                     params ? part : nullptr, R, C);
+  if (R >= (long)nb * TEAMS * RPT)
+    hipLaunchKernelGGL((layernorm_bwd_kernel<T, L, NV, RPT>), dim3(nb), dim3(BLOCK), lds, st, dy, x, ldx, gamma, mean, rstd, dx,
+                       params ? part : nullptr, R, C);
+  else
+    hipLaunchKernelGGL((layernorm_bwd_kernel<T, L, NV, 1>), dim3(nb), dim3(BLOCK), lds, st, dy, x, ldx, gamma, mean, rstd, dx,
+                       params ? part : nullptr, R, C);
   if (hipGetLastError() != hipSuccess) return INDM_E_LAUNCH;
   if (params) {
     hipLaunchKernelGGL(layernorm_param_kernel, dim3(cdiv(2L * C, 32)), dim3(1024), 0, st, part, dgamma, dbeta, nb, C);
@@ -352,35 +440,22 @@ int launch_ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const f
   return INDM_OK;
 }
 
-// the team and its vectors a lane: the fewest lanes that hold the row (ln_teams follows the same steps)
-#define LN_DISPATCH(CALL)                                  \
-  const int n = cdiv(C, Row<T>::V);                        \
-  if (n <= 16) return CALL(16, 1);                         \
-  if (n <= 32) return CALL(32, 1);                         \
-  if (n <= 64) return CALL(64, 1);                         \
-  if (n <= 128) return CALL(64, 2);                        \
-  if (n <= 256) return CALL(64, 4);                        \
-  if (n <= 512) return CALL(256, 2);                       \
-  if (n <= 1024) return CALL(256, 4);                      \
-  if (n <= 2048) return CALL(1024, 2);                     \
-  return CALL(1024, 4);
-
 template <typename T>
 int ln_fwd(const T* x, long ldx, const float* gamma, const float* beta, T* y, float* mean, float* rstd, long R, int C, float eps,
            hipStream_t st) {
-  if (R < 0 || C <= 0 || C > ln_max_c<T>() || ldx < 0) return INDM_E_SHAPE;
+  if (R < 0 || C <= 0 || C > LN_MAX_C || ldx < 0) return INDM_E_SHAPE;
   if ((mean == nullptr) != (rstd == nullptr)) return INDM_E_ARG;
   if (R == 0) return INDM_OK;
   if (x == nullptr || y == nullptr) return INDM_E_ARG;
 #define LN_FWD(L, NV) launch_ln_fwd<T, L, NV>(x, ldx, gamma, beta, y, mean, rstd, R, C, eps, st)
-  LN_DISPATCH(LN_FWD)
+  LN_DISPATCH_FWD(LN_FWD)
 #undef LN_FWD
 }
 
 template <typename T>
 int ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const float* mean, const float* rstd, T* dx, float* dgamma,
            float* dbeta, float* ws, long R, int C, hipStream_t st) {
-  if (R < 0 || C <= 0 || C > ln_max_c<T>() || ldx < 0) return INDM_E_SHAPE;
+  if (R < 0 || C <= 0 || C > LN_MAX_C || ldx < 0) return INDM_E_SHAPE;
   if (R == 0) {   // the gradients of no rows are zeros
     if (dgamma == nullptr && dbeta == nullptr) return INDM_OK;
     hipLaunchKernelGGL(layernorm_param_kernel, dim3(cdiv(2L * C, 32)), dim3(1024), 0, st, ws, dgamma, dbeta, 0, C);
@@ -389,25 +464,44 @@ int ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const float* m
   if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || dx == nullptr) return INDM_E_ARG;
   if ((dgamma != nullptr || dbeta != nullptr) && ws == nullptr) return INDM_E_ARG;
 #define LN_BWD(L, NV) launch_ln_bwd<T, L, NV>(dy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, ws, R, C, st)
-  LN_DISPATCH(LN_BWD)
+  LN_DISPATCH_BWD(LN_BWD)
 #undef LN_BWD
 }
 
+template <typename T>
+long ln_ws(long R, int C) {
+#define LN_WS(L, NV) (long)ln_bwd_blocks(R, L > 256 ? 1 : 256 / L, sizeof(T)) * 2 * C
+  LN_DISPATCH_BWD(LN_WS)
+#undef LN_WS
+}
+
 // ------------------------------------------------------------------------------------------------ dropout
-// factors of the 4 elements of flat quad idx4: the mask of the fused GroupNorm + dropout (norm_act.hip: same seed, same mask)
-__device__ __forceinline__ void keep4(uint64_t seed, uint64_t idx4, float p, bool (&k)[4]) {
-  const uint4 r = philox4x32(make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)),
-                             make_uint4((uint32_t)idx4, (uint32_t)(idx4 >> 32), 0u, 0u));
-  k[0] = u32_to_unit(r.x) > p;
-  k[1] = u32_to_unit(r.y) > p;
-  k[2] = u32_to_unit(r.z) > p;
-  k[3] = u32_to_unit(r.w) > p;
+// which of the 4 elements of flat quad idx4 stay: the mask of the fused GroupNorm + dropout (norm_act.hip: same seed, same mask).
+// There an element stays when ((word >> 8) + 1) 2^-24 > p, whose left side is exact: that is word >> 8 >= floor(p 2^24) = drop.
+// (Each round's products are written as 64-bit ones: one instruction instead of a high and a low half.)
+__device__ __forceinline__ void keep4(uint64_t seed, uint64_t idx4, uint32_t drop, bool (&k)[4]) {
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+  uint32_t c0 = (uint32_t)idx4, c1 = (uint32_t)(idx4 >> 32), c2 = 0u, c3 = 0u;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  k[0] = (c0 >> 8) >= drop;
+  k[1] = (c1 >> 8) >= drop;
+  k[2] = (c2 >> 8) >= drop;
+  k[3] = (c3 >> 8) >= drop;
 }
 
 // y = (res) + keep x / (1 - p).  A dropped element is 0 whatever x holds there (also an infinity or a NaN).
 template <typename T, bool RES>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, long n,   // (y may be x or res)
-                                                      float p, float factor, uint64_t seed, const uint64_t* seed_dev) {
+                                                      uint32_t drop, float factor, uint64_t seed, const uint64_t* seed_dev) {
   constexpr int V = Row<T>::V;
   if (seed_dev) seed += *seed_dev;
   const long nv = (n + V - 1) / V;
@@ -420,7 +514,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, 
 #pragma unroll
     for (int h = 0; h < V; h += 4) {
       bool k[4];
-      keep4(seed, (uint64_t)i * (V / 4) + h / 4, p, k);
+      keep4(seed, (uint64_t)i * (V / 4) + h / 4, drop, k);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         o[h + e] = k[e] ? v[h + e] * factor : 0.f;
@@ -437,12 +531,13 @@ int dropout(const T* x, const T* res, T* y, long n, float p, uint64_t seed, cons
   if (!(p >= 0.f && p <= 1.f)) return INDM_E_ARG;
   if (n == 0) return INDM_OK;
   if (x == nullptr || y == nullptr) return INDM_E_ARG;
-  const float factor = p < 1.f ? 1.f / (1.f - p) : 0.f;   // p = 1 drops every element (no uniform of (0, 1] is larger)
+  const float factor = p < 1.f ? 1.f / (1.f - p) : 0.f;   // p = 1 drops every element: word >> 8 < 2^24
+  const uint32_t drop = (uint32_t)(p * 16777216.f);
   const int grid = ew_grid((n + Row<T>::V - 1) / Row<T>::V, 256);
   if (res != nullptr)
-    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3(grid), dim3(256), 0, st, x, res, y, n, p, factor, seed, seed_dev);
+    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3(grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
   else
-    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3(grid), dim3(256), 0, st, x, res, y, n, p, factor, seed, seed_dev);
+    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3(grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
@@ -451,8 +546,11 @@ int dropout(const T* x, const T* res, T* y, long n, float p, uint64_t seed, cons
 // pos[token][axis of the pair's section] * freqs[pair]; the rest passes through.  A pair of a section of n entries at offset o is
 // (o + j, o + n/2 + j), or (o + 2 j, o + 2 j + 1) when interleaved.  The angle is formed and reduced to a quadrant in 64 bits
 // (a far position times a frequency needs more than fp32's 24 bits), its sine and cosine on [-pi/4, pi/4] in fp32.
-// A thread owns one vector (V entries) of a token's heads: it computes their sines once and applies them to HPT heads of q and k.
-constexpr int ROT_AXES = 8;
+// A workgroup takes tb tokens: their sines and cosines go to LDS once (one 64-bit angle a thread, not one per head), then its
+// lanes stream over the tokens' vectors (V entries of a head) in memory order -- the heads of a token are one contiguous run.
+// The mate of a vector whose entries all lie in one half of a section is one more (cached) vector load; a vector that a border
+// cuts takes its mates one by one.
+constexpr int ROT_AXES = 8, ROT_MAX_D = 4096;
 
 struct RotArgs {
   const void* x[2];   // q, k: [B, T, heads, D] with these strides (elements), D contiguous
@@ -463,88 +561,151 @@ struct RotArgs {
   long pos_sb;        // 0: shared by the batch
   const double* freqs;
   long B, T;
-  int D, axes, hpt, hchunks;
+  int D, axes, tb;
   int end[ROT_AXES];  // end offset of each section
   float sign;         // -1: the inverse rotation (the backward pass)
 };
 
-template <typename T, typename P, bool INTER>
-__global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
-  constexpr int V = Row<T>::V;
-  const int nvec = (a.D + V - 1) / V;
-  const long per = (long)nvec * a.hchunks;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.B * a.T * per) return;
-  const long tok = i / per;
-  const int rest = (int)(i - tok * per);
-  const int hc = rest / nvec, d0 = (rest - hc * nvec) * V;
-  const long b = tok / a.T, t = tok - b * a.T;
-  const int left = a.D - d0 < V ? a.D - d0 : V;
-  const P* pos = (const P*)a.pos + b * a.pos_sb + t * a.axes;
-
-  float c[V], s[V];
-  int mate[V];        // offset of the pair's other entry, 0: passes through
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int d = d0 + e;
-    int ax = -1, start = 0, from = 0, size = 0;
-    for (int k = 0; k < a.axes; ++k) {
-      if (ax < 0 && d < a.end[k]) {
-        ax = k;
-        start = from;
-        size = a.end[k] - from;
-      }
-      from = a.end[k];
+// entry d of a head: its pair, the offset of the pair's other entry (0: passes through) and whether it is the second
+struct RotEntry {
+  int pair, mate;
+  bool second;
+};
+template <bool INTER>
+__device__ __forceinline__ RotEntry rot_entry(const RotArgs& a, int d) {
+  int from = 0;
+  for (int k = 0; k < a.axes; ++k) {
+    const int end = a.end[k];
+    if (d < end) {
+      const int in = d - from, half = (end - from) >> 1;
+      if (INTER) return {(d >> 1), (in & 1) ? -1 : 1, (in & 1) != 0};
+      return in < half ? RotEntry{(from >> 1) + in, half, false} : RotEntry{(from >> 1) + in - half, -half, true};
     }
-    c[e] = 1.f;
-    s[e] = 0.f;
-    mate[e] = 0;
-    if (ax >= 0 && e < left) {
-      const int in = d - start, half = size / 2;
-      const bool second = INTER ? (in & 1) : in >= half;
-      const int j = INTER ? in >> 1 : second ? in - half : in;
-      mate[e] = INTER ? (second ? -1 : 1) : second ? -half : half;
-      const double quarter = (double)pos[ax] * a.freqs[start / 2 + j] * 0.63661977236758134308;   // angle in units of pi / 2
-      const double q = __builtin_rint(quarter);
-      float sn, cs;
-      indm_sincos_quadrant((float)((quarter - q) * 1.57079632679489661923), (int)(q - 4.0 * __builtin_floor(q * 0.25)), sn, cs);
-      c[e] = cs;
-      s[e] = (second ? sn : -sn) * a.sign;
+    from = end;
+  }
+  return {0, 0, false};
+}
+
+template <typename T, typename P, bool INTER>
+__global__ __launch_bounds__(512) void rotary_kernel(RotArgs a) {
+  constexpr int V = Row<T>::V, U = 4;   // tokens a lane has in flight
+  // [tb][pairs] (cos, sin); a token's offsets in q and k; a vector's first pair and mate; the list of the vectors that are cut
+  extern __shared__ __attribute__((aligned(16))) float2 turn[];
+  __shared__ int ncut;
+  const int nvec = (a.D + V - 1) / V, hq = a.heads[0], heads = hq + a.heads[1], pairs = a.end[a.axes - 1] >> 1;
+  long2* place = (long2*)(turn + (a.tb * pairs + 1) / 2 * 2);
+  int2* kind = (int2*)(place + a.tb);
+  int* cut = (int*)(kind + nvec);
+  const long tok0 = (long)blockIdx.x * a.tb, tokens = a.B * a.T;
+  const int nt = tokens - tok0 < a.tb ? (int)(tokens - tok0) : a.tb;
+  if (threadIdx.x == 0) ncut = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < nt * pairs; i += blockDim.x) {
+    const int t = i / pairs, j = i - t * pairs;
+    int ax = 0;
+    while (2 * j >= a.end[ax]) ++ax;    // (pairs never straddle sections; j < pairs, so ax < axes)
+    const long b = (tok0 + t) / a.T;
+    const P pos = ((const P*)a.pos)[b * a.pos_sb + (tok0 + t - b * a.T) * a.axes + ax];
+    const double quarter = (double)pos * a.freqs[j] * 0.63661977236758134308;   // the angle in units of pi / 2
+    const double q = __builtin_rint(quarter);
+    float sn, cs;
+    indm_sincos_quadrant((float)((quarter - q) * 1.57079632679489661923), (int)(q - 4.0 * __builtin_floor(q * 0.25)), sn, cs);
+    turn[i] = make_float2(cs, sn * a.sign);
+  }
+  for (int t = threadIdx.x; t < nt; t += blockDim.x) {
+    const long b = (tok0 + t) / a.T, at = tok0 + t - b * a.T;
+    place[t] = make_long2(b * a.sb[0] + at * a.st[0], b * a.sb[1] + at * a.st[1]);
+  }
+  // a vector: (its first pair, how far the mates are); (0, 0) passes through; (-1, 0) cut by a border, or the last, partial one
+  for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+    const int d0 = v * V;
+    const RotEntry first = rot_entry<INTER>(a, d0);
+    bool same = d0 + V <= a.D;
+    for (int e = 1; e < V && same; ++e) {
+      const RotEntry o = rot_entry<INTER>(a, d0 + e);
+      same = INTER ? (o.mate == 0) == (first.mate == 0) : o.mate == first.mate;
+    }
+    kind[v] = same ? make_int2(first.pair, first.mate) : make_int2(-1, 0);
+    if (!same) cut[atomicAdd(&ncut, 1)] = v;   // (their order does not matter: each is worked on by itself)
+  }
+  __syncthreads();
+
+  const T *xq = (const T*)a.x[0], *xk = (const T*)a.x[1];
+  T *yq = (T*)a.y[0] + tok0 * hq * a.D, *yk = (T*)a.y[1] + tok0 * (heads - hq) * a.D;
+  // a lane keeps its vector and head and takes every subs-th token: only the token's offset and its sines change
+  const int per = heads * nvec, width = per < (int)blockDim.x ? per : (int)blockDim.x, subs = blockDim.x / width;
+  const int sub = threadIdx.x / width;
+  for (int i = threadIdx.x - sub * width; i < per && sub < subs; i += width) {
+    const int h = i / nvec, v = i - h * nvec;
+    const int2 kd = kind[v];
+    if (kd.x < 0) continue;
+    const bool isq = h < hq;
+    const int hw = isq ? h : h - hq, stride = (isq ? hq : heads - hq) * a.D;
+    const T* x = (isq ? xq : xk) + hw * (isq ? a.sh[0] : a.sh[1]) + v * V;
+    T* y = (isq ? yq : yk) + hw * a.D + v * V;
+    const long* at = (const long*)place + (isq ? 0 : 1);
+    const unsigned flip = kd.y > 0 ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;   // the first of a pair takes minus its mate
+    for (int t = sub; t < nt; t += subs * U) {
+      typename Row<T>::raw own[U], mate[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int tu = t + u * subs;
+        if (tu < nt) {
+          const T* src = x + at[2 * tu];
+          own[u] = Row<T>::load(src);
+          if (!INTER && kd.y != 0) mate[u] = Row<T>::load(src + kd.y);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int tu = t + u * subs;
+        if (tu < nt) {
+          T* dst = y + tu * stride;
+          if (kd.y == 0) {
+            *(typename Row<T>::raw*)dst = own[u];
+          } else {
+            const float2* tr = turn + tu * pairs + kd.x;
+            float p[V], o[V];
+            Row<T>::unpack(own[u], p);
+            if constexpr (INTER) {
+#pragma unroll
+              for (int e = 0; e < V; e += 2) {
+                const float2 cs = tr[e >> 1];
+                o[e] = __builtin_fmaf(p[e], cs.x, -p[e + 1] * cs.y);
+                o[e + 1] = __builtin_fmaf(p[e + 1], cs.x, p[e] * cs.y);
+              }
+            } else {
+              float m[V];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mate[u][e] ^= flip;
+              Row<T>::unpack(mate[u], m);
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float2 cs = tr[e];
+                o[e] = __builtin_fmaf(p[e], cs.x, m[e] * cs.y);
+              }
+            }
+            Row<T>::store(dst, o);
+          }
+        }
+      }
     }
   }
-  // the mates of a whole vector are a whole vector when all lie equally far: one more (cached) vector load
-  bool same = left == V;
-#pragma unroll
-  for (int e = 1; e < V; ++e) same = same && mate[e] == mate[0];
-
-  const int total = a.heads[0] + a.heads[1];
-  const int h0 = hc * a.hpt, h1 = h0 + a.hpt < total ? h0 + a.hpt : total;
-#pragma unroll 4
-  for (int hh = h0; hh < h1; ++hh) {
-    const int w = hh < a.heads[0] ? 0 : 1;
-    const int h = w == 0 ? hh : hh - a.heads[0];
-    const T* x = (const T*)a.x[w] + b * a.sb[w] + t * a.st[w] + h * a.sh[w] + d0;
-    T* y = (T*)a.y[w] + ((b * a.T + t) * a.heads[w] + h) * a.D + d0;
-    float v[V], o[V];
-    load_part<T>(x, left, v);
-    if constexpr (INTER) {   // the sections are even: both entries of a pair are in this vector
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = mate[e] == 0 ? v[e] : v[e] * c[e] + v[e ^ 1] * s[e];
-    } else if (same) {
-      if (mate[0] == 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = v[e];
+  // the cut vectors, entry by entry
+  const int entries = nt * heads * ncut * V;
+  for (int i = threadIdx.x; i < entries; i += blockDim.x) {
+    const int e = i % V, c = i / V % ncut, th = i / V / ncut, h = th % heads, t = th / heads, d = cut[c] * V + e;
+    if (d < a.D) {
+      const RotEntry r = rot_entry<INTER>(a, d);
+      const T* src = h < hq ? xq + place[t].x + h * a.sh[0] + d : xk + place[t].y + (h - hq) * a.sh[1] + d;
+      T* dst = h < hq ? yq + (t * hq + h) * a.D + d : yk + (t * (heads - hq) + h - hq) * a.D + d;
+      if (r.mate == 0) {
+        *dst = *src;
       } else {
-        float u[V];
-        Row<T>::unpack(Row<T>::load(x + mate[0]), u);
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = v[e] * c[e] + u[e] * s[e];
+        const float2 cs = turn[t * pairs + r.pair];
+        Row<T>::put(dst, __builtin_fmaf(Row<T>::get(src), cs.x, Row<T>::get(src + r.mate) * (r.second ? cs.y : -cs.y)));
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = mate[e] == 0 ? v[e] : v[e] * c[e] + Row<T>::get(x + e + mate[e]) * s[e];
     }
-    store_part<T>(y, left, o);
   }
 }
 
@@ -552,7 +713,7 @@ template <typename T>
 int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, long Tn, int H, int Hk, int D, const void* pos,
            int pos_type, long pos_sb, const double* freqs, const int* sections, int axes, int interleaved, int inverse,
            hipStream_t st) {
-  if (B < 0 || Tn < 0 || H < 0 || Hk < 0 || D <= 0 || axes <= 0 || axes > ROT_AXES) return INDM_E_SHAPE;
+  if (B < 0 || Tn < 0 || H < 0 || Hk < 0 || D <= 0 || D > ROT_MAX_D || axes <= 0 || axes > ROT_AXES) return INDM_E_SHAPE;
   if (strides == nullptr || sections == nullptr || pos_type < 0 || pos_type > 2) return INDM_E_ARG;
   RotArgs a = {};
   int at = 0;
@@ -570,17 +731,34 @@ int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, lon
   a.heads[0] = H; a.heads[1] = Hk;
   a.pos = pos; a.pos_sb = pos_sb; a.freqs = freqs; a.B = B; a.T = Tn; a.D = D; a.axes = axes;
   a.sign = inverse ? -1.f : 1.f;
-  // heads a thread: all of them when the tokens fill the chip, else fewer
-  const int nvec = cdiv(D, Row<T>::V), total = H + Hk;
-  a.hpt = total;
-  while (a.hpt > 1 && (long)B * Tn * nvec * cdiv(total, a.hpt) < 256L * 1024) a.hpt = (a.hpt + 1) / 2;
-  a.hchunks = cdiv(total, a.hpt);
-  const long nb = ((long)B * Tn * nvec * a.hchunks + 255) / 256;
-  if (nb > 0x7fffffffL) return INDM_E_SHAPE;
+  // lanes: as many whole tokens as fill wavefronts best (up to 512 lanes; a token of more vectors is walked in several steps)
+  const int nvec = cdiv(D, Row<T>::V), pairs = at / 2;
+  const long per = (long)(H + Hk) * nvec, tokens = (long)B * Tn;
+  int lanes = 256;
+  if (per <= 512) {
+    double best = 0.;
+    for (int k = 1; k * per <= 512; ++k) {
+      const int n = (int)(k * per + 63) / 64 * 64;
+      const double full = (double)(k * per) / n * (n >= 256 ? 1. : n >= 128 ? 0.97 : 0.9);   // (few wavefronts share the sines badly)
+      if (full > best + 1e-9) {
+        best = full;
+        lanes = n;
+      }
+    }
+  }
+  // tokens a workgroup: 8 a lane where that still makes 1024 workgroups, down to one; the sines fit 32 KB of LDS
+  long tb = per <= lanes ? lanes / per * 8 : 8;
+  if (tb > 64) tb = 64;
+  while (tb > 1 && (tokens + tb - 1) / tb < 1024) tb = (tb + 1) / 2;
+  while (tb > 1 && tb * pairs * (long)sizeof(float2) > 32768) tb = (tb + 1) / 2;
+  a.tb = (int)tb;
+  const size_t lds = ((size_t)tb * pairs + 1) / 2 * 2 * sizeof(float2) + tb * sizeof(long2) + nvec * (sizeof(int2) + sizeof(int));
+  const long nb = (tokens + tb - 1) / tb;
+  if (nb > 0x7fffffffL || per * tb > 0x3fffffffL) return INDM_E_SHAPE;
 #define ROT_LAUNCH(P)                                                                                             \
   do {                                                                                                            \
-    if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, P, true>), dim3((unsigned)nb), dim3(256), 0, st, a);    \
-    else hipLaunchKernelGGL((rotary_kernel<T, P, false>), dim3((unsigned)nb), dim3(256), 0, st, a);               \
+    if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, P, true>), dim3((unsigned)nb), dim3(lanes), lds, st, a);  \
+    else hipLaunchKernelGGL((rotary_kernel<T, P, false>), dim3((unsigned)nb), dim3(lanes), lds, st, a);             \
   } while (0)
   if (pos_type == 0) ROT_LAUNCH(int);
   else if (pos_type == 1) ROT_LAUNCH(float);
@@ -603,7 +781,7 @@ INDM_API int indm_layernorm_fwd_bf16(const void* x, long ldx, const float* gamma
 
 INDM_API long indm_layernorm_bwd_ws_floats(long R, int C, int elem_bytes) {
   if (R <= 0 || C <= 0 || (elem_bytes != 2 && elem_bytes != 4)) return 0;
-  return (long)ln_bwd_blocks(R, C, 16 / elem_bytes) * 2 * C;
+  return elem_bytes == 4 ? ln_ws<float>(R, C) : ln_ws<unsigned short>(R, C);
 }
 INDM_API int indm_layernorm_bwd_f32(const float* dy, const float* x, long ldx, const float* gamma, const float* mean,
                                     const float* rstd, float* dx, float* dgamma, float* dbeta, float* ws, long R, int C,

@@ -2241,7 +2241,7 @@ def _rows2d(x):
     return x.contiguous(), R, C
 
 
-_LN_MAX_C = {torch.float32: 16384, torch.bfloat16: 32768}
+_LN_MAX_C = 16384
 
 
 def _ln_check(x, gamma, beta, eps):
@@ -2250,8 +2250,8 @@ def _ln_check(x, gamma, beta, eps):
     if x.dim() < 1 or x.shape[-1] < 1:
         _refuse(f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
     C = x.shape[-1]
-    if C > _LN_MAX_C[x.dtype]:
-        _refuse(f"layer_norm: rows of up to {_LN_MAX_C[x.dtype]} {x.dtype} elements, got {C}")
+    if C > _LN_MAX_C:
+        _refuse(f"layer_norm: rows of up to {_LN_MAX_C} elements, got {C}")
     for p in (gamma, beta):
         if p is not None and (p.dtype != torch.float32 or p.shape != (C,)):
             name = "gamma" if p is gamma else "beta"
@@ -2352,6 +2352,8 @@ def _rotary_check(q, k, pos, freqs, sections):
     if q.dim() != 4:
         _refuse(f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
     B, T, _, D = q.shape
+    if D > 4096:
+        _refuse(f"rotary: heads of up to 4096 entries, got {D}")
     if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D):
         _refuse(f"rotary: k is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
     A, R = len(sections), sum(sections)
