@@ -42,9 +42,10 @@ struct WAttnArgs {
   void *out, *dq, *dk, *dv;         // dense
   float* lse;                       // [B, H, T]: log2 of the sum of exponentials, in units of the exp2 argument
   float* delta;                     // [B, H, T]: <dO, o>
-  float* part;                      // sink partials [B Hk][chunks][32 key blocks][2][D]
+  float* part;                      // sink partials [B Hk][chunks][sinks][2][D]
+  float* split;                     // partial dk, dv [splits][B Hk][T][2][D]
   const int* lengths;               // [B] or NULL
-  int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks;
+  int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks, splits;
   float c, scale;                   // scale * log2(e), scale
 };
 
@@ -59,7 +60,7 @@ struct Geo {
   static constexpr int RB = NCH * 16;                              // bytes of a row in LDS
   static constexpr int BN = sizeof(T) == 2 ? 64 : 32, NY = BN / 32;   // streamed tokens a tile
   static constexpr int TILE = BN * RB;
-  static constexpr int KK = DP / 16, DB = DP / 32;
+  static constexpr int KK = DP / 16, DB = (DP + 31) / 32;     // 16-element steps of a product over d, blocks of 32 output elements
   // LDS address of chunk c of row r: c ^ swz(r).  16 successive rows at one chunk (the row-wise operand reads) and four
   // successive rows at one 64-byte unit (the transposed ones) then fall on different banks.
   static __device__ __forceinline__ int swz(int r) {
@@ -67,10 +68,12 @@ struct Geo {
   }
 };
 
-// wavefronts a SIMD that the register allocation aims at (kind 0: forward, 1: dq, 2: dk / dv).  512 registers a SIMD lane over 4, 3, 2 or
-// 1: what fits without spilling
-constexpr int waves_per_simd(int size, int DP, int kind) {
-  return size == 2 ? (DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : 2) : DP <= 32 ? 3 : DP <= 64 ? (kind == 0 ? 3 : 2) : DP <= 96 && kind == 0 ? 2 : 1;
+// wavefronts a SIMD that the register allocation aims at (kind 0: forward, 1: dq, 2: dk / dv): 512 registers a SIMD lane over 4, 3, 2 or
+// 1, what fits without spilling.  Workgroups of one wavefront are few by their own rule: 2 or 1.
+constexpr int waves_per_simd(int size, int DP, int kind, int WV) {
+  if (WV == 1) return DP <= (size == 2 ? 80 : 48) || (kind == 0 && size == 2) ? 2 : 1;
+  if (size == 2) return DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : 2;
+  return DP <= 32 ? 3 : DP <= 64 ? (kind == 0 ? 3 : 2) : DP <= 96 && kind == 0 ? 2 : 1;
 }
 
 template <typename T> struct Op;
@@ -311,7 +314,7 @@ __device__ __forceinline__ KeyTiles key_tiles(const WAttnArgs& p, int q0, int q1
 
 // ---------------------------------------------------------------------------------------------- owner = queries: forward, dq
 template <typename T, int DP, int WV, bool BWD>
-__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0)) void wattn_query_kernel(WAttnArgs p) {
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0, WV)) void wattn_query_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
@@ -491,26 +494,29 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0)
 }
 
 // ---------------------------------------------------------------------------------------------- owner = keys: dk, dv
-// The queries of every head of the group stream past the key.  SINK = false: the window's part of all keys.  SINK = true: what the sink
-// keys get from queries whose window they are outside of -- a few keys against all queries, so the queries are split over p.chunks
-// workgroups whose fp32 partial sums the first kind adds up in order (no atomics).
-template <typename T, int DP, int WV, bool SINK>
-__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wattn_key_kernel(WAttnArgs p) {
+// The queries of every head of the group stream past the key.  WHOLE: the window's part of all keys.  SPLIT: the same where there are
+// few key blocks, their queries shared by p.splits workgroups that leave fp32 partial sums.  SINK: what the sink keys get from queries
+// whose window they are outside of -- a few keys against all queries, shared by p.chunks workgroups.  Partial sums are added up in
+// order (no atomics).
+enum { WHOLE = 0, SPLIT = 1, SINKS = 2 };
+template <typename T, int DP, int WV, int MODE>
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void wattn_key_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
+  constexpr bool SINK = MODE == SINKS;
   constexpr int BUF = 2 * G::TILE + 2 * G::BN * (int)sizeof(float);
   extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile, dO tile, lse, delta]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<T, DP> at(lane);
   const int item = xcd_item(blockIdx.x, gridDim.x);
-  const int per = SINK ? p.tiles * p.chunks : p.tiles;
+  const int shares = SINK ? p.chunks : MODE == SPLIT ? p.splits : 1, per = p.tiles * shares;
   const int bh = item / per, hk = bh % p.Hk, b = bh / p.Hk;
-  const int chunk = SINK ? item % per % p.chunks : 0, tile = SINK ? item % per / p.chunks : item % per;
+  const int share = item % per % shares, tile = item % per / shares;
   const int n = seq_len(p, b), group = p.H / p.Hk;
   const int j0 = tile * (WV * 32), jw = j0 + wave * 32, j = jw + at.l31;
   const bool live = j < n;
-  // tiles of queries: i0 .. i1 of each head of the group, one after the other (SINK: this chunk's share of all of them)
+  // tiles of queries: i0 .. i1 of each head of the group, one after the other, of which this workgroup takes its share
   int i0, i1;
   if constexpr (SINK) {
     i0 = p.causal ? j0 : 0;
@@ -522,11 +528,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wat
     i1 = i1 > n - 1 ? n - 1 : i1;
   }
   const int t0 = i0 / G::BN, nt = j0 < n && i1 >= i0 ? i1 / G::BN - t0 + 1 : 0;
-  int from = 0, to = nt * group;
-  if constexpr (SINK) {
-    from = (int)((long)to * chunk / p.chunks);
-    to = (int)((long)to * (chunk + 1) / p.chunks);
-  }
+  const int all_tiles = nt * group, from = (int)((long)all_tiles * share / shares), to = (int)((long)all_tiles * (share + 1) / shares);
   const Stager<T, DP, WV> qs(p.qt, wave, lane), ds((long)p.H * p.D, wave, lane);
   float hold[2];
   auto fetch = [&](int it) {
@@ -600,17 +602,20 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wat
       for (int r = 0; r < 16; ++r) P[r] = dP[r] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < G::KK; ++kk) P = O::mma(at.rowwise(qb, y, kk), kf[kk], P);
-      const unsigned at0 = (unsigned)(ia + 4 * at.lhi - lo);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         const f32x4 l4 = *(const f32x4*)(st + 32 * y + 8 * a + 4 * at.lhi);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * a + e;
-          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(P[r], p.c, -l4[e]));
-          if constexpr (SINK) w = ia + 4 * at.lhi + 8 * a + e <= last && at0 + 8 * a + e > span ? w : 0.f;
-          else if (!all) w = at0 + 8 * a + e <= span ? w : 0.f;
-          P[r] = w;
+        for (int e = 0; e < 4; ++e) P[4 * a + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(P[4 * a + e], p.c, -l4[e]));
+      }
+      if (!all) {
+        asm volatile("" ::: "memory");   // (keeps the masks behind the branch)
+        const unsigned at0 = (unsigned)(ia + 4 * at.lhi - lo);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = 8 * (r >> 2) + (r & 3);
+          if constexpr (SINK) P[r] = ia + 4 * at.lhi + i <= last && at0 + i > span ? P[r] : 0.f;
+          else P[r] = at0 + i <= span ? P[r] : 0.f;
         }
       }
 #pragma unroll
@@ -639,10 +644,13 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wat
   }
 
   if constexpr (SINK) {
-    // part[bh][chunk][key of the sink tiles][dk, dv][D]
-    float* row = p.part + ((((long)bh * p.chunks + chunk) * p.tiles * (WV * 32) + j) * 2) * p.D;
-    store_owner<float, DP>(row, dk, 1.f, true, p.D, at.lhi);
-    store_owner<float, DP>(row + p.D, dv, 1.f, true, p.D, at.lhi);
+    float* row = p.part + ((((long)bh * p.chunks + share) * p.sinks + j) * 2) * p.D;
+    store_owner<float, DP>(row, dk, 1.f, j < p.sinks, p.D, at.lhi);
+    store_owner<float, DP>(row + p.D, dv, 1.f, j < p.sinks, p.D, at.lhi);
+  } else if constexpr (MODE == SPLIT) {
+    float* row = p.split + ((((long)share * p.B * p.Hk + bh) * p.T + j) * 2) * p.D;
+    store_owner<float, DP>(row, dk, 1.f, live, p.D, at.lhi);
+    store_owner<float, DP>(row + p.D, dv, 1.f, live, p.D, at.lhi);
   } else {
     if (!live) {
 #pragma unroll
@@ -650,9 +658,8 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wat
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
     }
-    const int sp = (p.sinks + 31) / 32 * 32;
-    if (p.chunks > 0 && jw < sp && live) {   // add what the sink kernel gathered
-      const float* row = p.part + ((long)bh * p.chunks * sp + j) * 2 * p.D;
+    if (p.chunks > 0 && j < p.sinks && live) {   // add what the sink kernel gathered
+      const float* row = p.part + ((long)bh * p.chunks * p.sinks + j) * 2 * p.D;
 #pragma unroll
       for (int d = 0; d < G::DB; ++d)
 #pragma unroll
@@ -674,18 +681,49 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2)) void wat
   }
 }
 
-// the sink partials of each (sequence, key head) added up over the chunks, in order, into chunk 0: a workgroup's lanes own 64 columns
-// of the n = key blocks x 2 D values, its wavefronts a quarter of the chunks each
+// the sink partials of each (sequence, key head) added up over the chunks, in order, into chunk 0: a workgroup's lanes own 64 of the
+// n = sinks x 2 D values, its wavefronts a quarter of the chunks each
 __global__ __launch_bounds__(256) void wattn_join_kernel(float* part, int chunks, int n) {
   __shared__ float sh[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;   // (n is a multiple of 64 x 8)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   float* base = part + (long)blockIdx.y * chunks * n + col;
   float s = 0.f;
+  if (col < n) {
 #pragma unroll 4
-  for (int c = chunks * wave / 4; c < chunks * (wave + 1) / 4; ++c) s += base[(long)c * n];
+    for (int c = chunks * wave / 4; c < chunks * (wave + 1) / 4; ++c) s += base[(long)c * n];
+  }
   sh[wave][lane] = s;
   __syncthreads();
-  if (wave == 0) base[0] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+  if (wave == 0 && col < n) base[0] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+}
+
+// dk, dv = the splits' partial sums, in order, and the sinks' -- four elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void wattn_sum_kernel(WAttnArgs p) {
+  const int d4 = p.D / 4;
+  const long total = (long)p.B * p.T * p.Hk * 2 * d4;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const int d = (int)(i % d4) * 4;
+    const long row = i / d4;                 // ((b T + j) Hk + hk) 2 + which
+    const int which = (int)(row & 1);
+    const long k = row >> 1, hk = k % p.Hk, bj = k / p.Hk, b = bj / p.T;
+    const int j = (int)(bj - b * p.T);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (j < seq_len(p, (int)b)) {
+      const float* src = p.split + (((b * p.Hk + hk) * p.T + j) * 2 + which) * p.D + d;
+      for (int c = 0; c < p.splits; ++c) s += *(const f32x4*)(src + (long)c * p.B * p.Hk * p.T * 2 * p.D);
+      if (p.chunks > 0 && j < p.sinks) s += *(const f32x4*)(p.part + (((b * p.Hk + hk) * p.chunks * p.sinks + j) * 2 + which) * p.D + d);
+      if (which == 0) s *= p.scale;
+    }
+    T* out = (T*)(which == 0 ? p.dk : p.dv) + k * p.D + d;
+    if constexpr (sizeof(T) == 2) {
+      const f32x2 a = {s[0], s[1]}, c = {s[2], s[3]};
+      const u32x2 w = {__builtin_bit_cast(unsigned, __builtin_convertvector(a, bf16x2)), __builtin_bit_cast(unsigned, __builtin_convertvector(c, bf16x2))};
+      *(u32x2*)out = w;
+    } else {
+      *(f32x4*)out = s;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -702,36 +740,58 @@ int run_query(WAttnArgs p, hipStream_t st) {
   p.tiles = cdiv(p.T, WV * 32);
   return launch<wattn_query_kernel<T, DP, WV, BWD>>(p, (long)p.tiles * p.H * p.B, WV * 64, 4 * (size_t)Geo<T, DP>::TILE, st);
 }
-template <typename T, int DP, int WV, bool SINK>
+template <typename T, int DP, int WV, int MODE>
 int run_key(WAttnArgs p, hipStream_t st) {
   using G = Geo<T, DP>;
-  p.tiles = SINK ? cdiv(p.sinks, 32) : cdiv(p.T, WV * 32);
-  return launch<wattn_key_kernel<T, DP, WV, SINK>>(p, (long)p.tiles * (SINK ? p.chunks : 1) * p.Hk * p.B, WV * 64,
+  p.tiles = MODE == SINKS ? cdiv(p.sinks, 32) : cdiv(p.T, WV * 32);
+  return launch<wattn_key_kernel<T, DP, WV, MODE>>(p, (long)p.tiles * (MODE == SINKS ? p.chunks : MODE == SPLIT ? p.splits : 1) * p.Hk * p.B, WV * 64,
                                                    2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
 }
-
 inline int run_join(const WAttnArgs& p, hipStream_t st) {
-  const int n = cdiv(p.sinks, 32) * 64 * p.D;
-  if ((long)p.B * p.Hk > 65535) return INDM_E_SHAPE;
-  hipLaunchKernelGGL(wattn_join_kernel, dim3(n / 64, p.B * p.Hk), dim3(256), 0, st, p.part, p.chunks, n);
+  const int n = p.sinks * 2 * p.D;
+  if ((long)p.B * p.Hk > 65535 || (long)p.sinks * 2 * p.D > 0x7fffffffL) return INDM_E_SHAPE;
+  hipLaunchKernelGGL(wattn_join_kernel, dim3(cdiv(n, 64), p.B * p.Hk), dim3(256), 0, st, p.part, p.chunks, n);
+  return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
+}
+template <typename T>
+int run_sum(const WAttnArgs& p, hipStream_t st) {
+  hipLaunchKernelGGL(wattn_sum_kernel<T>, dim3(ew_grid((long)p.B * p.T * p.Hk * 2 * (p.D / 4), 256)), dim3(256), 0, st, p);
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
-// do the sinks reach queries outside of the window?  (sinks are clamped to T before)
-inline bool sinks_matter(int T, int left, int right, int sinks, int causal) {
-  return sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right));
+// How the work is laid out, from the sizes alone (the scratch is sized by the same rules).
+struct Plan {
+  int chunks, splits;   // workgroups that share a sink block's queries (0: the sinks reach nothing), and a key block's
+  bool one;             // one wavefront a workgroup
+};
+inline Plan plan_keys(int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
+  Plan r = {0, 1, false};
+  // do the sinks reach queries outside of the window?
+  if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
+    const long rows = (long)B * Hk * cdiv(sinks, 32), units = (long)(H / Hk) * cdiv(T, 64);   // of at least one tile each
+    long c = 1024 / rows;
+    c = c < 1 ? 1 : c;
+    r.chunks = (int)(c < units ? c : units);
+  }
+  // few key blocks: share each one's queries among workgroups, as long as that leaves each about four tiles (of all heads of the group)
+  const long blocks = (long)cdiv(T, 128) * Hk * B;
+  if (blocks < 384) {
+    const long reach = (long)(left < T ? left : T) + (causal ? 0 : (right < T ? right : T)) + 128;
+    const long tiles = (long)(H / Hk) * cdiv(reach < T ? reach : T, 64);
+    long s = (512 + blocks - 1) / blocks;
+    if (s > tiles / 4) s = tiles / 4;
+    r.splits = s < 1 ? 1 : (int)s;
+    r.one = blocks * r.splits < 256;
+  }
+  return r;
 }
-inline int sink_chunks(int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
-  if (!sinks_matter(T, left, right, sinks, causal)) return 0;
-  const long rows = (long)B * Hk * cdiv(sinks, 32), units = (long)(H / Hk) * cdiv(T, 64);   // of at least one tile each
-  long c = 1024 / rows;
-  c = c < 1 ? 1 : c;
-  return (int)(c < units ? c : units);
-}
+inline bool one_wave_queries(int B, int T, int H) { return (long)cdiv(T, 128) * H * B < 256; }
 
 #define WA_DISPATCH(CALL)                 \
   if (p.D <= 32) return CALL(32);         \
+  if (p.D <= 48) return CALL(48);         \
   if (p.D <= 64) return CALL(64);         \
+  if (p.D <= 80) return CALL(80);         \
   if (p.D <= 96) return CALL(96);         \
   return CALL(128);
 
@@ -765,16 +825,19 @@ int fwd(WAttnArgs p, const long* strides, void* o, void* olo, float* lse, hipStr
   if (r <= 0) return r;
   if (o == nullptr || (((uintptr_t)o | (uintptr_t)olo) & 15)) return INDM_E_ARG;
   p.out = o; p.olo = olo; p.lse = lse;
-#define WA_FWD(DP) run_query<T, DP, 4, false>(p, st)
+#define WA_FWD(DP) (one_wave_queries(p.B, p.T, p.H) ? run_query<T, DP, 1, false>(p, st) : run_query<T, DP, 4, false>(p, st))
   WA_DISPATCH(WA_FWD)
 }
 
 template <typename T, int DP>
-int bwd_dp(const WAttnArgs& p, hipStream_t st) {
-  int r = run_query<T, DP, 4, true>(p, st);   // dq, and delta for the others
-  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, 1, true>(p, st);
+int bwd_dp(const WAttnArgs& p, bool one, hipStream_t st) {
+  int r = one_wave_queries(p.B, p.T, p.H) ? run_query<T, DP, 1, true>(p, st) : run_query<T, DP, 4, true>(p, st);   // dq, and delta for the others
+  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, 1, SINKS>(p, st);
   if (r == INDM_OK && p.chunks > 1) r = run_join(p, st);
-  if (r == INDM_OK) r = run_key<T, DP, 4, false>(p, st);
+  if (r == INDM_OK)
+    r = p.splits > 1 ? (one ? run_key<T, DP, 1, SPLIT>(p, st) : run_key<T, DP, 4, SPLIT>(p, st))
+                     : (one ? run_key<T, DP, 1, WHOLE>(p, st) : run_key<T, DP, 4, WHOLE>(p, st));
+  if (r == INDM_OK && p.splits > 1) r = run_sum<T>(p, st);
   return r;
 }
 template <typename T>
@@ -786,9 +849,12 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
       (((uintptr_t)o | (uintptr_t)olo | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
   p.o = o; p.olo = const_cast<void*>(olo); p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = ws;
+  const Plan plan = plan_keys(p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
+  p.chunks = plan.chunks;
+  p.splits = plan.splits;
   p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
-  p.chunks = sink_chunks(p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
-#define WA_BWD(DP) bwd_dp<T, DP>(p, st)
+  p.split = p.part + (long)p.B * p.Hk * p.chunks * p.sinks * 2 * p.D;
+#define WA_BWD(DP) bwd_dp<T, DP>(p, plan.one, st)
   WA_DISPATCH(WA_BWD)
 }
 
@@ -810,8 +876,9 @@ INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, co
 INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
   sinks = sinks < T ? sinks : T;
-  const long chunks = sink_chunks(B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal);
-  return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * chunks * cdiv(sinks, 32) * 32 * 2 * D;
+  const Plan plan = plan_keys(B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal != 0);
+  return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * plan.chunks * sinks * 2 * D +
+         (plan.splits > 1 ? (long)plan.splits * B * Hk * T * 2 * D : 0);
 }
 INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const void*,
                                 const float* dO, const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,
