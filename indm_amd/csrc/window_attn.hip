@@ -6,7 +6,9 @@
 //
 // All three kernels (FWD, DQ: the owner is a query; DKV: the owner is a key) have one shape.  A wavefront owns 32 tokens and holds
 // their vectors as matrix-instruction operands in registers; the other side streams through LDS in double-buffered tiles of BN
-// tokens that all wavefronts of the workgroup share.
+// tokens that all wavefronts of the workgroup share.  Where that makes too few workgroups for the chip (SHARE), the wavefronts of a
+// workgroup own the same 32 tokens instead, each streams every WV-th tile through LDS of its own, without barriers, and their partial
+// results are joined in LDS at the end.
 //   S^T[y][x] = sum_d Y[y][d] X[x][d]      A = rows of the tile, B = the owners: lane (l31, lhi) ends up with the owner x = l31 and
 //                                          y = 32 yb + 8 (r >> 2) + (r & 3) + 4 lhi in accumulator register r of block yb -- so a
 //                                          row's maximum and sum are in-lane work and one exchange with lane ^ 32
@@ -69,12 +71,14 @@ struct Geo {
 };
 
 // wavefronts a SIMD that the register allocation aims at (kind 0: forward, 1: dq, 2: dk / dv): 512 registers a SIMD lane over 4, 3, 2 or
-// 1, what fits without spilling.  Workgroups of one wavefront are few by their own rule: 2 or 1.
-constexpr int waves_per_simd(int size, int DP, int kind, int WV) {
-  if (WV == 1) return DP <= (size == 2 ? 80 : 48) || (kind == 0 && size == 2) ? 2 : 1;
+// 1, what fits without spilling.  Workgroups that share an owner block fill a compute unit's LDS: one wavefront a SIMD.
+constexpr int waves_per_simd(int size, int DP, int kind, bool share) {
+  if (share) return 1;
   if (size == 2) return DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : 2;
   return DP <= 32 ? 3 : DP <= 64 ? (kind == 0 ? 3 : 2) : DP <= 96 && kind == 0 ? 2 : 1;
 }
+// wavefronts of a workgroup that shares an owner block: each streams tiles of its own, 128 KB of LDS together
+template <typename T, int DP> constexpr int share_waves() { return Geo<T, DP>::TILE <= 8192 ? 4 : 2; }
 
 template <typename T> struct Op;
 template <> struct Op<u16> {
@@ -231,9 +235,11 @@ struct Stager {
     }
   }
 };
+// this wavefront's copies have landed -- and, where a workgroup shares its tiles, everybody's
+template <bool SHARE>
 __device__ __forceinline__ void staged() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  if constexpr (!SHARE) __syncthreads();
 }
 
 // the owner's row as operands (rows from n on: zeros)
@@ -313,32 +319,35 @@ __device__ __forceinline__ KeyTiles key_tiles(const WAttnArgs& p, int q0, int q1
 }
 
 // ---------------------------------------------------------------------------------------------- owner = queries: forward, dq
-template <typename T, int DP, int WV, bool BWD>
-__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0, WV)) void wattn_query_kernel(WAttnArgs p) {
+template <typename T, int DP, int WV, bool SHARE, bool BWD>
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0, SHARE)) void wattn_query_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][K tile, V tile]
+  constexpr int OWN = SHARE ? 32 : WV * 32, STEP = SHARE ? WV : 1;
+  extern __shared__ __attribute__((aligned(16))) char smem_all[];   // [2 buffers][K tile, V tile], SHARE: for each wavefront
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<T, DP> at(lane);
   const int item = xcd_item(blockIdx.x, gridDim.x);
   const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.H, b = bh / p.H;
   const int n = seq_len(p, b);
-  const int q0 = tile * (WV * 32), qw = q0 + wave * 32, i = qw + at.l31;
+  char* smem = smem_all + (SHARE ? wave * 4 * G::TILE : 0);
+  const int q0 = tile * OWN, qw = q0 + (SHARE ? 0 : wave * 32), i = qw + at.l31;
   const int hk = h / (p.H / p.Hk);
   const T* K = (const T*)p.k + b * p.kb + hk * p.kh;
   const T* V = (const T*)p.v + b * p.vb + hk * p.vh;
   const long orow = (((long)b * p.T + i) * p.H + h) * p.D, srow = ((long)b * p.H + h) * p.T + i;
   const bool live = i < n;
-  const KeyTiles kt = key_tiles(p, q0, q0 + WV * 32 - 1, n, G::BN);
+  const KeyTiles kt = key_tiles(p, q0, q0 + OWN - 1, n, G::BN);
   auto first_of = [&](int it) { return (it < kt.ns ? it : kt.t0 + it - kt.ns) * G::BN; };
-  const Stager<T, DP, WV> ks(p.kt, wave, lane), vs(p.vt, wave, lane);
-  auto fetch = [&](int it) {
-    char* buf = smem + (it & 1) * 2 * G::TILE;
-    ks.fetch(buf, K, p.kt, first_of(it), n, p.D, wave, lane);
-    vs.fetch(buf + G::TILE, V, p.vt, first_of(it), n, p.D, wave, lane);
+  const int swave = SHARE ? 0 : wave, it0 = SHARE ? wave : 0;
+  const Stager<T, DP, SHARE ? 1 : WV> ks(p.kt, swave, lane), vs(p.vt, swave, lane);
+  auto fetch = [&](int it, int side) {
+    char* buf = smem + side * 2 * G::TILE;
+    ks.fetch(buf, K, p.kt, first_of(it), n, p.D, swave, lane);
+    vs.fetch(buf + G::TILE, V, p.vt, first_of(it), n, p.D, swave, lane);
   };
-  if (kt.count > 0) fetch(0);
+  if (it0 < kt.count) fetch(it0, 0);
 
   frag qf[G::KK], df[BWD ? G::KK : 1];
   load_owner<T, DP>((const T*)p.q + b * p.qb + (long)i * p.qt + h * p.qh, live, p.D, at.lhi, qf);
@@ -360,7 +369,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
     }
     delta = half_sum(delta);
     if (live) lse = p.lse[srow];
-    if (i < p.T && at.lhi == 0) p.delta[srow] = delta;
+    if (i < p.T && at.lhi == 0 && (!SHARE || wave == 0)) p.delta[srow] = delta;
   }
   // the lane's visible keys: lo .. lo + span, and those below sk (a row behind the sequence: none)
   int lo = i - p.left, hi = p.causal ? i : i + p.right, sk = p.sinks;
@@ -382,10 +391,10 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
   float m = -INFINITY, sum = 0.f;   // running maximum in use (units of the exp2 argument), this lane's half of the sum
   const int qa = qw, qb = qw + 31 < n - 1 ? qw + 31 : n - 1;
 
-  if (kt.count > 0) staged();
-  for (int it = 0; it < kt.count; ++it) {
-    if (it + 1 < kt.count) fetch(it + 1);
-    const char* kb = smem + (it & 1) * 2 * G::TILE;
+  if (it0 < kt.count) staged<SHARE>();
+  for (int it = it0, side = 0; it < kt.count; it += STEP, side ^= 1) {
+    if (it + STEP < kt.count) fetch(it + STEP, side ^ 1);
+    const char* kb = smem + side * 2 * G::TILE;
     const char* vb = kb + G::TILE;
 #pragma unroll
     for (int y = 0; y < G::NY; ++y) {
@@ -462,9 +471,42 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
         }
       }
     }
-    staged();
+    staged<SHARE>();
   }
 
+  if constexpr (!BWD) sum = half_sum(sum);
+  if constexpr (SHARE) {   // join: the wavefronts leave their maximum, sum and accumulators in LDS, the first one adds them up
+    constexpr int N = G::DB * 16 + 2;
+    float* red = (float*)smem_all;
+    __syncthreads();
+    if (wave > 0) {
+      float* mine = red + (wave - 1) * N * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[(d * 16 + r) * 64] = acc[d][r];
+      mine[(N - 2) * 64] = m;
+      mine[(N - 1) * 64] = sum;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 0; w < WV - 1; ++w) {
+      const float* other = red + w * N * 64 + lane;
+      float f = 1.f, g = 1.f;
+      if constexpr (!BWD) {
+        const float mo = other[(N - 2) * 64], up = fmaxf(m, mo);
+        f = up > -INFINITY ? __builtin_amdgcn_exp2f(m - up) : 1.f;
+        g = up > -INFINITY ? __builtin_amdgcn_exp2f(mo - up) : 1.f;
+        m = up;
+        sum = sum * f + other[(N - 1) * 64] * g;
+      }
+#pragma unroll
+      for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[d][r] = BWD ? acc[d][r] + other[(d * 16 + r) * 64] : acc[d][r] * f + other[(d * 16 + r) * 64] * g;
+    }
+  }
   if (!live) {   // (also where a visible key's values were infinite: 0 times that is not 0)
 #pragma unroll
     for (int d = 0; d < G::DB; ++d)
@@ -472,7 +514,6 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
       for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   }
   if constexpr (!BWD) {
-    sum = half_sum(sum);
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
     store_owner<T, DP>((T*)p.out + orow, acc, inv, i < p.T, p.D, at.lhi);
     if constexpr (sizeof(T) == 2) {
@@ -499,14 +540,14 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
 // whose window they are outside of -- a few keys against all queries, shared by p.chunks workgroups.  Partial sums are added up in
 // order (no atomics).
 enum { WHOLE = 0, SPLIT = 1, SINKS = 2 };
-template <typename T, int DP, int WV, int MODE>
-__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void wattn_key_kernel(WAttnArgs p) {
+template <typename T, int DP, int WV, bool SHARE, int MODE>
+__global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) void wattn_key_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
   constexpr bool SINK = MODE == SINKS;
-  constexpr int BUF = 2 * G::TILE + 2 * G::BN * (int)sizeof(float);
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile, dO tile, lse, delta]
+  constexpr int OWN = SHARE ? 32 : WV * 32, STEP = SHARE ? WV : 1, BUF = 2 * G::TILE + 2 * G::BN * (int)sizeof(float);
+  extern __shared__ __attribute__((aligned(16))) char smem_all[];   // [2 buffers][Q tile, dO tile, lse, delta], SHARE: for each wavefront
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<T, DP> at(lane);
   const int item = xcd_item(blockIdx.x, gridDim.x);
@@ -514,7 +555,8 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void
   const int bh = item / per, hk = bh % p.Hk, b = bh / p.Hk;
   const int share = item % per % shares, tile = item % per / shares;
   const int n = seq_len(p, b), group = p.H / p.Hk;
-  const int j0 = tile * (WV * 32), jw = j0 + wave * 32, j = jw + at.l31;
+  char* smem = smem_all + (SHARE ? wave * 2 * BUF : 0);
+  const int j0 = tile * OWN, jw = j0 + (SHARE ? 0 : wave * 32), j = jw + at.l31;
   const bool live = j < n;
   // tiles of queries: i0 .. i1 of each head of the group, one after the other, of which this workgroup takes its share
   int i0, i1;
@@ -523,34 +565,35 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void
     i1 = n - 1;
   } else {
     i0 = p.causal ? j0 : j0 - p.right;
-    i1 = j0 + WV * 32 - 1 + p.left;
+    i1 = j0 + OWN - 1 + p.left;
     i0 = i0 < 0 ? 0 : i0;
     i1 = i1 > n - 1 ? n - 1 : i1;
   }
   const int t0 = i0 / G::BN, nt = j0 < n && i1 >= i0 ? i1 / G::BN - t0 + 1 : 0;
-  const int all_tiles = nt * group, from = (int)((long)all_tiles * share / shares), to = (int)((long)all_tiles * (share + 1) / shares);
-  const Stager<T, DP, WV> qs(p.qt, wave, lane), ds((long)p.H * p.D, wave, lane);
+  const int all_tiles = nt * group, to = (int)((long)all_tiles * (share + 1) / shares);
+  const int from = (int)((long)all_tiles * share / shares) + (SHARE ? wave : 0), swave = SHARE ? 0 : wave;
+  const Stager<T, DP, SHARE ? 1 : WV> qs(p.qt, swave, lane), ds((long)p.H * p.D, swave, lane);
   float hold[2];
-  auto fetch = [&](int it) {
+  auto fetch = [&](int it, int side) {
     const int h = hk * group + it / nt, first = (t0 + it % nt) * G::BN;
-    char* buf = smem + (it & 1) * BUF;
-    qs.fetch(buf, (const T*)p.q + b * p.qb + h * p.qh, p.qt, first, n, p.D, wave, lane);
-    ds.fetch(buf + G::TILE, (const T*)p.dO + ((long)b * p.T * p.H + h) * p.D, (long)p.H * p.D, first, n, p.D, wave, lane);
+    char* buf = smem + side * BUF;
+    qs.fetch(buf, (const T*)p.q + b * p.qb + h * p.qh, p.qt, first, n, p.D, swave, lane);
+    ds.fetch(buf + G::TILE, (const T*)p.dO + ((long)b * p.T * p.H + h) * p.D, (long)p.H * p.D, first, n, p.D, swave, lane);
     const int i = first + lane;
-    if (wave == 0 && lane < G::BN) {
+    if (swave == 0 && lane < G::BN) {
       const long s = ((long)b * p.H + h) * p.T + i;
       hold[0] = i < n ? p.lse[s] : INFINITY;
       hold[1] = i < n ? p.delta[s] : 0.f;
     }
   };
-  auto put = [&](int it) {   // (the row statistics go through registers: written once the tile's reads are on their way)
-    if (wave == 0 && lane < G::BN) {
-      float* st = (float*)(smem + (it & 1) * BUF + 2 * G::TILE);
+  auto put = [&](int side) {   // (the row statistics go through registers: written once the tile's reads are on their way)
+    if (swave == 0 && lane < G::BN) {
+      float* st = (float*)(smem + side * BUF + 2 * G::TILE);
       st[lane] = hold[0];
       st[G::BN + lane] = hold[1];
     }
   };
-  if (from < to) fetch(from);
+  if (from < to) fetch(from, 0);
 
   frag kf[G::KK], vf[G::KK];
   load_owner<T, DP>((const T*)p.k + b * p.kb + (long)j * p.kt + hk * p.kh, live, p.D, at.lhi, kf);
@@ -576,12 +619,12 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
 
   if (from < to) {
-    put(from);
-    staged();
+    put(0);
+    staged<SHARE>();
   }
-  for (int it = from; it < to; ++it) {
-    if (it + 1 < to) fetch(it + 1);
-    const char* qb = smem + (it & 1) * BUF;
+  for (int it = from, side = 0; it < to; it += STEP, side ^= 1) {
+    if (it + STEP < to) fetch(it + STEP, side ^ 1);
+    const char* qb = smem + side * BUF;
     const char* db = qb + G::TILE;
     const float* st = (const float*)(db + G::TILE);
     const int first = (t0 + it % nt) * G::BN;
@@ -639,8 +682,35 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, WV)) void
         for (int d = 0; d < G::DB; ++d) dk[d] = O::mma(at.transposed(qb, 32 * y + 16 * a, d), w, dk[d]);
       }
     }
-    if (it + 1 < to) put(it + 1);
-    staged();
+    if (it + STEP < to) put(side ^ 1);
+    staged<SHARE>();
+  }
+  if constexpr (SHARE) {   // join, as in the other kernel
+    constexpr int N = G::DB * 32;
+    float* red = (float*)smem_all;
+    __syncthreads();
+    if (wave > 0) {
+      float* mine = red + (wave - 1) * N * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          mine[(d * 32 + r) * 64] = dk[d][r];
+          mine[(d * 32 + 16 + r) * 64] = dv[d][r];
+        }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 0; w < WV - 1; ++w) {
+      const float* other = red + w * N * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          dk[d][r] += other[(d * 32 + r) * 64];
+          dv[d][r] += other[(d * 32 + 16 + r) * 64];
+        }
+    }
   }
 
   if constexpr (SINK) {
@@ -735,17 +805,21 @@ int launch(const WAttnArgs& p, long groups, int threads, size_t lds, hipStream_t
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
-template <typename T, int DP, int WV, bool BWD>
+template <typename T, int DP, bool SHARE, bool BWD>
 int run_query(WAttnArgs p, hipStream_t st) {
-  p.tiles = cdiv(p.T, WV * 32);
-  return launch<wattn_query_kernel<T, DP, WV, BWD>>(p, (long)p.tiles * p.H * p.B, WV * 64, 4 * (size_t)Geo<T, DP>::TILE, st);
+  constexpr int WV = SHARE ? share_waves<T, DP>() : 4;
+  p.tiles = cdiv(p.T, SHARE ? 32 : WV * 32);
+  return launch<wattn_query_kernel<T, DP, WV, SHARE, BWD>>(p, (long)p.tiles * p.H * p.B, WV * 64,
+                                                           (SHARE ? WV : 1) * 4 * (size_t)Geo<T, DP>::TILE, st);
 }
-template <typename T, int DP, int WV, int MODE>
+template <typename T, int DP, bool SHARE, int MODE>
 int run_key(WAttnArgs p, hipStream_t st) {
   using G = Geo<T, DP>;
-  p.tiles = MODE == SINKS ? cdiv(p.sinks, 32) : cdiv(p.T, WV * 32);
-  return launch<wattn_key_kernel<T, DP, WV, MODE>>(p, (long)p.tiles * (MODE == SINKS ? p.chunks : MODE == SPLIT ? p.splits : 1) * p.Hk * p.B, WV * 64,
-                                                   2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
+  constexpr int WV = SHARE ? share_waves<T, DP>() : 4;
+  p.tiles = cdiv(MODE == SINKS ? p.sinks : p.T, SHARE ? 32 : WV * 32);
+  return launch<wattn_key_kernel<T, DP, WV, SHARE, MODE>>(
+      p, (long)p.tiles * (MODE == SINKS ? p.chunks : MODE == SPLIT ? p.splits : 1) * p.Hk * p.B, WV * 64,
+      (SHARE ? WV : 1) * 2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
 }
 inline int run_join(const WAttnArgs& p, hipStream_t st) {
   const int n = p.sinks * 2 * p.D;
@@ -759,19 +833,22 @@ int run_sum(const WAttnArgs& p, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
+// Up to this many workgroups of four owner blocks, four times as many that share one each do better: half of the compute units would
+// idle, and a shared block takes a quarter of the time.
+constexpr long SHARE_BELOW = 128;
 // How the work is laid out, from the sizes alone (the scratch is sized by the same rules).
 struct Plan {
   int chunks, splits;   // workgroups that share a sink block's queries (0: the sinks reach nothing), and a key block's
-  bool one;             // one wavefront a workgroup
+  bool share;           // a key block's wavefronts share 32 keys
 };
 inline Plan plan_keys(int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
   Plan r = {0, 1, false};
   // do the sinks reach queries outside of the window?
   if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
-    const long rows = (long)B * Hk * cdiv(sinks, 32), units = (long)(H / Hk) * cdiv(T, 64);   // of at least one tile each
-    long c = 1024 / rows;
-    c = c < 1 ? 1 : c;
-    r.chunks = (int)(c < units ? c : units);
+    const long rows = (long)B * Hk * cdiv(sinks, 32), tiles = (long)(H / Hk) * cdiv(T, 64);
+    long c = 256 / rows;                    // one workgroup a compute unit, each of its wavefronts a tile at least
+    if (c > (tiles + 3) / 4) c = (tiles + 3) / 4;
+    r.chunks = (int)(c < 1 ? 1 : c);
   }
   // few key blocks: share each one's queries among workgroups, as long as that leaves each about four tiles (of all heads of the group)
   const long blocks = (long)cdiv(T, 128) * Hk * B;
@@ -781,11 +858,11 @@ inline Plan plan_keys(int B, int T, int H, int Hk, int left, int right, int sink
     long s = (512 + blocks - 1) / blocks;
     if (s > tiles / 4) s = tiles / 4;
     r.splits = s < 1 ? 1 : (int)s;
-    r.one = blocks * r.splits < 256;
+    r.share = blocks * r.splits <= SHARE_BELOW;
   }
   return r;
 }
-inline bool one_wave_queries(int B, int T, int H) { return (long)cdiv(T, 128) * H * B < 256; }
+inline bool share_queries(int B, int T, int H) { return (long)cdiv(T, 128) * H * B <= SHARE_BELOW; }
 
 #define WA_DISPATCH(CALL)                 \
   if (p.D <= 32) return CALL(32);         \
@@ -825,18 +902,18 @@ int fwd(WAttnArgs p, const long* strides, void* o, void* olo, float* lse, hipStr
   if (r <= 0) return r;
   if (o == nullptr || (((uintptr_t)o | (uintptr_t)olo) & 15)) return INDM_E_ARG;
   p.out = o; p.olo = olo; p.lse = lse;
-#define WA_FWD(DP) (one_wave_queries(p.B, p.T, p.H) ? run_query<T, DP, 1, false>(p, st) : run_query<T, DP, 4, false>(p, st))
+#define WA_FWD(DP) (share_queries(p.B, p.T, p.H) ? run_query<T, DP, true, false>(p, st) : run_query<T, DP, false, false>(p, st))
   WA_DISPATCH(WA_FWD)
 }
 
 template <typename T, int DP>
-int bwd_dp(const WAttnArgs& p, bool one, hipStream_t st) {
-  int r = one_wave_queries(p.B, p.T, p.H) ? run_query<T, DP, 1, true>(p, st) : run_query<T, DP, 4, true>(p, st);   // dq, and delta for the others
-  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, 1, SINKS>(p, st);
+int bwd_dp(const WAttnArgs& p, bool share, hipStream_t st) {
+  int r = share_queries(p.B, p.T, p.H) ? run_query<T, DP, true, true>(p, st) : run_query<T, DP, false, true>(p, st);   // dq; delta for the others
+  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, true, SINKS>(p, st);
   if (r == INDM_OK && p.chunks > 1) r = run_join(p, st);
   if (r == INDM_OK)
-    r = p.splits > 1 ? (one ? run_key<T, DP, 1, SPLIT>(p, st) : run_key<T, DP, 4, SPLIT>(p, st))
-                     : (one ? run_key<T, DP, 1, WHOLE>(p, st) : run_key<T, DP, 4, WHOLE>(p, st));
+    r = p.splits > 1 ? (share ? run_key<T, DP, true, SPLIT>(p, st) : run_key<T, DP, false, SPLIT>(p, st))
+                     : (share ? run_key<T, DP, true, WHOLE>(p, st) : run_key<T, DP, false, WHOLE>(p, st));
   if (r == INDM_OK && p.splits > 1) r = run_sum<T>(p, st);
   return r;
 }
@@ -854,7 +931,7 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
   p.splits = plan.splits;
   p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
   p.split = p.part + (long)p.B * p.Hk * p.chunks * p.sinks * 2 * p.D;
-#define WA_BWD(DP) bwd_dp<T, DP>(p, plan.one, st)
+#define WA_BWD(DP) bwd_dp<T, DP>(p, plan.share, st)
   WA_DISPATCH(WA_BWD)
 }
 
