@@ -1,0 +1,455 @@
+// Autograd of the token operators (ops.layer_norm, dropout, rotary, window_attention) in C++: the module indm_amd._token.
+//
+// On small tensors a training call of these is host time: a backward pass runs on autograd's own thread, where a Python function
+// takes the interpreter's lock and starts with cold caches (layer norm forward and backward of 256 x 256: 108 us through Python
+// functions, of which the kernels are 12).  Here a call is one crossing into C++: checks, allocations, the launch, and a backward node
+// that never enters the interpreter.  The kernels stay behind the C ABI: bind() takes the addresses of the entry points from the one
+// loaded library (indm_amd/hip.py), nothing is linked.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <c10/util/accumulate.h>
+#include <c10/util/strides.h>
+#include <map>
+#include <mutex>
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+// ---------------------------------------------------------------------------------------------- the C ABI (include/indm_hip.h)
+struct Abi {
+  int (*layernorm_fwd[2])(const void*, long, const float*, const float*, void*, float*, float*, long, int, float, void*);
+  long (*layernorm_bwd_ws_floats)(long, int, int);
+  int (*layernorm_bwd[2])(const void*, const void*, long, const float*, const float*, const float*, void*, float*, float*, float*, long, int, void*);
+  int (*dropout[2])(const void*, const void*, void*, long, float, unsigned long long, const void*, void*);
+  int (*rotary[2])(const void*, const void*, void*, void*, const long*, int, long, int, int, int, const void*, int, long, const double*, const int*, int, int, int, void*);
+  int (*wattn_fwd[2])(const void*, const void*, const void*, const long*, void*, void*, float*, const int*, int, int, int, int, int, int, int, int, int, float, void*);
+  long (*wattn_bwd_ws_floats)(int, int, int, int, int, int, int, int, int);
+  int (*wattn_bwd[2])(const void*, const void*, const void*, const long*, const void*, const void*, const void*, const float*, const int*, void*, void*, void*, float*,
+                      int, int, int, int, int, int, int, int, int, float, void*);
+} abi;
+
+void bind(const std::map<std::string, uint64_t>& at) {
+  auto set = [&](auto& fn, const std::string& name) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(at.at("indm_" + name)); };
+  for (int i = 0; i < 2; ++i) {
+    const std::string t = i == 0 ? "_f32" : "_bf16";
+    set(abi.layernorm_fwd[i], "layernorm_fwd" + t);
+    set(abi.layernorm_bwd[i], "layernorm_bwd" + t);
+    set(abi.dropout[i], "dropout" + t);
+    set(abi.rotary[i], "rotary" + t);
+    set(abi.wattn_fwd[i], "wattn_fwd" + t);
+    set(abi.wattn_bwd[i], "wattn_bwd" + t);
+  }
+  set(abi.layernorm_bwd_ws_floats, "layernorm_bwd_ws_floats");
+  set(abi.wattn_bwd_ws_floats, "wattn_bwd_ws_floats");
+}
+
+// ---------------------------------------------------------------------------------------------- what all of them do
+#define REFUSE(...) TORCH_CHECK(false, "indm_amd: ", __VA_ARGS__)
+
+void ok(int status, const char* name) {
+  const char* what = status == -1 ? "INDM_E_SHAPE" : status == -2 ? "INDM_E_DTYPE" : status == -3 ? "INDM_E_LAUNCH" : "INDM_E_ARG";
+  TORCH_CHECK(status == 0, name, " failed: ", what);
+}
+bool given(const Maybe& t) { return t.has_value() && t->defined(); }
+Tensor plain(const Maybe& t) { return given(t) ? *t : Tensor(); }
+bool tracked(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// which entry point: 0 float32, 1 bfloat16
+int type_of(const char* op, const Tensor& x) {
+  if (x.scalar_type() == at::kFloat) return 0;
+  if (x.scalar_type() != at::kBFloat16) REFUSE(op, ": expected float32 or bfloat16, got ", x.scalar_type());
+  return 1;
+}
+void on_one_gpu(const char* op, std::initializer_list<const Tensor*> ts) {
+  const Tensor& x = **ts.begin();
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(t->is_cuda(), "indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback");
+    if (t->device() != x.device()) REFUSE(op, ": tensors on ", x.device(), " and ", t->device());
+  }
+}
+void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
+// Every tensor that a kernel writes comes from here.  guard(bytes) pads them with bands of that many bytes of a pattern on both sides
+// (a debugging mode, like POISON_WS: a store outside of a tensor that hits a free block would go unseen), broken_guards() counts the
+// bands that were written to and forgets the tensors.
+struct Guards {
+  int64_t bytes = 0;
+  std::vector<Tensor> raw;
+  std::mutex lock;
+} guards;
+constexpr uint8_t GUARD = 0xA5;
+Tensor fresh(at::IntArrayRef sizes, const at::TensorOptions& opt) {
+  if (guards.bytes == 0) return at::empty(sizes, opt);
+  const int64_t n = c10::multiply_integers(sizes), e = (int64_t)opt.dtype().itemsize();
+  Tensor raw = at::empty({n * e + 2 * guards.bytes}, opt.dtype(at::kByte));
+  raw.fill_(GUARD);
+  Tensor t = at::empty({0}, opt).set_(raw.storage(), guards.bytes / e, sizes, c10::contiguous_strides(sizes));
+  const std::lock_guard<std::mutex> hold(guards.lock);
+  guards.raw.push_back(raw);
+  return t;
+}
+void guard(int64_t bytes) { guards.bytes = bytes / 256 * 256; }
+int64_t broken_guards() {
+  std::vector<Tensor> raw;
+  {
+    const std::lock_guard<std::mutex> hold(guards.lock);
+    raw.swap(guards.raw);
+  }
+  int64_t broken = 0;
+  for (const Tensor& r : raw) {
+    const int64_t g = guards.bytes;
+    broken += r.narrow(0, 0, g).ne(GUARD).any().item<bool>() + r.narrow(0, r.size(0) - g, g).ne(GUARD).any().item<bool>();
+  }
+  return broken;
+}
+Tensor dense_like(const Tensor& x) { return fresh(x.sizes(), x.options()); }
+Tensor floats(int64_t n, const Tensor& x) { return fresh({n}, x.options().dtype(at::kFloat)); }
+template <typename P = float>
+P* ptr(const Tensor& t) {
+  return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr;
+}
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+// A backward pass that is itself recorded (create_graph): its results refuse to be differentiated again
+variable_list once(variable_list grads) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  variable_list leaves;
+  for (const Tensor& g : grads)
+    if (g.defined()) leaves.push_back(g.detach().set_requires_grad(true));
+  auto refuse = std::make_shared<torch::autograd::DelayedError>("indm_amd: the token operators are differentiable once", static_cast<int64_t>(leaves.size()));
+  variable_list out = (*refuse)(std::move(leaves));
+  size_t k = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = out[k++];
+  return grads;
+}
+
+// ---------------------------------------------------------------------------------------------- layer norm
+constexpr int64_t LN_MAX_C = 16384;
+
+// x [..., C] as R rows with one stride and dense columns; a copy only where its strides allow no such view
+struct Rows {
+  Tensor x;
+  long n, ld;
+};
+Rows rows_of(const Tensor& x) {
+  const int64_t C = x.size(-1), R = x.numel() / C;
+  if (x.is_contiguous()) return {x, R, C};
+  if (R > 0 && (x.stride(-1) == 1 || C == 1)) {
+    int64_t ld = -1, run = 1;   // the rows' stride, and how many of them the dimensions seen so far make
+    bool one = true;
+    for (int64_t d = x.dim() - 2; d >= 0; --d) {
+      if (x.size(d) == 1) continue;
+      if (ld < 0) ld = x.stride(d);
+      one = one && x.stride(d) == ld * run;
+      run *= x.size(d);
+    }
+    if (one) return {x, R, ld < 0 ? C : ld};
+  }
+  return {x.contiguous(), R, C};
+}
+
+void layer_norm_check(const Tensor& x, const Tensor& gamma, const Tensor& beta, double eps) {
+  type_of("layer_norm", x);
+  if (x.dim() < 1 || x.size(-1) < 1) REFUSE("layer_norm: x needs a last dimension that is not empty, got ", x.sizes());
+  const int64_t C = x.size(-1);
+  if (C > LN_MAX_C) REFUSE("layer_norm: rows of up to ", LN_MAX_C, " elements, got ", C);
+  for (const Tensor* p : {&gamma, &beta}) {
+    if (!p->defined()) continue;
+    const char* name = p == &gamma ? "gamma" : "beta";
+    if (p->scalar_type() != at::kFloat) REFUSE("layer_norm: ", name, " is float32, got ", p->scalar_type());
+    if (p->dim() != 1 || p->size(0) != C) REFUSE("layer_norm: ", name, " is [", C, "], got ", p->sizes());
+  }
+  if (!(eps >= 0.)) REFUSE("layer_norm: eps >= 0, got ", eps);
+  on_one_gpu("layer_norm", {&x, &gamma, &beta});
+}
+// -> y, and with stats [2 R]: the rows' means, then their 1 / standard deviations
+std::pair<Tensor, Tensor> layer_norm_run(const Tensor& x, const Tensor& gamma_, const Tensor& beta_, double eps, bool stats) {
+  const c10::DeviceGuard guard(x.device());
+  const Tensor gamma = dense(gamma_), beta = dense(beta_);
+  const Rows r = rows_of(x);
+  Tensor y = dense_like(x), st = stats ? floats(2 * r.n, x) : Tensor();
+  ok(abi.layernorm_fwd[type_of("layer_norm", x)](r.x.data_ptr(), r.ld, ptr(gamma), ptr(beta), y.data_ptr(), ptr(st), stats ? ptr(st) + r.n : nullptr, r.n,
+                                                 (int)x.size(-1), (float)eps, stream_of(x)),
+     "indm_layernorm_fwd");
+  return {y, st};
+}
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& gamma_, const Maybe& beta_, double eps) {
+    const Tensor gamma = plain(gamma_), beta = plain(beta_);
+    auto [y, stats] = layer_norm_run(x, gamma, beta, eps, true);
+    ctx->save_for_backward({x, gamma, stats});
+    ctx->saved_data["want"] = (int64_t)((x.requires_grad() ? 1 : 0) | (gamma.defined() && gamma.requires_grad() ? 2 : 0) | (beta.defined() && beta.requires_grad() ? 4 : 0));
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &stats = saved[2];
+    const int64_t want = ctx->saved_data["want"].toInt(), C = x.size(-1);
+    const c10::DeviceGuard guard(x.device());
+    const Tensor gamma = dense(saved[1]), dy = grads[0].contiguous();
+    const Rows r = rows_of(x);
+    Tensor dx = dense_like(x), dgamma = want & 2 ? floats(C, x) : Tensor(), dbeta = want & 4 ? floats(C, x) : Tensor(), ws;
+    // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
+    if (want & 6) ws = floats(std::max(1L, abi.layernorm_bwd_ws_floats(r.n, (int)C, (int)x.element_size())), x);
+    ok(abi.layernorm_bwd[type_of("layer_norm", x)](dy.data_ptr(), r.x.data_ptr(), r.ld, ptr(gamma), ptr(stats), ptr(stats) + r.n, dx.data_ptr(), ptr(dgamma),
+                                                   ptr(dbeta), ptr(ws), r.n, (int)C, stream_of(x)),
+       "indm_layernorm_bwd");
+    return once({dx, dgamma, dbeta, Tensor()});
+  }
+};
+Tensor layer_norm(const Tensor& x, const Maybe& gamma_, const Maybe& beta_, double eps) {
+  const Tensor gamma = plain(gamma_), beta = plain(beta_);
+  layer_norm_check(x, gamma, beta, eps);
+  return tracked({&x, &gamma, &beta}) ? LayerNorm::apply(x, gamma_, beta_, eps) : layer_norm_run(x, gamma, beta, eps, false).first;
+}
+
+// ---------------------------------------------------------------------------------------------- dropout
+Tensor dropout_run(const Tensor& x_, double p, uint64_t seed, const Tensor& res_, const Tensor& seed_dev) {
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = dense(x_), res = dense(res_);
+  Tensor y = dense_like(x);
+  ok(abi.dropout[type_of("dropout", x)](x.data_ptr(), ptr<void>(res), y.data_ptr(), x.numel(), (float)p, seed, ptr<void>(seed_dev), stream_of(x)),
+     "indm_dropout");
+  return y;
+}
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& res_, double p, int64_t seed, const Maybe& seed_dev_) {
+    const Tensor res = plain(res_), seed_dev = plain(seed_dev_);
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["want"] = (int64_t)((x.requires_grad() ? 1 : 0) | (res.defined() && res.requires_grad() ? 2 : 0));
+    if (seed_dev.defined()) ctx->saved_data["seed_dev"] = seed_dev;   // (not a saved variable: a graph's owner advances it in place)
+    return dropout_run(x, p, (uint64_t)seed, res, seed_dev);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const int64_t want = ctx->saved_data["want"].toInt();
+    const auto at = ctx->saved_data.find("seed_dev");
+    Tensor dx;
+    if (want & 1)
+      dx = dropout_run(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), Tensor(),
+                       at == ctx->saved_data.end() ? Tensor() : at->second.toTensor());
+    variable_list out = once({dx});
+    return {out[0], want & 2 ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& res_, const Maybe& seed_dev_) {
+  const Tensor res = plain(res_), seed_dev = plain(seed_dev_);
+  type_of("dropout", x);
+  if (!(p >= 0. && p <= 1.)) REFUSE("dropout: 0 <= p <= 1, got ", p);
+  if (res.defined() && (res.sizes() != x.sizes() || res.scalar_type() != x.scalar_type()))
+    REFUSE("dropout: res is ", x.sizes(), " ", x.scalar_type(), ", got ", res.sizes(), " ", res.scalar_type());
+  if (seed_dev.defined() && (seed_dev.scalar_type() != at::kLong || seed_dev.numel() != 1)) REFUSE("dropout: seed_dev is one int64 on the device");
+  on_one_gpu("dropout", {&x, &res, &seed_dev});
+  return tracked({&x, &res}) ? Dropout::apply(x, res_, p, (int64_t)seed, seed_dev_) : dropout_run(x, p, seed, res, seed_dev);
+}
+
+// ---------------------------------------------------------------------------------------------- rotary positions
+void rotary_check(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& freqs, const std::vector<int64_t>& sections) {
+  type_of("rotary", q);
+  if (q.dim() != 4) REFUSE("rotary: q is [B, T, H, D], got ", q.sizes());
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3), A = (int64_t)sections.size();
+  if (D > 4096) REFUSE("rotary: heads of up to 4096 entries, got ", D);
+  if (k.defined() && (k.scalar_type() != q.scalar_type() || k.dim() != 4 || k.size(0) != B || k.size(1) != T || k.size(3) != D))
+    REFUSE("rotary: k is [", B, ", ", T, ", Hk, ", D, "] ", q.scalar_type(), ", got ", k.sizes(), " ", k.scalar_type());
+  int64_t sum = 0;
+  bool even = A >= 1 && A <= 8;
+  for (int64_t n : sections) {
+    even = even && n >= 2 && n % 2 == 0 && n <= D - sum;
+    sum += even ? n : 0;
+  }
+  if (!even) REFUSE("rotary: sections are 1 to 8 even positive numbers that sum to ", D, " at most, got ", sections);
+  const auto type = pos.scalar_type();
+  if (type != at::kInt && type != at::kLong && type != at::kFloat) REFUSE("rotary: positions are int32, int64 or float32, got ", type);
+  const int64_t lead = pos.dim() - 2;
+  if (lead < 0 || lead > 1 || pos.size(lead) != T || pos.size(lead + 1) != A || (lead == 1 && pos.size(0) != B))
+    REFUSE("rotary: pos is [", T, ", ", A, "] or [", B, ", ", T, ", ", A, "], got ", pos.sizes());
+  if (freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || freqs.size(0) != sum / 2)
+    REFUSE("rotary: freqs is float64 [", sum / 2, "], got ", freqs.sizes(), " ", freqs.scalar_type());
+  on_one_gpu("rotary", {&q, &k, &pos, &freqs});
+}
+Tensor unit_columns(const Tensor& x) { return !x.defined() || x.stride(3) == 1 || x.size(3) == 1 ? x : x.contiguous(); }
+// q or k may be undefined, not both -> the rotated ones (dense)
+std::pair<Tensor, Tensor> rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& pos_, const Tensor& freqs_, at::IntArrayRef sections, bool interleaved,
+                                     bool inverse) {
+  const Tensor& any = q_.defined() ? q_ : k_;
+  const c10::DeviceGuard guard(any.device());
+  const Tensor q = unit_columns(q_), k = unit_columns(k_), pos = pos_.contiguous(), freqs = freqs_.contiguous();
+  Tensor yq = q.defined() ? dense_like(q) : Tensor(), yk = k.defined() ? dense_like(k) : Tensor();
+  long strides[6] = {};
+  for (int i = 0; i < 3; ++i) {
+    if (q.defined()) strides[i] = q.stride(i);
+    if (k.defined()) strides[3 + i] = k.stride(i);
+  }
+  int s[8];
+  for (size_t i = 0; i < sections.size(); ++i) s[i] = (int)sections[i];
+  const int64_t B = any.size(0), T = any.size(1), A = (int64_t)sections.size();
+  const auto type = pos.scalar_type();
+  TORCH_CHECK(B <= INT32_MAX && any.size(2) <= INT32_MAX, "indm_amd: rotary: too many samples or heads");
+  ok(abi.rotary[type_of("rotary", any)](ptr<void>(q), ptr<void>(k), ptr<void>(yq), ptr<void>(yk), strides, (int)B, T, q.defined() ? (int)q.size(2) : 0,
+                                        k.defined() ? (int)k.size(2) : 0, (int)any.size(3), pos.data_ptr(), type == at::kInt ? 0 : type == at::kFloat ? 1 : 2,
+                                        pos.dim() == 3 ? T * A : 0, ptr<double>(freqs), s, (int)A, interleaved, inverse, stream_of(any)),
+     "indm_rotary");
+  return {yq, yk};
+}
+struct Rotary : torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k_, const Tensor& pos, const Tensor& freqs, at::IntArrayRef sections,
+                               bool interleaved) {
+    const Tensor k = plain(k_);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({pos, freqs});
+    ctx->saved_data["sections"] = sections.vec();
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["want"] = (int64_t)((q.requires_grad() ? 1 : 0) | (k.defined() && k.requires_grad() ? 2 : 0));
+    auto [yq, yk] = rotary_run(q, k, pos, freqs, sections, interleaved, false);
+    return k.defined() ? variable_list{yq, yk} : variable_list{yq};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t want = ctx->saved_data["want"].toInt();
+    const Tensor dq = want & 1 ? grads[0] : Tensor(), dk = want & 2 && grads.size() > 1 ? grads[1] : Tensor();
+    std::pair<Tensor, Tensor> g;
+    if (dq.defined() || dk.defined())
+      g = rotary_run(dq, dk, saved[0], saved[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
+    return once({g.first, g.second, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k_, const Tensor& pos, const Tensor& freqs, const std::vector<int64_t>& sections,
+                                bool interleaved) {
+  const Tensor k = plain(k_);
+  rotary_check(q, k, pos, freqs, sections);
+  Tensor yq, yk;
+  if (tracked({&q, &k})) {
+    const variable_list y = Rotary::apply(q, k_, pos, freqs, at::IntArrayRef(sections), interleaved);
+    yq = y[0];
+    if (y.size() > 1) yk = y[1];
+  } else {
+    std::tie(yq, yk) = rotary_run(q, k, pos, freqs, sections, interleaved, false);
+  }
+  return {yq, yk.defined() ? Maybe(yk) : std::nullopt};
+}
+
+// ---------------------------------------------------------------------------------------------- window attention
+struct Window {
+  int64_t left, right, sinks;
+  bool causal;
+  double scale;
+};
+void window_check(const Tensor& q, const Tensor& k, const Tensor& v, const Window& w, const Tensor& lengths) {
+  type_of("window_attention", q);
+  if (q.dim() != 4) REFUSE("window_attention: q is [B, T, H, D], got ", q.sizes());
+  const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
+  for (const Tensor* x : {&k, &v})
+    if (x->scalar_type() != q.scalar_type() || x->dim() != 4 || x->size(0) != B || x->size(1) != T || x->size(3) != D || x->sizes() != k.sizes())
+      REFUSE("window_attention: ", x == &k ? "k" : "v", " is [", B, ", ", T, ", Hk, ", D, "] ", q.scalar_type(), ", got ", x->sizes(), " ", x->scalar_type());
+  const int64_t Hk = k.size(2);
+  if (H < 1 || Hk < 1 || H % Hk) REFUSE("window_attention: the ", H, " heads of q are a multiple of the ", Hk, " of k and v");
+  if (D % 8 || D < 8 || D > 128) REFUSE("window_attention: heads of 8, 16, ... 128 entries, got ", D);
+  if (T > (1 << 28) || B > INT32_MAX || H * D > (1 << 22)) REFUSE("window_attention: up to ", 1 << 28, " tokens of ", 1 << 22, " entries, got ", T, " of ", H * D);
+  if (w.left < 0 || w.right < 0 || w.sinks < 0) REFUSE("window_attention: window and sinks >= 0, got (", w.left, ", ", w.right, "), ", w.sinks);
+  if (!(w.scale > 0. && (float)w.scale < INFINITY && (float)w.scale > 0.f)) REFUSE("window_attention: scale > 0, got ", w.scale);
+  if (lengths.defined() && (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B))
+    REFUSE("window_attention: lengths is int32 [", B, "], got ", lengths.sizes(), " ", lengths.scalar_type());
+  on_one_gpu("window_attention", {&q, &k, &v, &lengths});
+}
+// x with dense columns, every row on 16 bytes and tokens at most 2^22 elements apart; a copy where it is not so
+Tensor aligned_rows(const Tensor& x) {
+  const int64_t e = 16 / x.element_size();
+  if (x.stride(3) == 1 && x.stride(0) % e == 0 && x.stride(1) % e == 0 && x.stride(2) % e == 0 && x.stride(1) <= (1 << 22) &&
+      (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0)
+    return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+struct Heads {
+  long strides[9];
+  Heads(const Tensor& q, const Tensor& k, const Tensor& v) {
+    const Tensor* t[3] = {&q, &k, &v};
+    for (int i = 0; i < 9; ++i) strides[i] = t[i / 3]->stride(i % 3);
+  }
+};
+struct WindowOut {
+  Tensor o, rest, lse, q, k, v;   // rest: what rounding o to bfloat16 left; q, k, v as the kernels read them
+};
+WindowOut window_run(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Window& w, const Tensor& lengths_, bool stats) {
+  const c10::DeviceGuard guard(q_.device());
+  WindowOut r;
+  r.q = aligned_rows(q_);
+  r.k = aligned_rows(k_);
+  r.v = aligned_rows(v_);
+  const Tensor lengths = dense(lengths_);
+  const int64_t B = r.q.size(0), T = r.q.size(1), H = r.q.size(2), D = r.q.size(3);
+  r.o = dense_like(r.q);
+  if (stats) {
+    r.lse = floats(B * H * T, r.q);
+    if (r.q.scalar_type() == at::kBFloat16) r.rest = dense_like(r.q);
+  }
+  ok(abi.wattn_fwd[type_of("window_attention", r.q)](r.q.data_ptr(), r.k.data_ptr(), r.v.data_ptr(), Heads(r.q, r.k, r.v).strides, r.o.data_ptr(), ptr<void>(r.rest), ptr(r.lse),
+                                                     ptr<int>(lengths), (int)B, (int)T, (int)H, (int)r.k.size(2), (int)D, (int)std::min(w.left, T), (int)std::min(w.right, T),
+                                                     (int)std::min(w.sinks, T), w.causal, (float)w.scale, stream_of(r.q)),
+     "indm_wattn_fwd");
+  return r;
+}
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, int64_t right, int64_t sinks, bool causal,
+                        const Maybe& lengths_, double scale) {
+    const Tensor lengths = plain(lengths_);
+    WindowOut r = window_run(q, k, v, {left, right, sinks, causal, scale}, lengths, true);
+    ctx->save_for_backward({r.q, r.k, r.v, r.o, r.rest, r.lse, lengths});
+    ctx->saved_data["window"] = std::vector<int64_t>{left, right, sinks, causal};
+    ctx->saved_data["scale"] = scale;
+    return r.o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5];
+    const c10::DeviceGuard guard(q.device());
+    const Tensor lengths = dense(saved[6]);
+    Tensor dout = grads[0].contiguous();
+    if (reinterpret_cast<uintptr_t>(dout.data_ptr()) & 15) dout = dout.clone();
+    const std::vector<int64_t> w = ctx->saved_data["window"].toIntVector();
+    const int64_t T = q.size(1);
+    const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), D = (int)q.size(3);
+    const int left = (int)std::min(w[0], T), right = (int)std::min(w[1], T), sinks = (int)std::min(w[2], T), causal = (int)w[3];
+    Tensor dq = dense_like(q), dk = dense_like(k), dv = dense_like(v);
+    // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
+    Tensor ws = floats(std::max(1L, abi.wattn_bwd_ws_floats(B, (int)T, H, Hk, D, left, right, sinks, causal)), q);
+    ok(abi.wattn_bwd[type_of("window_attention", q)](q.data_ptr(), k.data_ptr(), v.data_ptr(), Heads(q, k, v).strides, o.data_ptr(), ptr<void>(rest), dout.data_ptr(), ptr(lse),
+                                                     ptr<int>(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(ws), B, (int)T, H, Hk, D, left, right, sinks, causal,
+                                                     (float)ctx->saved_data["scale"].toDouble(), stream_of(q)),
+       "indm_wattn_bwd");
+    return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, int64_t right, int64_t sinks, bool causal, const Maybe& lengths_,
+                        double scale) {
+  const Tensor lengths = plain(lengths_);
+  const Window w = {left, right, sinks, causal, scale};
+  window_check(q, k, v, w, lengths);
+  return tracked({&q, &k, &v}) ? WindowAttention::apply(q, k, v, left, right, sinks, causal, lengths_, scale) : window_run(q, k, v, w, lengths, false).o;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_token, m) {
+  namespace py = pybind11;
+  m.def("bind", &bind);
+  m.def("guard", &guard);
+  m.def("broken_guards", &broken_guards);
+  m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
+  m.def("rotary", &rotary, py::call_guard<py::gil_scoped_release>());
+  m.def("window_attention", &window_attention, py::call_guard<py::gil_scoped_release>());
+}

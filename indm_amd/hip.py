@@ -2189,299 +2189,20 @@ def iresblock_inverse(y, cb, W1, W2T, W3, b1, b2, b3, preact, atol, rtol):
 
 
 # --------------------------------------------------------------------------- operators of a block over tokens (csrc/token_ops.hip, window_attn.hip)
-# A call of these costs more host time than GPU time on small tensors: the checks build their messages only when they refuse, nothing is
-# looked up by a name that has to be put together first, and a tensor's scratch is one allocation.
-_TOKEN_DTYPES = {torch.float32: "f32", torch.bfloat16: "bf16"}
-_token_fns = {}
+_token = [None]
 
 
-def _token_fn(op, dtype):
-    """the entry point indm_<op>_<type> of the library"""
-    fn = _token_fns.get((op, dtype))
-    if fn is None:
-        if dtype not in _TOKEN_DTYPES:
-            _refuse(f"{op}: expected float32 or bfloat16, got {dtype}")
-        fn = _token_fns[op, dtype] = getattr(lib(), f"indm_{op}_{_TOKEN_DTYPES[dtype]}")
-    return fn
-
-
-def _refuse(what):
-    raise RuntimeError("indm_amd: " + what)
-
-
-def _token_device(op, *tensors):
-    """None if every tensor is on the current GPU; if all are on another one, a context in which that one is current (allocations and the
-    launch belong there)"""
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            if not (t.is_cuda and tensors[0].is_cuda):
-                raise RuntimeError("indm_amd.hip: tensor is not on the GPU; the HIP path has no CPU fallback")
-            _refuse(f"{op}: tensors on {tensors[0].device} and {t.device}")
-    return None if torch.cuda.current_device() == dev else torch.cuda.device(dev)
-
-
-def _like(x):
-    """a dense tensor of x's shape, type and device"""
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
-def _rows2d(x):
-    """(x, R, row stride) of x [..., C] as R rows with one stride and contiguous columns; a copy only where x has no such view"""
-    C = x.shape[-1]
-    R = x.numel() // C
-    if x.is_contiguous():
-        return x, R, C
-    if R and (x.stride(-1) == 1 or C == 1):
+def token_ops():
+    """the compiled module behind ops.layer_norm / dropout / rotary / window_attention (csrc/token_bind.cpp: their argument checks,
+    allocations and autograd nodes in C++), bound to the entry points of the loaded library; fails loudly if it has not been built"""
+    if _token[0] is None:
+        L = lib()
         try:
-            v = x.view(R, C)
-            return v, R, v.stride(0)
-        except RuntimeError:
-            pass
-    return x.contiguous(), R, C
-
-
-_LN_MAX_C = 16384
-
-
-def _ln_check(x, gamma, beta, eps):
-    if x.dtype not in _TOKEN_DTYPES:
-        _refuse(f"layer_norm: expected float32 or bfloat16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        _refuse(f"layer_norm: x needs a last dimension that is not empty, got {tuple(x.shape)}")
-    C = x.shape[-1]
-    if C > _LN_MAX_C:
-        _refuse(f"layer_norm: rows of up to {_LN_MAX_C} elements, got {C}")
-    for p in (gamma, beta):
-        if p is not None and (p.dtype != torch.float32 or p.shape != (C,)):
-            name = "gamma" if p is gamma else "beta"
-            if p.dtype != torch.float32:
-                _refuse(f"layer_norm: {name} is float32, got {p.dtype}")
-            _refuse(f"layer_norm: {name} is [{C}], got {tuple(p.shape)}")
-    if not eps >= 0.0:
-        _refuse(f"layer_norm: eps >= 0, got {eps}")
-
-
-def layernorm_fwd(x, gamma=None, beta=None, eps=1e-6, stats=True):
-    """x [..., C] -> y, the rows' statistics for the backward (fp32 [2 R]: means, then rstds; None without stats)"""
-    _ln_check(x, gamma, beta, eps)
-    away = _token_device("layer_norm", x, gamma, beta)
-    if away is not None:
-        with away:
-            return layernorm_fwd(x, gamma, beta, eps, stats)
-    if gamma is not None and not gamma.is_contiguous():
-        gamma = gamma.contiguous()
-    if beta is not None and not beta.is_contiguous():
-        beta = beta.contiguous()
-    xr, R, ldx = _rows2d(x)
-    y = _like(x)
-    mean = torch.empty((2 * R,), dtype=torch.float32, device=x.device) if stats else None
-    m = mean.data_ptr() if stats else 0
-    st = _token_fn("layernorm_fwd", x.dtype)(
-        xr.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), y.data_ptr(),
-        m, m + 4 * R if stats else 0, R, x.shape[-1], eps, _stream())
-    if st:
-        _chk(st, "indm_layernorm_fwd")
-    return y, mean
-
-
-def layernorm_bwd(dy, x, gamma, stats, want_gamma=True, want_beta=True):
-    """x, gamma, stats: layernorm_fwd's -> dx, dgamma, dbeta (fp32 [C]; None where not wanted).  The scratch is an allocation of its
-    own: calls on different streams, or in different captured graphs, share nothing."""
-    if dy.dtype != x.dtype or dy.shape != x.shape:
-        _refuse(f"layer_norm: dy is {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    away = _token_device("layer_norm", x, dy, gamma, stats)
-    if away is not None:
-        with away:
-            return layernorm_bwd(dy, x, gamma, stats, want_gamma, want_beta)
-    C = x.shape[-1]
-    if gamma is not None and not gamma.is_contiguous():
-        gamma = gamma.contiguous()
-    if not dy.is_contiguous():
-        dy = dy.contiguous()
-    xr, R, ldx = _rows2d(x)
-    dx, dgamma, dbeta, ws = _like(x), None, None, None
-    if want_gamma:
-        dgamma = torch.empty((C,), dtype=torch.float32, device=x.device)
-    if want_beta:
-        dbeta = torch.empty((C,), dtype=torch.float32, device=x.device)
-    if want_gamma or want_beta:
-        ws = torch.empty((lib().indm_layernorm_bwd_ws_floats(R, C, x.element_size()) or 1,), dtype=torch.float32, device=x.device)
-    m = stats.data_ptr()
-    st = _token_fn("layernorm_bwd", x.dtype)(
-        dy.data_ptr(), xr.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(), m, m + 4 * R, dx.data_ptr(),
-        None if dgamma is None else dgamma.data_ptr(), None if dbeta is None else dbeta.data_ptr(), None if ws is None else ws.data_ptr(),
-        R, C, _stream())
-    if st:
-        _chk(st, "indm_layernorm_bwd")
-    return dx, dgamma, dbeta
-
-
-def dropout(x, p, seed, res=None, seed_dev=None):
-    """(res) + keep(seed + *seed_dev) x / (1 - p), the mask by x's dense (row-major) element index"""
-    fn = _token_fn("dropout", x.dtype)
-    if not 0.0 <= p <= 1.0:
-        _refuse(f"dropout: 0 <= p <= 1, got {p}")
-    if not 0 <= seed < 1 << 64:
-        _refuse(f"dropout: the seed is a whole number of 64 bits, got {seed}")
-    if res is not None and (res.shape != x.shape or res.dtype != x.dtype):
-        _refuse(f"dropout: res is {tuple(x.shape)} {x.dtype}, got {tuple(res.shape)} {res.dtype}")
-    if seed_dev is not None and (seed_dev.dtype != torch.int64 or seed_dev.numel() != 1):
-        _refuse("dropout: seed_dev is one int64 on the device")
-    away = _token_device("dropout", x, res, seed_dev)
-    if away is not None:
-        with away:
-            return dropout(x, p, seed, res, seed_dev)
-    if not x.is_contiguous():
-        x = x.contiguous()
-    if res is not None and not res.is_contiguous():
-        res = res.contiguous()
-    y = torch.empty_like(x)
-    st = fn(x.data_ptr(), None if res is None else res.data_ptr(), y.data_ptr(), x.numel(), p, seed, _seed_ptr(seed_dev), _stream())
-    if st:
-        _chk(st, "indm_dropout")
-    return y
-
-
-_POS_TYPES = {torch.int32: 0, torch.float32: 1, torch.int64: 2}
-
-
-def _rotary_check(q, k, pos, freqs, sections):
-    if q.dtype not in _TOKEN_DTYPES:
-        _refuse(f"rotary: expected float32 or bfloat16, got {q.dtype}")
-    if q.dim() != 4:
-        _refuse(f"rotary: q is [B, T, H, D], got {tuple(q.shape)}")
-    B, T, _, D = q.shape
-    if D > 4096:
-        _refuse(f"rotary: heads of up to 4096 entries, got {D}")
-    if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D):
-        _refuse(f"rotary: k is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
-    A, R = len(sections), sum(sections)
-    if not 1 <= A <= 8 or R > D or any(n < 2 or n % 2 for n in sections):
-        _refuse(f"rotary: sections are 1 to 8 even positive numbers that sum to {D} at most, got {tuple(sections)}")
-    if pos.dtype not in _POS_TYPES:
-        _refuse(f"rotary: positions are int32, int64 or float32, got {pos.dtype}")
-    if pos.shape != (T, A) and pos.shape != (B, T, A):
-        _refuse(f"rotary: pos is [{T}, {A}] or [{B}, {T}, {A}], got {tuple(pos.shape)}")
-    if freqs.dtype != torch.float64 or freqs.shape != (R // 2,):
-        _refuse(f"rotary: freqs is float64 [{R // 2}], got {tuple(freqs.shape)} {freqs.dtype}")
-
-
-def rotary(q, k, pos, freqs, sections, interleaved=False, inverse=False):
-    """q [B, T, H, D], k [B, T, Hk, D] or None -> their rotated copies (dense)"""
-    _rotary_check(q, k, pos, freqs, sections)
-    away = _token_device("rotary", q, k, pos, freqs)
-    if away is not None:
-        with away:
-            return rotary(q, k, pos, freqs, sections, interleaved, inverse)
-    B, T, H, D = q.shape
-    if q.stride(3) != 1 and D > 1:
-        q = q.contiguous()
-    sq, A = q.stride(), len(sections)
-    yq = _like(q)
-    if k is None:
-        Hk, pk, pyk, sk, yk = 0, None, None, sq, None
-    else:
-        if k.stride(3) != 1 and D > 1:
-            k = k.contiguous()
-        yk = _like(k)
-        Hk, pk, pyk, sk = k.shape[2], k.data_ptr(), yk.data_ptr(), k.stride()
-    if not pos.is_contiguous():
-        pos = pos.contiguous()
-    if not freqs.is_contiguous():
-        freqs = freqs.contiguous()
-    st = _token_fn("rotary", q.dtype)(
-        q.data_ptr(), pk, yq.data_ptr(), pyk, (c_l * 6)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2]), B, T, H, Hk, D, pos.data_ptr(),
-        _POS_TYPES[pos.dtype], T * A if pos.dim() == 3 else 0, freqs.data_ptr(), (c_i * A)(*sections), A, interleaved, inverse, _stream())
-    if st:
-        _chk(st, "indm_rotary")
-    return yq, yk
-
-
-def _aligned_rows(x):
-    """x [B, T, heads, D] with D contiguous, every row on 16 bytes and tokens at most 2^22 elements apart; a copy where it is not so"""
-    s, e = x.stride(), 16 // x.element_size()
-    if s[3] == 1 and s[0] % e == 0 and s[1] % e == 0 and s[2] % e == 0 and s[1] <= 1 << 22 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _wattn_check(q, k, v, left, right, sinks, lengths, scale):
-    if q.dtype not in _TOKEN_DTYPES:
-        _refuse(f"window_attention: expected float32 or bfloat16, got {q.dtype}")
-    if q.dim() != 4:
-        _refuse(f"window_attention: q is [B, T, H, D], got {tuple(q.shape)}")
-    B, T, H, D = q.shape
-    for x in (k, v):
-        if x.dtype != q.dtype or x.dim() != 4 or x.shape[:2] != q.shape[:2] or x.shape[3] != D or x.shape != k.shape:
-            _refuse(f"window_attention: {'k' if x is k else 'v'} is [{B}, {T}, Hk, {D}] {q.dtype}, got {tuple(x.shape)} {x.dtype}")
-    Hk = k.shape[2]
-    if H < 1 or Hk < 1 or H % Hk:
-        _refuse(f"window_attention: the {H} heads of q are a multiple of the {Hk} of k and v")
-    if D % 8 or not 8 <= D <= 128:
-        _refuse(f"window_attention: heads of 8, 16, ... 128 entries, got {D}")
-    if T > 1 << 28 or H * D > 1 << 22:
-        _refuse(f"window_attention: up to {1 << 28} tokens of {1 << 22} entries, got {T} of {H * D}")
-    if left < 0 or right < 0 or sinks < 0:
-        _refuse(f"window_attention: window and sinks >= 0, got ({left}, {right}), {sinks}")
-    if not 0.0 < scale < float("inf"):
-        _refuse(f"window_attention: scale > 0, got {scale}")
-    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
-        _refuse(f"window_attention: lengths is int32 [{B}], got {tuple(lengths.shape)} {lengths.dtype}")
-
-
-def wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats=True):
-    """-> o [B, T, H, D]; with stats for the backward: what rounding o to bf16 left (None for float32) and lse [B, H, T]; and q, k, v as
-    the kernel read them (copies where rows were not on 16 bytes)"""
-    _wattn_check(q, k, v, left, right, sinks, lengths, scale)
-    away = _token_device("window_attention", q, k, v, lengths)
-    if away is not None:
-        with away:
-            return wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale, stats)
-    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
-    if lengths is not None and not lengths.is_contiguous():
-        lengths = lengths.contiguous()
-    B, T, H, D = q.shape
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
-    strides = (c_l * 9)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
-    o, olo, lse = _like(q), None, None
-    if stats:
-        lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device)
-        if q.dtype == torch.bfloat16:
-            olo = torch.empty_like(o)
-    st = _token_fn("wattn_fwd", q.dtype)(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), None if olo is None else olo.data_ptr(),
-        None if lse is None else lse.data_ptr(), None if lengths is None else lengths.data_ptr(), B, T, H, k.shape[2], D, min(left, T),
-        min(right, T), min(sinks, T), causal, scale, _stream())
-    if st:
-        _chk(st, "indm_wattn_fwd")
-    return o, olo, lse, q, k, v
-
-
-def wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale):
-    """-> dq, dk, dv (dense).  q, k, v, o, olo, lse: wattn_fwd's, which checked the arguments.  The scratch is an allocation of its own."""
-    if do.dtype != q.dtype or do.shape != q.shape:
-        _refuse(f"window_attention: do is {tuple(q.shape)} {q.dtype}, got {tuple(do.shape)} {do.dtype}")
-    away = _token_device("window_attention", q, k, v, o, lse, do, lengths)
-    if away is not None:
-        with away:
-            return wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale)
-    if not do.is_contiguous():
-        do = do.contiguous()
-    if do.data_ptr() % 16:
-        do = do.clone()
-    if lengths is not None and not lengths.is_contiguous():
-        lengths = lengths.contiguous()
-    B, T, H, D = q.shape
-    Hk, left, right, sinks = k.shape[2], min(left, T), min(right, T), min(sinks, T)
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
-    strides = (c_l * 9)(sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
-    dq, dk, dv = _like(q), _like(k), _like(v)
-    ws = torch.empty((lib().indm_wattn_bwd_ws_floats(B, T, H, Hk, D, left, right, sinks, causal) or 1,), dtype=torch.float32, device=q.device)
-    st = _token_fn("wattn_bwd", q.dtype)(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, o.data_ptr(), None if olo is None else olo.data_ptr(), do.data_ptr(),
-        lse.data_ptr(), None if lengths is None else lengths.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), B, T, H,
-        Hk, D, left, right, sinks, causal, scale, _stream())
-    if st:
-        _chk(st, "indm_wattn_bwd")
-    return dq, dk, dv
+            from . import _token as ext
+        except ImportError as e:
+            raise RuntimeError("indm_amd: indm_amd/_token.so is missing or does not load. Build it with `python -c 'import __graft_entry__ as g; "
+                               "g.build()'` or `make -C indm_amd/csrc`. There is no CPU fallback.") from e
+        ext.bind({name: ctypes.cast(getattr(L, name), c_p).value for name in _SIGS
+                  if name.startswith(("indm_layernorm_", "indm_dropout_", "indm_rotary_", "indm_wattn_"))})
+        _token[0] = ext
+    return _token[0]

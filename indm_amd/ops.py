@@ -10,7 +10,6 @@ import math
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -964,58 +963,11 @@ def slogdet(w):
     return _SlogdetInv.apply(w)
 
 
-# ----------------------------------------------------------------------------- a block over tokens (csrc/token_ops.hip, window_attn.hip)
-def _tracked(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _once(backward):
-    """once_differentiable, whose bookkeeping (some microseconds) is only needed where the backward pass is itself recorded"""
-    recorded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return run
-
-
-class _LayerNorm(Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, eps):
-        y, stats = hip.layernorm_fwd(x, gamma, beta, eps)
-        ctx.save_for_backward(x, gamma, stats)
-        return y
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        x, gamma, stats = ctx.saved_tensors
-        _, want_gamma, want_beta, _ = ctx.needs_input_grad
-        dx, dg, db = hip.layernorm_bwd(dy, x, gamma, stats, want_gamma, want_beta)
-        return dx, dg, db, None
-
-
+# ----------------------------------------------------------------------------- a block over tokens (csrc/token_ops.hip, window_attn.hip, token_bind.cpp)
 def layer_norm(x, gamma=None, beta=None, eps=1e-6):
     """Layer norm over the last dimension of x [..., C] (fp32 or bf16, any strides), times gamma [C], plus beta [C] (fp32; either
     may be None).  Statistics and the sums of the parameters' gradients are fp32; the same bits on every call."""
-    if not _tracked(x, gamma, beta):
-        return hip.layernorm_fwd(x, gamma, beta, eps, stats=False)[0]
-    return _LayerNorm.apply(x, gamma, beta, float(eps))
-
-
-class _Dropout(Function):
-    @staticmethod
-    def forward(ctx, x, res, p, seed):
-        sd = hip.SEED_DEV[0] if p > 0 else None
-        ctx.cfg = (p, seed, sd)
-        return hip.dropout(x, p, seed, res, sd)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dy):
-        p, seed, sd = ctx.cfg
-        dx = hip.dropout(dy, p, seed, None, sd) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+    return hip.token_ops().layer_norm(x, gamma, beta, eps)
 
 
 def dropout(x, p, seed, res=None):
@@ -1023,7 +975,9 @@ def dropout(x, p, seed, res=None):
     of (seed, element index) -- the one group_norm(drop_p=, seed=) applies for the same seed --, is regenerated in the backward pass
     and never stored; seeds come from rng.dropout_seed().  fp32 or bf16; dropped elements are 0 whatever x holds.  A captured graph
     replays the seed that it was captured with, unless hip.SEED_DEV holds a device offset to it (as graphed.py sets it)."""
-    return _Dropout.apply(x, res, float(p), int(seed))
+    if not 0 <= seed < 1 << 64:
+        raise RuntimeError(f"indm_amd: dropout: the seed is a whole number of 64 bits, got {seed}")
+    return hip.token_ops().dropout(x, p, seed, res, hip.SEED_DEV[0])
 
 
 def rotary_freqs(sections, base=10000.0, device=None):
@@ -1032,52 +986,12 @@ def rotary_freqs(sections, base=10000.0, device=None):
     return torch.cat([float(base) ** (-2.0 * torch.arange(int(n) // 2, dtype=torch.float64) / int(n)) for n in sections]).to(device)
 
 
-class _Rotary(Function):
-    @staticmethod
-    def forward(ctx, q, k, pos, freqs, sections, interleaved):
-        ctx.save_for_backward(pos, freqs)
-        ctx.cfg = (sections, interleaved)
-        ctx.set_materialize_grads(False)
-        return hip.rotary(q, k, pos, freqs, sections, interleaved)
-
-    @staticmethod
-    @_once
-    def backward(ctx, dq, dk):
-        pos, freqs = ctx.saved_tensors
-        sections, interleaved = ctx.cfg
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
-        if dq is None:
-            if dk is not None:
-                dk = hip.rotary(dk, None, pos, freqs, sections, interleaved, inverse=True)[0]
-        else:
-            dq, dk = hip.rotary(dq, dk, pos, freqs, sections, interleaved, inverse=True)
-        return dq, dk, None, None, None, None
-
-
 def rotary(q, k, pos, freqs, sections, interleaved=False):
     """Rotary positions over several axes (time, height, width of image or clip tokens) -> (q', k').  q [B, T, H, D], k [B, T, Hk, D] or
     None, fp32 or bf16, any strides (columns of one fused product).  sections: entries of a head per axis (even), the rest passes
     through; pos [T, A] or [B, T, A] (int32, int64 or fp32), the token's coordinate on each axis; freqs from rotary_freqs().  A pair
     (a, b) -> (a cos - b sin, b cos + a sin) of the angle pos freq; pairs are the halves of a section, or neighbours if interleaved."""
-    return _Rotary.apply(q, k, pos, freqs, sections, bool(interleaved))
-
-
-class _WindowAttention(Function):
-    @staticmethod
-    def forward(ctx, q, k, v, left, right, sinks, causal, lengths, scale):
-        o, olo, lse, q, k, v = hip.wattn_fwd(q, k, v, left, right, sinks, causal, lengths, scale)
-        ctx.save_for_backward(q, k, v, o, olo, lse, lengths)
-        ctx.cfg = (left, right, sinks, causal, scale)
-        return o
-
-    @staticmethod
-    @_once
-    def backward(ctx, do):
-        q, k, v, o, olo, lse, lengths = ctx.saved_tensors
-        left, right, sinks, causal, scale = ctx.cfg
-        dq, dk, dv = hip.wattn_bwd(q, k, v, o, olo, lse, do, left, right, sinks, causal, lengths, scale)
-        return dq, dk, dv, None, None, None, None, None, None
+    return hip.token_ops().rotary(q, k, pos, freqs, sections, interleaved)
 
 
 def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, scale=None):
@@ -1088,11 +1002,8 @@ def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, 
     they are visible to nobody, whatever they hold, and their rows of o and of the gradients are zeros.  scale: default D ** -0.5."""
     left, right = window if isinstance(window, (tuple, list)) else (window, window)
     far = q.shape[1] if q.dim() > 1 else 0
-    left, right = far if left is None else int(left), far if right is None else int(right)
-    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
-    if not _tracked(q, k, v):
-        return hip.wattn_fwd(q, k, v, left, right, int(sinks), bool(causal), lengths, scale, stats=False)[0]
-    return _WindowAttention.apply(q, k, v, left, right, int(sinks), bool(causal), lengths, scale)
+    left, right = far if left is None else min(left, far), far if right is None else min(right, far)
+    return hip.token_ops().window_attention(q, k, v, left, right, min(sinks, far), causal, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
 
 
 INV_SQRT2 = 1.0 / math.sqrt(2.0)
