@@ -279,6 +279,7 @@ void rotary_check(const Tensor& q, const Tensor& k, const Tensor& pos, const Ten
     REFUSE("rotary: pos is [", T, ", ", A, "] or [", B, ", ", T, ", ", A, "], got ", pos.sizes());
   if (freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || freqs.size(0) != sum / 2)
     REFUSE("rotary: freqs is float64 [", sum / 2, "], got ", freqs.sizes(), " ", freqs.scalar_type());
+  if (c10::GradMode::is_enabled() && (pos.requires_grad() || freqs.requires_grad())) REFUSE("rotary: positions and frequencies have no gradient; detach them");
   on_one_gpu("rotary", {&q, &k, &pos, &freqs});
 }
 Tensor unit_columns(const Tensor& x) { return !x.defined() || x.stride(3) == 1 || x.size(3) == 1 ? x : x.contiguous(); }

@@ -425,7 +425,7 @@ int launch_ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const f
   constexpr int BLOCK = L > 256 ? L : 256, TEAMS = BLOCK / L, RPT = ln_bwd_rpt(Row<T>::V, NV, L);
   const int nb = ln_bwd_blocks(R, TEAMS, sizeof(T));
   const bool params = dgamma != nullptr || dbeta != nullptr;
-  const size_t lds = params && L < 256 ? 2 * (size_t)C * sizeof(float) : 0;   // (at most 2 x 2048 floats: four teams of 64 lanes)
+  const size_t lds = params && L < 256 ? 2 * (size_t)C * sizeof(float) : 0;   // (at most 2 x 1024 floats: four teams of 64 lanes with 16 elements each)
   if (R >= (long)nb * TEAMS * RPT)
     hipLaunchKernelGGL((layernorm_bwd_kernel<T, L, NV, RPT>), dim3(nb), dim3(BLOCK), lds, st, dy, x, ldx, gamma, mean, rstd, dx,
                        params ? part : nullptr, R, C);
@@ -754,7 +754,7 @@ int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, lon
   a.tb = (int)tb;
   const size_t lds = ((size_t)tb * pairs + 1) / 2 * 2 * sizeof(float2) + tb * sizeof(long2) + nvec * (sizeof(int2) + sizeof(int));
   const long nb = (tokens + tb - 1) / tb;
-  if (nb > 0x7fffffffL || per * tb > 0x3fffffffL) return INDM_E_SHAPE;
+  if (nb > 0x7fffffffL || per * Row<T>::V * tb > 0x3fffffffL) return INDM_E_SHAPE;   // (a workgroup's own offsets are 32-bit)
 #define ROT_LAUNCH(P)                                                                                             \
   do {                                                                                                            \
     if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, P, true>), dim3((unsigned)nb), dim3(lanes), lds, st, a);  \

@@ -822,8 +822,7 @@ int run_key(WAttnArgs p, hipStream_t st) {
       (SHARE ? WV : 1) * 2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
 }
 inline int run_join(const WAttnArgs& p, hipStream_t st) {
-  const int n = p.sinks * 2 * p.D;
-  if ((long)p.B * p.Hk > 65535 || (long)p.sinks * 2 * p.D > 0x7fffffffL) return INDM_E_SHAPE;
+  const int n = p.sinks * 2 * p.D;   // (several chunks only for up to 128 sink blocks of all heads: few rows of few values)
   hipLaunchKernelGGL(wattn_join_kernel, dim3(cdiv(n, 64), p.B * p.Hk), dim3(256), 0, st, p.part, p.chunks, n);
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }

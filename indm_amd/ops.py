@@ -990,7 +990,8 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     """Rotary positions over several axes (time, height, width of image or clip tokens) -> (q', k').  q [B, T, H, D], k [B, T, Hk, D] or
     None, fp32 or bf16, any strides (columns of one fused product).  sections: entries of a head per axis (even), the rest passes
     through; pos [T, A] or [B, T, A] (int32, int64 or fp32), the token's coordinate on each axis; freqs from rotary_freqs().  A pair
-    (a, b) -> (a cos - b sin, b cos + a sin) of the angle pos freq; pairs are the halves of a section, or neighbours if interleaved."""
+    (a, b) -> (a cos - b sin, b cos + a sin) of the angle pos freq; pairs are the halves of a section, or neighbours if interleaved.
+    Gradients go to q and k only: pos or freqs that require one are refused."""
     return hip.token_ops().rotary(q, k, pos, freqs, sections, interleaved)
 
 
@@ -999,11 +1000,13 @@ def window_attention(q, k, v, window=None, sinks=0, causal=False, lengths=None, 
     k, v [B, T, Hk, D] (H a multiple of Hk: groups of heads share a key head; fp32 or bf16, any strides, D a multiple of 8 up to 128).
     Token j is visible to token i when i - left <= j <= i + right or j < sinks, and, if causal, j <= i.  window: (left, right), one
     number for both sides, or None; None for a side: no limit.  lengths: int32 [B], tokens from lengths[b] on belong to no sequence --
-    they are visible to nobody, whatever they hold, and their rows of o and of the gradients are zeros.  scale: default D ** -0.5."""
+    they are visible to nobody, whatever they hold, and their rows of o and of the gradients are zeros.  scale: default D ** -0.5.
+    Values inside a sequence are finite: a NaN or an infinity there meets zero weights too, on rows up to 64 tokens beyond the window
+    that sees it, and on every row if it is within 32 tokens of the sinks."""
     left, right = window if isinstance(window, (tuple, list)) else (window, window)
-    far = q.shape[1] if q.dim() > 1 else 0
+    far, D = (q.shape[1], q.shape[3]) if q.dim() == 4 else (0, 0)
     left, right = far if left is None else min(left, far), far if right is None else min(right, far)
-    return hip.token_ops().window_attention(q, k, v, left, right, min(sinks, far), causal, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
+    return hip.token_ops().window_attention(q, k, v, left, right, min(sinks, far), causal, lengths, max(D, 1) ** -0.5 if scale is None else scale)
 
 
 INV_SQRT2 = 1.0 / math.sqrt(2.0)

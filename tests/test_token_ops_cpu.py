@@ -70,6 +70,8 @@ def _rot(q=None, k=None, pos=None, freqs=None, sections=(4, 4), **kw):
     (dict(pos=t(5, 2, dtype=torch.float64)), "positions are"),
     (dict(freqs=ops.rotary_freqs((4, 6))), "freqs is"),
     (dict(freqs=ops.rotary_freqs((4, 4)).float()), "freqs is"),
+    (dict(freqs=ops.rotary_freqs((4, 4)).requires_grad_()), "no gradient"),
+    (dict(pos=t(5, 2).requires_grad_()), "no gradient"),
     ({}, "no CPU fallback"),
 ])
 def test_rotary_refuses(kw, what):

@@ -173,6 +173,21 @@ def test_layer_norm_offset_rows_keep_their_variance():
     close(y, want, 48 * U * 4100 + 60 * U * 5, "y")
 
 
+def test_layer_norm_offsets_past_32_bits():
+    """2^31 and more elements: the last rows come out as those rows alone do, and their gradients"""
+    R, C = (1 << 22) + 5, 520
+    x = torch.zeros((R, C), dtype=torch.bfloat16, device=DEV)
+    x[-9:] = randn((9, C), 90, torch.bfloat16, 2.0, 1.0)
+    x.requires_grad_()
+    dy = torch.zeros((R, C), dtype=torch.bfloat16, device=DEV)
+    dy[-9:] = randn((9, C), 91, torch.bfloat16)
+    tail, dtail = x.detach()[-9:].clone().requires_grad_(), dy[-9:].clone()
+    y, yt = ops.layer_norm(x), ops.layer_norm(tail)
+    assert torch.equal(y[-9:], yt) and (y[:-9:100_003] == 0).all()
+    (g,), (gt,) = torch.autograd.grad(y, x, dy), torch.autograd.grad(yt, tail, dtail)
+    assert torch.equal(g[-9:], gt) and (g[:-9:100_003] == 0).all()
+
+
 def test_layer_norm_infinities_stay_in_their_rows():
     x = randn((6, 96), 18)
     clean = ops.layer_norm(x)
@@ -424,6 +439,16 @@ def test_rotary_only_one_gradient_wanted():
     rot_close(gk, torch.ones_like(gk), pos, freqs, (8,), False, -1.0, "dk")
     (gq,) = torch.autograd.grad(yq.sum(), q)
     rot_close(gq, torch.ones_like(gq), pos, freqs, (8,), False, -1.0, "dq")
+
+
+def test_rotary_offsets_past_32_bits():
+    T, H, D = 70_003, 250, 128
+    q = torch.zeros((1, T, H, D), dtype=torch.bfloat16, device=DEV)
+    q[:, -5:] = randn((1, 5, H, D), 92, torch.bfloat16)
+    freqs, pos = ops.rotary_freqs((64, 32), device=DEV), torch.randint(0, 300, (T, 2), generator=gen(93), device=DEV)
+    y, _ = ops.rotary(q, None, pos, freqs, (64, 32))
+    alone, _ = ops.rotary(q[:, -5:].clone(), None, pos[-5:], freqs, (64, 32))
+    assert torch.equal(y[:, -5:], alone) and (y[:, :-5:1009] == 0).all()
 
 
 def test_rotary_empty():

@@ -20,6 +20,8 @@ def call(q=None, k=None, v=None, **kw):
 @pytest.mark.parametrize("kw,what", [
     (dict(q=t(2, 5, 4, 16, dtype=torch.float16)), "float32 or bfloat16"),
     (dict(q=t(5, 4, 16)), r"q is \[B, T, H, D\]"),
+    (dict(q=t()), r"q is \[B, T, H, D\]"),
+    (dict(q=t(2, 5, 4, 0), k=t(2, 5, 4, 0)), "8, 16"),
     (dict(k=t(2, 4, 2, 16)), "k is"),
     (dict(k=t(2, 5, 2, 8)), "k is"),
     (dict(k=t(2, 5, 2, 16, dtype=torch.bfloat16)), "k is"),

@@ -179,6 +179,42 @@ def test_strides(guards, dtype, how):
     assert guards.broken_guards() == 0
 
 
+def test_offsets_past_32_bits():
+    """more than 2^31 elements in every tensor: the last tokens against the definition on the tokens that they reach"""
+    T, H, D, n = 140_000, 124, 128, 40
+    xs = [torch.zeros((1, T, H, D), dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+    for i, x in enumerate(xs):
+        x[:, -n:] = randn((1, n, H, D), 110 + i, torch.bfloat16)
+    leaves = [x.requires_grad_() for x in xs[:3]]
+    o = ops.window_attention(*leaves, (n, 0))
+    grads = torch.autograd.grad(o, leaves, xs[3])
+    want, tol = reference(*(x.detach()[:, -2 * n:] for x in xs), n, 0, 0, False, None, D ** -0.5)
+    for name, got, w, e in zip(("o", "dq", "dk", "dv"), (o.detach(), *grads), want, tol):
+        close(got[:, -n:], w[:, -n:], e[:, -n:], name)
+    assert (o.detach()[:, :-2 * n:997] == 0).all() and (grads[2][:, :-2 * n:997] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_is_not_finite_stays_near(dtype):
+    """a token of NaN leaves the rows beyond its window and 64 more as they are, bit for bit"""
+    T, w, at = 600, 20, 333
+    xs = [randn((1, T, h, 64), 120 + i, dtype) for i, h in enumerate((4, 2, 2, 4))]
+    runs = []
+    for bad in (False, True):
+        leaves = [x.clone() for x in xs]
+        if bad:
+            for x in leaves:
+                x[:, at] = math.nan
+        *qkv, do = leaves
+        qkv = [x.requires_grad_() for x in qkv]
+        o = ops.window_attention(*qkv, w, sinks=3)
+        runs.append((o.detach(), *torch.autograd.grad(o, qkv, do)))
+    far = (torch.arange(T, device=DEV) - at).abs() > w + 64
+    sinks = torch.arange(T, device=DEV) < 3      # (they gather from every query: their dk and dv)
+    for clean, got in zip(*runs):
+        assert torch.equal(clean[:, far & ~sinks], got[:, far & ~sinks])
+
+
 def test_large_logits_keep_the_row_maximum():
     """logits of several hundred, growing along the keys, so that the running maximum has to be raised again and again"""
     T = 500
