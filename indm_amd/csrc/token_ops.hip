@@ -498,31 +498,32 @@ __device__ __forceinline__ void keep4(uint64_t seed, uint64_t idx4, uint32_t dro
   k[3] = (c3 >> 8) >= drop;
 }
 
-// y = (res) + keep x / (1 - p).  A dropped element is 0 whatever x holds there (also an infinity or a NaN).
+// y = (res) + keep x / (1 - p).  A dropped element is 0 whatever x holds there (also an infinity or a NaN).  HBM-bound, with the
+// generator's products close behind: 20 of them at a quarter of the rate for every 4 elements, 17 of the 25 us below.  One vector a
+// lane, nothing carried over: 2^25 elements of bf16 take 25 us (5.4 TB/s; a loop of 8 vectors a lane 27), with a residual 39 us (5.2
+// TB/s; 40), 2^22 + 3 of fp32 6.8 us.  Stores that bypass the caches measured 22 and 30 us on the same tensors again and again, but no
+// gain on fresh ones, and the layer norm that reads 128 MB next lost 10 us to them.
 template <typename T, bool RES>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, long n,   // (y may be x or res)
                                                       uint32_t drop, float factor, uint64_t seed, const uint64_t* seed_dev) {
   constexpr int V = Row<T>::V;
   if (seed_dev) seed += *seed_dev;
-  const long nv = (n + V - 1) / V;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < nv; i += (long)gridDim.x * 256) {
-    const long at = i * V;
-    const int left = n - at < V ? (int)(n - at) : V;
-    float v[V], w[V], o[V];
-    load_part<T>(x + at, left, v);
-    if constexpr (RES) load_part<T>(res + at, left, w);
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, at = i * V;
+  const int left = n - at < V ? (int)(n - at) : V;
+  float v[V], w[V], o[V];
+  load_part<T>(x + at, left, v);
+  if constexpr (RES) load_part<T>(res + at, left, w);
 #pragma unroll
-    for (int h = 0; h < V; h += 4) {
-      bool k[4];
-      keep4(seed, (uint64_t)i * (V / 4) + h / 4, drop, k);
+  for (int h = 0; h < V; h += 4) {
+    bool k[4];
+    keep4(seed, (uint64_t)i * (V / 4) + h / 4, drop, k);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[h + e] = k[e] ? v[h + e] * factor : 0.f;
-        if constexpr (RES) o[h + e] += w[h + e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      o[h + e] = k[e] ? v[h + e] * factor : 0.f;
+      if constexpr (RES) o[h + e] += w[h + e];
     }
-    store_part<T>(y + at, left, o);
   }
+  store_part<T>(y + at, left, o);
 }
 
 template <typename T>
@@ -533,11 +534,12 @@ int dropout(const T* x, const T* res, T* y, long n, float p, uint64_t seed, cons
   if (x == nullptr || y == nullptr) return INDM_E_ARG;
   const float factor = p < 1.f ? 1.f / (1.f - p) : 0.f;   // p = 1 drops every element: word >> 8 < 2^24
   const uint32_t drop = (uint32_t)(p * 16777216.f);
-  const int grid = ew_grid((n + Row<T>::V - 1) / Row<T>::V, 256);
+  const long grid = (n + 256L * Row<T>::V - 1) / (256L * Row<T>::V);
+  if (grid > 0x7fffffffL) return INDM_E_SHAPE;
   if (res != nullptr)
-    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3(grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
+    hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
   else
-    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3(grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
+    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, st, x, res, y, n, drop, factor, seed, seed_dev);
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 
@@ -546,10 +548,13 @@ int dropout(const T* x, const T* res, T* y, long n, float p, uint64_t seed, cons
 // pos[token][axis of the pair's section] * freqs[pair]; the rest passes through.  A pair of a section of n entries at offset o is
 // (o + j, o + n/2 + j), or (o + 2 j, o + 2 j + 1) when interleaved.  The angle is formed and reduced to a quadrant in 64 bits
 // (a far position times a frequency needs more than fp32's 24 bits), its sine and cosine on [-pi/4, pi/4] in fp32.
-// A workgroup takes tb tokens: their sines and cosines go to LDS once (one 64-bit angle a thread, not one per head), then its
-// lanes stream over the tokens' vectors (V entries of a head) in memory order -- the heads of a token are one contiguous run.
-// The mate of a vector whose entries all lie in one half of a section is one more (cached) vector load; a vector that a border
-// cuts takes its mates one by one.
+// A workgroup takes tp positions of ts samples that share them: their sines and cosines go to LDS once (one 64-bit angle a thread, not
+// one per head and sample).  A head is cut
+// into units of one vector (V entries): a unit of a section's first half takes its second half along, so that every entry is loaded
+// once; an interleaved section's units hold whole pairs, the rest of the head passes through.  What no unit covers (halves, or a rest,
+// that are no multiple of V) goes entry by entry.  Bound by HBM and, half as much, by the angles: 64 x 1024 tokens of 8 heads of 64
+// entries (q and k out of a fused product, bf16, 134 MB) take 29 us (4.6 TB/s; a copy of as much 24 us); with every vector loading its
+// mates a second time they took 34 us.
 constexpr int ROT_AXES = 8, ROT_MAX_D = 4096;
 
 struct RotArgs {
@@ -558,113 +563,127 @@ struct RotArgs {
   long sb[2], st[2], sh[2];
   int heads[2];
   const void* pos;    // [T, A] or [B, T, A]
-  long pos_sb;        // 0: shared by the batch
   const double* freqs;
-  long B, T;
-  int D, axes, tb;
+  long T, S, N;       // tokens of a sample; positions that differ, and the samples that share them: T and B, or B T and 1
+  long tiles;         // of positions
+  int D, axes, ts, tp, units, loose;   // ts samples at tp positions a workgroup
   int end[ROT_AXES];  // end offset of each section
   float sign;         // -1: the inverse rotation (the backward pass)
 };
 
-// entry d of a head: its pair, the offset of the pair's other entry (0: passes through) and whether it is the second
-struct RotEntry {
-  int pair, mate;
-  bool second;
-};
-template <bool INTER>
-__device__ __forceinline__ RotEntry rot_entry(const RotArgs& a, int d) {
-  int from = 0;
-  for (int k = 0; k < a.axes; ++k) {
-    const int end = a.end[k];
-    if (d < end) {
-      const int in = d - from, half = (end - from) >> 1;
-      if (INTER) return {(d >> 1), (in & 1) ? -1 : 1, (in & 1) != 0};
-      return in < half ? RotEntry{(from >> 1) + in, half, false} : RotEntry{(from >> 1) + in - half, -half, true};
-    }
-    from = end;
+// the regions that are cut into units: a section's first half, or all that is interleaved; and the rest of the head.  Calls
+// f(first entry, entries, first pair, distance of the mates -- 0: passes through) for each.
+template <bool INTER, typename F>
+__host__ __device__ __forceinline__ void rot_regions(const RotArgs& a, F f) {
+  const int sum = a.end[a.axes - 1];
+  if (INTER) {
+    f(0, sum, 0, 1);
+  } else {
+    for (int k = 0, from = 0; k < a.axes; from = a.end[k++]) f(from, (a.end[k] - from) >> 1, from >> 1, (a.end[k] - from) >> 1);
   }
-  return {0, 0, false};
+  f(sum, a.D - sum, 0, 0);
 }
 
 template <typename T, typename P, bool INTER>
 __global__ __launch_bounds__(512) void rotary_kernel(RotArgs a) {
-  constexpr int V = Row<T>::V, U = 4;   // tokens a lane has in flight
-  // [tb][pairs] (cos, sin); a token's offsets in q and k; a vector's first pair and mate; the list of the vectors that are cut
+    constexpr int V = Row<T>::V, U = 4;   // tokens a lane has in flight
+  typedef typename Row<T>::raw raw;
+  // [tp][pairs] (cos, sin); a token's offsets in q and k, its index and the row of its sines; a unit's, and a loose entry's (first entry, first pair, mate)
   extern __shared__ __attribute__((aligned(16))) float2 turn[];
-  __shared__ int ncut;
-  const int nvec = (a.D + V - 1) / V, hq = a.heads[0], heads = hq + a.heads[1], pairs = a.end[a.axes - 1] >> 1;
-  long2* place = (long2*)(turn + (a.tb * pairs + 1) / 2 * 2);
-  int2* kind = (int2*)(place + a.tb);
-  int* cut = (int*)(kind + nvec);
-  const long tok0 = (long)blockIdx.x * a.tb, tokens = a.B * a.T;
-  const int nt = tokens - tok0 < a.tb ? (int)(tokens - tok0) : a.tb;
-  if (threadIdx.x == 0) ncut = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < nt * pairs; i += blockDim.x) {
-    const int t = i / pairs, j = i - t * pairs;
-    int ax = 0;
-    while (2 * j >= a.end[ax]) ++ax;    // (pairs never straddle sections; j < pairs, so ax < axes)
-    const long b = (tok0 + t) / a.T;
-    const P pos = ((const P*)a.pos)[b * a.pos_sb + (tok0 + t - b * a.T) * a.axes + ax];
-    const double quarter = (double)pos * a.freqs[j] * 0.63661977236758134308;   // the angle in units of pi / 2
-    const double q = __builtin_rint(quarter);
-    float sn, cs;
-    indm_sincos_quadrant((float)((quarter - q) * 1.57079632679489661923), (int)(q - 4.0 * __builtin_floor(q * 0.25)), sn, cs);
-    turn[i] = make_float2(cs, sn * a.sign);
-  }
+  const int hq = a.heads[0], heads = hq + a.heads[1], pairs = a.end[a.axes - 1] >> 1;
+  long4* place = (long4*)(turn + (a.tp * pairs + 1) / 2 * 2);
+  int4* unit = (int4*)(place + a.ts * a.tp);
+  int4* loose = unit + a.units;
+  const long s0 = blockIdx.x / a.tiles * a.ts, p0 = blockIdx.x % a.tiles * a.tp;
+  const int np = a.S - p0 < a.tp ? (int)(a.S - p0) : a.tp, ns = a.N - s0 < a.ts ? (int)(a.N - s0) : a.ts, nt = np * ns;
   for (int t = threadIdx.x; t < nt; t += blockDim.x) {
-    const long b = (tok0 + t) / a.T, at = tok0 + t - b * a.T;
-    place[t] = make_long2(b * a.sb[0] + at * a.st[0], b * a.sb[1] + at * a.st[1]);
+    const int s = t / np;
+    const long p = p0 + t - s * np, b = a.N > 1 ? s0 + s : p / a.T, at = a.N > 1 ? p : p - b * a.T;
+    place[t] = make_long4(b * a.sb[0] + at * a.st[0], b * a.sb[1] + at * a.st[1], (s0 + s) * a.S + p, t - s * np);
   }
-  // a vector: (its first pair, how far the mates are); (0, 0) passes through; (-1, 0) cut by a border, or the last, partial one
-  for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-    const int d0 = v * V;
-    const RotEntry first = rot_entry<INTER>(a, d0);
-    bool same = d0 + V <= a.D;
-    for (int e = 1; e < V && same; ++e) {
-      const RotEntry o = rot_entry<INTER>(a, d0 + e);
-      same = INTER ? (o.mate == 0) == (first.mate == 0) : o.mate == first.mate;
-    }
-    kind[v] = same ? make_int2(first.pair, first.mate) : make_int2(-1, 0);
-    if (!same) cut[atomicAdd(&ncut, 1)] = v;   // (their order does not matter: each is worked on by itself)
+  for (int w = threadIdx.x; w < a.units + a.loose; w += blockDim.x) {
+    int u = w, l = w - a.units;   // its place among the units, and among the loose entries
+    rot_regions<INTER>(a, [&](int from, int n, int pair, int mate) {
+      const int nu = n / V, nl = n - nu * V;
+      const int d = w < a.units ? u * V : nu * V + l;
+      if (w < a.units ? u >= 0 && u < nu : l >= 0 && l < nl)
+        unit[w] = make_int4(from + d, mate == 0 ? 0 : pair + (INTER ? d >> 1 : d), INTER && mate != 0 && (d & 1) ? -1 : mate, 0);
+      u -= nu;
+      l -= nl;
+    });
   }
   __syncthreads();
 
   const T *xq = (const T*)a.x[0], *xk = (const T*)a.x[1];
-  T *yq = (T*)a.y[0] + tok0 * hq * a.D, *yk = (T*)a.y[1] + tok0 * (heads - hq) * a.D;
-  // a lane keeps its vector and head and takes every subs-th token: only the token's offset and its sines change
-  const int per = heads * nvec, width = per < (int)blockDim.x ? per : (int)blockDim.x, subs = blockDim.x / width;
-  const int sub = threadIdx.x / width;
-  for (int i = threadIdx.x - sub * width; i < per && sub < subs; i += width) {
-    const int h = i / nvec, v = i - h * nvec;
-    const int2 kd = kind[v];
-    if (kd.x < 0) continue;
+  T *yq = (T*)a.y[0], *yk = (T*)a.y[1];
+  // a lane keeps its unit and head and takes every subs-th token: only the token's offset and its sines change
+  const int per = heads * a.units, width = per < (int)blockDim.x ? per : (int)blockDim.x, subs = width > 0 ? blockDim.x / width : 0;
+  const int sub = width > 0 ? threadIdx.x / width : 0;
+  int i = threadIdx.x - sub * width;
+  bool more = i < per && sub < subs;
+  raw own[U], mate[U];
+  const T* x = nullptr;
+  T* y = nullptr;
+  const long* at = nullptr;
+  int4 un = make_int4(0, 0, 0, 0);
+  int stride = 0, out = 0;
+  auto take = [&]() {   // item i: its unit and head
+    const int h = i / a.units;
+    un = unit[i - h * a.units];
     const bool isq = h < hq;
-    const int hw = isq ? h : h - hq, stride = (isq ? hq : heads - hq) * a.D;
-    const T* x = (isq ? xq : xk) + hw * (isq ? a.sh[0] : a.sh[1]) + v * V;
-    T* y = (isq ? yq : yk) + hw * a.D + v * V;
-    const long* at = (const long*)place + (isq ? 0 : 1);
-    const unsigned flip = kd.y > 0 ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;   // the first of a pair takes minus its mate
-    for (int t = sub; t < nt; t += subs * U) {
-      typename Row<T>::raw own[U], mate[U];
+    const int hw = isq ? h : h - hq;
+    stride = (isq ? hq : heads - hq) * a.D;
+    x = (isq ? xq : xk) + hw * (isq ? a.sh[0] : a.sh[1]) + un.x;
+    y = (isq ? yq : yk) + hw * a.D + un.x;
+    at = (const long*)place + (isq ? 0 : 1);
+    out = isq ? 2 : 1;
+  };
+  auto load = [&](int t) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int tu = t + u * subs;
-        if (tu < nt) {
-          const T* src = x + at[2 * tu];
-          own[u] = Row<T>::load(src);
-          if (!INTER && kd.y != 0) mate[u] = Row<T>::load(src + kd.y);
-        }
+    for (int u = 0; u < U; ++u) {
+      const int tu = t + u * subs;
+      if (tu < nt) {
+        const T* src = x + at[4 * tu];
+        own[u] = Row<T>::load(src);
+        if (!INTER && un.z != 0) mate[u] = Row<T>::load(src + un.z);
       }
+    }
+  };
+  if (more) {   // (the first tokens are on their way while the angles are worked out)
+    take();
+    load(sub);
+  }
+  // (a division for the first of a lane's angles only: the next ones are blockDim pairs further)
+  const int dt = blockDim.x / pairs, dj = blockDim.x - dt * pairs;
+  for (int t = threadIdx.x / pairs, j = threadIdx.x - t * pairs; t < np;) {
+    int ax = 0;
+    while (2 * j >= a.end[ax]) ++ax;    // (pairs never straddle sections; j < pairs, so ax < axes)
+    const P pos = ((const P*)a.pos)[(p0 + t) * a.axes + ax];
+    const double quarter = (double)pos * a.freqs[j] * 0.63661977236758134308;   // the angle in units of pi / 2
+    const double q = __builtin_rint(quarter);
+    float sn, cs;
+    indm_sincos_quadrant((float)((quarter - q) * 1.57079632679489661923), (int)(q - 4.0 * __builtin_floor(q * 0.25)), sn, cs);
+    turn[t * pairs + j] = make_float2(cs, sn * a.sign);
+    t += dt;
+    j += dj;
+    if (j >= pairs) {
+      j -= pairs;
+      ++t;
+    }
+  }
+  __syncthreads();
+  for (bool first = true; more; first = false) {
+    for (int t = sub; t < nt; t += subs * U) {
+      if (!first || t != sub) load(t);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int tu = t + u * subs;
         if (tu < nt) {
-          T* dst = y + tu * stride;
-          if (kd.y == 0) {
-            *(typename Row<T>::raw*)dst = own[u];
+          T* dst = y + at[4 * tu + out] * stride;
+          if (un.z == 0) {
+            *(raw*)dst = own[u];
           } else {
-            const float2* tr = turn + tu * pairs + kd.x;
+            const float2* tr = turn + (int)at[4 * tu + out + 1] * pairs + un.y;
             float p[V], o[V];
             Row<T>::unpack(own[u], p);
             if constexpr (INTER) {
@@ -674,37 +693,41 @@ __global__ __launch_bounds__(512) void rotary_kernel(RotArgs a) {
                 o[e] = __builtin_fmaf(p[e], cs.x, -p[e + 1] * cs.y);
                 o[e + 1] = __builtin_fmaf(p[e + 1], cs.x, p[e] * cs.y);
               }
+              Row<T>::store(dst, o);
             } else {
-              float m[V];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mate[u][e] ^= flip;
+              float m[V], w[V];
               Row<T>::unpack(mate[u], m);
 #pragma unroll
               for (int e = 0; e < V; ++e) {
                 const float2 cs = tr[e];
-                o[e] = __builtin_fmaf(p[e], cs.x, m[e] * cs.y);
+                o[e] = __builtin_fmaf(p[e], cs.x, -m[e] * cs.y);
+                w[e] = __builtin_fmaf(m[e], cs.x, p[e] * cs.y);
               }
+              Row<T>::store(dst, o);
+              Row<T>::store(dst + un.z, w);
             }
-            Row<T>::store(dst, o);
           }
         }
       }
     }
+    i += width;
+    more = i < per;
+    if (more) take();
   }
-  // the cut vectors, entry by entry
-  const int entries = nt * heads * ncut * V;
-  for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-    const int e = i % V, c = i / V % ncut, th = i / V / ncut, h = th % heads, t = th / heads, d = cut[c] * V + e;
-    if (d < a.D) {
-      const RotEntry r = rot_entry<INTER>(a, d);
-      const T* src = h < hq ? xq + place[t].x + h * a.sh[0] + d : xk + place[t].y + (h - hq) * a.sh[1] + d;
-      T* dst = h < hq ? yq + (t * hq + h) * a.D + d : yk + (t * (heads - hq) + h - hq) * a.D + d;
-      if (r.mate == 0) {
-        *dst = *src;
-      } else {
-        const float2 cs = turn[t * pairs + r.pair];
-        Row<T>::put(dst, __builtin_fmaf(Row<T>::get(src), cs.x, Row<T>::get(src + r.mate) * (r.second ? cs.y : -cs.y)));
-      }
+  // the loose entries of each head; a section's halves go together
+  const int entries = nt * heads * a.loose;
+  for (int w = threadIdx.x; w < entries; w += blockDim.x) {
+    const int th = w / a.loose, h = th % heads, t = th / heads;
+    const int4 un = loose[w - th * a.loose];
+    const T* src = (h < hq ? xq + place[t].x + h * a.sh[0] : xk + place[t].y + (h - hq) * a.sh[1]) + un.x;
+    T* dst = (h < hq ? yq + (place[t].z * hq + h) * a.D : yk + (place[t].z * (heads - hq) + h - hq) * a.D) + un.x;
+    if (un.z == 0) {
+      *dst = *src;
+    } else {
+      const float2 cs = turn[(int)place[t].w * pairs + un.y];
+      const float p = Row<T>::get(src), m = Row<T>::get(src + un.z);
+      Row<T>::put(dst, __builtin_fmaf(p, cs.x, un.z < 0 ? m * cs.y : -m * cs.y));
+      if (!INTER) Row<T>::put(dst + un.z, __builtin_fmaf(m, cs.x, p * cs.y));
     }
   }
 }
@@ -721,6 +744,7 @@ int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, lon
     if (sections[i] <= 0 || (sections[i] & 1) || sections[i] > D - at) return INDM_E_SHAPE;
     a.end[i] = at += sections[i];
   }
+  if (pos_sb != 0 && pos_sb != Tn * axes) return INDM_E_ARG;
   if (B == 0 || Tn == 0 || H + Hk == 0) return INDM_OK;
   if ((H > 0 && (q == nullptr || yq == nullptr)) || (Hk > 0 && (k == nullptr || yk == nullptr)) || pos == nullptr || freqs == nullptr)
     return INDM_E_ARG;
@@ -729,13 +753,20 @@ int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, lon
     a.sb[w] = strides[3 * w]; a.st[w] = strides[3 * w + 1]; a.sh[w] = strides[3 * w + 2];
   }
   a.heads[0] = H; a.heads[1] = Hk;
-  a.pos = pos; a.pos_sb = pos_sb; a.freqs = freqs; a.B = B; a.T = Tn; a.D = D; a.axes = axes;
+  a.pos = pos; a.freqs = freqs; a.T = Tn; a.D = D; a.axes = axes;
+  a.S = pos_sb == 0 ? Tn : B * Tn; a.N = pos_sb == 0 ? B : 1;
   a.sign = inverse ? -1.f : 1.f;
-  // lanes: as many whole tokens as fill wavefronts best (up to 512 lanes; a token of more vectors is walked in several steps)
-  const int nvec = cdiv(D, Row<T>::V), pairs = at / 2;
-  const long per = (long)(H + Hk) * nvec, tokens = (long)B * Tn;
+  // lanes: as many whole tokens as fill wavefronts best (up to 512 lanes; a token of more units is walked in several steps)
+  const int pairs = at / 2;
+  auto count = [&](int, int n, int, int) {
+    a.units += n / Row<T>::V;
+    a.loose += n % Row<T>::V;
+  };
+  if (interleaved) rot_regions<true>(a, count);
+  else rot_regions<false>(a, count);
+  const long heads = (long)H + Hk, per = heads * a.units, tokens = (long)B * Tn;
   int lanes = 256;
-  if (per <= 512) {
+  if (per > 0 && per <= 512) {
     double best = 0.;
     for (int k = 1; k * per <= 512; ++k) {
       const int n = (int)(k * per + 63) / 64 * 64;
@@ -747,14 +778,19 @@ int rotary(const T* q, const T* k, T* yq, T* yk, const long* strides, int B, lon
     }
   }
   // tokens a workgroup: 8 a lane where that still makes 1024 workgroups, down to one; the sines fit 32 KB of LDS
-  long tb = per <= lanes ? lanes / per * 8 : 8;
+  long tb = per > 0 && per <= lanes ? lanes / per * 8 : 8;
   if (tb > 64) tb = 64;
   while (tb > 1 && (tokens + tb - 1) / tb < 1024) tb = (tb + 1) / 2;
   while (tb > 1 && tb * pairs * (long)sizeof(float2) > 32768) tb = (tb + 1) / 2;
-  a.tb = (int)tb;
-  const size_t lds = ((size_t)tb * pairs + 1) / 2 * 2 * sizeof(float2) + tb * sizeof(long2) + nvec * (sizeof(int2) + sizeof(int));
-  const long nb = (tokens + tb - 1) / tb;
-  if (nb > 0x7fffffffL || per * Row<T>::V * tb > 0x3fffffffL) return INDM_E_SHAPE;   // (a workgroup's own offsets are 32-bit)
+  // samples that share their positions: up to four of them at one position (64 x 1024 tokens, bf16: 2 heads of 256 entries 45 -> 31 us, 8
+  // of 64 31 -> 29 us; eight or sixteen samples gain no more)
+  a.ts = a.N < 4 ? (int)a.N : 4;
+  if (a.ts > tb) a.ts = (int)tb;
+  a.tp = (int)(tb / a.ts);
+  a.tiles = (a.S + a.tp - 1) / a.tp;
+  const size_t lds = ((size_t)a.tp * pairs + 1) / 2 * 2 * sizeof(float2) + a.ts * a.tp * sizeof(long4) + (a.units + a.loose) * sizeof(int4);
+  const long nb = a.tiles * ((a.N + a.ts - 1) / a.ts);
+  if (nb > 0x7fffffffL || heads * D * tb > 0x3fffffffL) return INDM_E_SHAPE;   // (a workgroup's own offsets are 32-bit)
 #define ROT_LAUNCH(P)                                                                                             \
   do {                                                                                                            \
     if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, P, true>), dim3((unsigned)nb), dim3(lanes), lds, st, a);  \

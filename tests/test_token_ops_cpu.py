@@ -113,6 +113,7 @@ def test_c_entry_points_refuse_and_ignore_empty_work():
         assert rot(p, None, p, None, st, 1, 1, 1, 0, 16, p, 0, 0, p, (ctypes.c_int * 2)(3, 4), 2, 0, 0, None) == -1
         assert rot(p, None, p, None, st, 1, 1, 1, 0, 16, p, 0, 0, p, sec, 9, 0, 0, None) == -1
         assert rot(p, None, p, None, st, 1, 1, 1, 0, 16, p, 3, 0, p, sec, 2, 0, 0, None) == -4
+        assert rot(p, None, p, None, st, 2, 3, 1, 0, 16, p, 0, 5, p, sec, 2, 0, 0, None) == -4     # (samples' positions lie one after the other)
         assert rot(p, None, p, None, None, 1, 1, 1, 0, 16, p, 0, 0, p, sec, 2, 0, 0, None) == -4
         assert rot(None, None, p, None, st, 1, 1, 1, 0, 16, p, 0, 0, p, sec, 2, 0, 0, None) == -4
         assert rot(p, None, p, None, st, 1, 1, 1, 1, 16, p, 0, 0, p, sec, 2, 0, 0, None) == -4

@@ -386,6 +386,20 @@ def test_rotary_sizes(guards, dtype, interleaved, case):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T", [(1, 20011), (2, 9001), (5, 1501), (7, 4099), (3000, 3)])
+def test_rotary_many_tokens(guards, dtype, B, T):
+    """several tokens a workgroup, of several samples where these share their positions, and parts of both at the ends"""
+    q, k = randn((B, T, 2, 18), 54, dtype), randn((B, T, 1, 18), 55, dtype)
+    freqs = ops.rotary_freqs((8, 6), device=DEV)
+    for pos in (torch.randint(0, 300, (T, 2), generator=gen(56), device=DEV), torch.randint(0, 300, (B, T, 2), generator=gen(57), device=DEV)):
+        for interleaved in (False, True):
+            yq, yk = ops.rotary(q, k, pos, freqs, (8, 6), interleaved)
+            rot_close(yq, q, pos, freqs, (8, 6), interleaved, what="q")
+            rot_close(yk, k, pos, freqs, (8, 6), interleaved, what="k")
+    assert guards.broken_guards() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("how", ["fused product", "odd offset", "heads first", "columns not contiguous"])
 def test_rotary_strides(guards, dtype, how):
     B, T, H, Hk, D, sections = 2, 6, 4, 2, 48, (16, 24)
