@@ -250,39 +250,67 @@ __device__ __forceinline__ void load_owner(const T* row, bool live, int D, int l
     f[kk] = live && 16 * kk + 8 * lhi < D ? Op<T>::global(row + 16 * kk + 8 * lhi) : Op<T>::zero();
 }
 
-// out^T in the accumulators -> the owner's row: 16 bytes a lane and store.  (bf16: the halves trade, so that lane l31 holds elements
-// 0 .. 7 and lane l31 + 32 elements 8 .. 15 of each 16.)
-template <typename T, int DP>
-__device__ __forceinline__ void store_owner(T* row, const f32x16 (&acc)[Geo<T, DP>::DB], float f, bool live, int D, int lhi) {
+// half a block of out^T -- accumulator registers 8 half .. + 7, elements 32 db + 16 half .. + 15 of the owner's row -- times f: 16
+// bytes a lane and store.  (bf16: the halves of the wavefront trade, so that lane l31 holds elements 0 .. 7 and lane l31 + 32
+// elements 8 .. 15.)
+template <typename T>
+__device__ __forceinline__ void store_half(T* row, const float (&a)[8], float f, bool live, int d0, int D, int lhi) {
+  if constexpr (sizeof(T) == 2) {
+    unsigned w[2][2];
 #pragma unroll
-  for (int db = 0; db < Geo<T, DP>::DB; ++db) {
-    if constexpr (sizeof(T) == 2) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int a = 0; a < 4; a += 2) {
-        unsigned w[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const f32x2 v = {acc[db][4 * (a + h) + 2 * e] * f, acc[db][4 * (a + h) + 2 * e + 1] * f};
-            w[h][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
-          }
-        const u32x2 s0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false));
-        const u32x2 s1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false));
-        const u32x4 o = {s0[0], s1[0], s0[1], s1[1]};
-        const int d = 32 * db + 8 * a + 8 * lhi;
-        if (live && d < D) *(u32x4*)(row + d) = o;
+      for (int e = 0; e < 2; ++e) {
+        const f32x2 v = {a[4 * h + 2 * e] * f, a[4 * h + 2 * e + 1] * f};
+        w[h][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
       }
-    } else {
+    const u32x2 s0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false));
+    const u32x2 s1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false));
+    const u32x4 o = {s0[0], s1[0], s0[1], s1[1]};
+    const int d = d0 + 8 * lhi;
+    if (live && d < D) *(u32x4*)(row + d) = o;
+  } else {
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const f32x4 o = {acc[db][4 * a] * f, acc[db][4 * a + 1] * f, acc[db][4 * a + 2] * f, acc[db][4 * a + 3] * f};
-        const int d = 32 * db + 8 * a + 4 * lhi;
-        if (live && d < D) *(f32x4*)(row + d) = o;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 o = {a[4 * h] * f, a[4 * h + 1] * f, a[4 * h + 2] * f, a[4 * h + 3] * f};
+      const int d = d0 + 8 * h + 4 * lhi;
+      if (live && d < D) *(f32x4*)(row + d) = o;
     }
   }
 }
+template <int DB>
+__device__ __forceinline__ void half_of(const f32x16 (&acc)[DB], int u, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = acc[u >> 1][8 * (u & 1) + e];
+}
+
+// Where the wavefronts of a workgroup shared an owner block: their accumulators go to LDS (a wavefront's N vectors of four registers,
+// [vector][lane]), and each wavefront adds up some of the halves, over the wavefronts in order.
+template <int WV, int N>
+struct Join {
+  float* red;
+  int lane;
+  template <int DB>
+  __device__ __forceinline__ void leave(const f32x16 (&acc)[DB], int wave, int first) const {
+#pragma unroll
+    for (int v = 0; v < 4 * DB; ++v) {
+      const f32x4 w = {acc[v >> 2][4 * (v & 3)], acc[v >> 2][4 * (v & 3) + 1], acc[v >> 2][4 * (v & 3) + 2], acc[v >> 2][4 * (v & 3) + 3]};
+      *(f32x4*)(red + ((wave * N + first + v) * 64 + lane) * 4) = w;
+    }
+  }
+  __device__ __forceinline__ void half(int u, const float (&f)[WV], float (&v)[8]) const {   // sum of f[w] times wavefront w's half u
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WV; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 a = *(const f32x4*)(red + ((w * N + 2 * u + h) * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = __builtin_fmaf(a[e], f[w], v[4 * h + e]);
+      }
+  }
+};
 
 // workgroup -> work item, so that neighbouring items (which share most of their tiles) run on one XCD's L2
 __device__ __forceinline__ int xcd_item(int id, int total) {
@@ -475,63 +503,64 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
   }
 
   if constexpr (!BWD) sum = half_sum(sum);
-  if constexpr (SHARE) {   // join: the wavefronts leave their maximum, sum and accumulators in LDS, the first one adds them up
-    constexpr int N = G::DB * 16 + 2;
-    float* red = (float*)smem_all;
-    __syncthreads();
-    if (wave > 0) {
-      float* mine = red + (wave - 1) * N * 64 + lane;
+  float inv = sum > 0.f ? 1.f / sum : 0.f;
+  auto emit = [&](int u, float (&v)[8]) {   // a half of the result, before the division by the sum
+    if (!live) {   // (also where a visible key's values were infinite: 0 times that is not 0)
 #pragma unroll
-      for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mine[(d * 16 + r) * 64] = acc[d][r];
-      mine[(N - 2) * 64] = m;
-      mine[(N - 1) * 64] = sum;
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
     }
-    __syncthreads();
-    if (wave > 0) return;
-    for (int w = 0; w < WV - 1; ++w) {
-      const float* other = red + w * N * 64 + lane;
-      float f = 1.f, g = 1.f;
-      if constexpr (!BWD) {
-        const float mo = other[(N - 2) * 64], up = fmaxf(m, mo);
-        f = up > -INFINITY ? __builtin_amdgcn_exp2f(m - up) : 1.f;
-        g = up > -INFINITY ? __builtin_amdgcn_exp2f(mo - up) : 1.f;
-        m = up;
-        sum = sum * f + other[(N - 1) * 64] * g;
-      }
+    if constexpr (BWD) {
+      store_half<T>((T*)p.dq + orow, v, p.scale, i < p.T, 16 * u, p.D, at.lhi);
+    } else {
+      store_half<T>((T*)p.out + orow, v, inv, i < p.T, 16 * u, p.D, at.lhi);
+      if (sizeof(T) == 2 && p.olo != nullptr) {
 #pragma unroll
-      for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          acc[d][r] = BWD ? acc[d][r] + other[(d * 16 + r) * 64] : acc[d][r] * f + other[(d * 16 + r) * 64] * g;
-    }
-  }
-  if (!live) {   // (also where a visible key's values were infinite: 0 times that is not 0)
-#pragma unroll
-    for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  }
-  if constexpr (!BWD) {
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    store_owner<T, DP>((T*)p.out + orow, acc, inv, i < p.T, p.D, at.lhi);
-    if constexpr (sizeof(T) == 2) {
-      if (p.olo != nullptr) {
-#pragma unroll
-        for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float v = acc[d][r] * inv;
-            acc[d][r] = v - (float)(__bf16)v;
-          }
-        store_owner<T, DP>((T*)p.olo + orow, acc, 1.f, i < p.T, p.D, at.lhi);
+        for (int e = 0; e < 8; ++e) {
+          const float x = v[e] * inv;
+          v[e] = x - (float)(__bf16)x;
+        }
+        store_half<T>((T*)p.olo + orow, v, 1.f, i < p.T, 16 * u, p.D, at.lhi);
       }
     }
-    if (p.lse != nullptr && i < p.T && at.lhi == 0) p.lse[srow] = live ? m + __log2f(sum) : INFINITY;
+  };
+  if constexpr (SHARE) {
+    const Join<WV, 4 * G::DB> join = {(float*)smem_all, lane};
+    float2* stats = (float2*)(smem_all + WV * 4 * G::DB * 1024);
+    __syncthreads();
+    join.leave(acc, wave, 0);
+    if constexpr (!BWD) stats[wave * 64 + lane] = make_float2(m, sum);
+    __syncthreads();
+    float f[WV];
+#pragma unroll
+    for (int w = 0; w < WV; ++w) f[w] = 1.f;
+    if constexpr (!BWD) {
+      m = -INFINITY;
+      sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WV; ++w) m = fmaxf(m, stats[w * 64 + lane].x);
+#pragma unroll
+      for (int w = 0; w < WV; ++w) {
+        const float2 s = stats[w * 64 + lane];
+        f[w] = m > -INFINITY ? __builtin_amdgcn_exp2f(s.x - m) : 1.f;
+        sum += s.y * f[w];
+      }
+      inv = sum > 0.f ? 1.f / sum : 0.f;
+    }
+#pragma unroll
+    for (int u = wave; u < 2 * G::DB; u += WV) {
+      float v[8];
+      join.half(u, f, v);
+      emit(u, v);
+    }
   } else {
-    store_owner<T, DP>((T*)p.dq + orow, acc, p.scale, i < p.T, p.D, at.lhi);
+#pragma unroll
+    for (int u = 0; u < 2 * G::DB; ++u) {
+      float v[8];
+      half_of(acc, u, v);
+      emit(u, v);
+    }
   }
+  if (!BWD && p.lse != nullptr && i < p.T && at.lhi == 0 && (!SHARE || wave == 0)) p.lse[srow] = live ? m + __log2f(sum) : INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------- owner = keys: dk, dv
@@ -685,69 +714,57 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
     if (it + STEP < to) put(side ^ 1);
     staged<SHARE>();
   }
-  if constexpr (SHARE) {   // join, as in the other kernel
-    constexpr int N = G::DB * 32;
-    float* red = (float*)smem_all;
-    __syncthreads();
-    if (wave > 0) {
-      float* mine = red + (wave - 1) * N * 64 + lane;
+  const bool sunk = p.chunks > 0 && jw < p.sinks, ends = jw + 31 >= n;   // (wave-uniform)
+  auto emit = [&](int u, float (&v)[8]) {   // a half: of dk, then of dv
+    const bool first = u < 2 * G::DB;
+    const int d0 = 16 * (first ? u : u - 2 * G::DB), at0 = first ? 0 : p.D;
+    if constexpr (SINK) {
+      store_half<float>(p.part + ((((long)bh * p.chunks + share) * p.sinks + j) * 2) * p.D + at0, v, 1.f, j < p.sinks, d0, p.D, at.lhi);
+    } else if constexpr (MODE == SPLIT) {
+      store_half<float>(p.split + ((((long)share * p.B * p.Hk + bh) * p.T + j) * 2) * p.D + at0, v, 1.f, live, d0, p.D, at.lhi);
+    } else {
+      if (sunk) {   // add what the sink kernel gathered
+        const float* gathered = p.part + ((long)bh * p.chunks * p.sinks + j) * 2 * p.D + at0;
 #pragma unroll
-      for (int d = 0; d < G::DB; ++d)
+        for (int h = 0; h < 2; ++h) {
+          const int d = d0 + 8 * h + 4 * at.lhi;
+          if (d < p.D && j < p.sinks) {
+            const f32x4 more = *(const f32x4*)(gathered + d);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          mine[(d * 32 + r) * 64] = dk[d][r];
-          mine[(d * 32 + 16 + r) * 64] = dv[d][r];
-        }
-    }
-    __syncthreads();
-    if (wave > 0) return;
-    for (int w = 0; w < WV - 1; ++w) {
-      const float* other = red + w * N * 64 + lane;
-#pragma unroll
-      for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          dk[d][r] += other[(d * 32 + r) * 64];
-          dv[d][r] += other[(d * 32 + 16 + r) * 64];
-        }
-    }
-  }
-
-  if constexpr (SINK) {
-    float* row = p.part + ((((long)bh * p.chunks + share) * p.sinks + j) * 2) * p.D;
-    store_owner<float, DP>(row, dk, 1.f, j < p.sinks, p.D, at.lhi);
-    store_owner<float, DP>(row + p.D, dv, 1.f, j < p.sinks, p.D, at.lhi);
-  } else if constexpr (MODE == SPLIT) {
-    float* row = p.split + ((((long)share * p.B * p.Hk + bh) * p.T + j) * 2) * p.D;
-    store_owner<float, DP>(row, dk, 1.f, live, p.D, at.lhi);
-    store_owner<float, DP>(row + p.D, dv, 1.f, live, p.D, at.lhi);
-  } else {
-    if (!live) {
-#pragma unroll
-      for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-    }
-    if (p.chunks > 0 && j < p.sinks && live) {   // add what the sink kernel gathered
-      const float* row = p.part + ((long)bh * p.chunks * p.sinks + j) * 2 * p.D;
-#pragma unroll
-      for (int d = 0; d < G::DB; ++d)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const int dd = 32 * d + 8 * a + 4 * at.lhi;
-          if (dd < p.D) {
-            const f32x4 u = *(const f32x4*)(row + dd), w = *(const f32x4*)(row + p.D + dd);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              dk[d][4 * a + e] += u[e];
-              dv[d][4 * a + e] += w[e];
-            }
+            for (int e = 0; e < 4; ++e) v[4 * h + e] += more[e];
           }
         }
+      }
+      if (ends && !live) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      }
+      store_half<T>((T*)(first ? p.dk : p.dv) + (((long)b * p.T + j) * p.Hk + hk) * p.D, v, first ? p.scale : 1.f, j < p.T, d0, p.D, at.lhi);
     }
-    const long orow = (((long)b * p.T + j) * p.Hk + hk) * p.D;
-    store_owner<T, DP>((T*)p.dk + orow, dk, p.scale, j < p.T, p.D, at.lhi);
-    store_owner<T, DP>((T*)p.dv + orow, dv, 1.f, j < p.T, p.D, at.lhi);
+  };
+  if constexpr (SHARE) {
+    const Join<WV, 8 * G::DB> join = {(float*)smem_all, lane};
+    __syncthreads();
+    join.leave(dk, wave, 0);
+    join.leave(dv, wave, 4 * G::DB);
+    __syncthreads();
+    float f[WV];
+#pragma unroll
+    for (int w = 0; w < WV; ++w) f[w] = 1.f;
+#pragma unroll
+    for (int u = wave; u < 4 * G::DB; u += WV) {
+      float v[8];
+      join.half(u, f, v);
+      emit(u, v);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4 * G::DB; ++u) {
+      float v[8];
+      if (u < 2 * G::DB) half_of(dk, u, v);
+      else half_of(dv, u - 2 * G::DB, v);
+      emit(u, v);
+    }
   }
 }
 
@@ -840,11 +857,11 @@ struct Plan {
   int chunks, splits;   // workgroups that share a sink block's queries (0: the sinks reach nothing), and a key block's
   bool share;           // a key block's wavefronts share 32 keys
 };
-inline Plan plan_keys(int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
+inline Plan plan_keys(int tile, int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
   Plan r = {0, 1, false};
   // do the sinks reach queries outside of the window?
   if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
-    const long rows = (long)B * Hk * cdiv(sinks, 32), tiles = (long)(H / Hk) * cdiv(T, 64);
+    const long rows = (long)B * Hk * cdiv(sinks, 32), tiles = (long)(H / Hk) * cdiv(T, tile);
     long c = 256 / rows;                    // one workgroup a compute unit, each of its wavefronts a tile at least
     if (c > (tiles + 3) / 4) c = (tiles + 3) / 4;
     r.chunks = (int)(c < 1 ? 1 : c);
@@ -925,7 +942,7 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
       (((uintptr_t)o | (uintptr_t)olo | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
   p.o = o; p.olo = const_cast<void*>(olo); p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = ws;
-  const Plan plan = plan_keys(p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
+  const Plan plan = plan_keys(Geo<T, 32>::BN, p.B, p.T, p.H, p.Hk, p.left, p.right, p.sinks, p.causal);
   p.chunks = plan.chunks;
   p.splits = plan.splits;
   p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
@@ -952,7 +969,7 @@ INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, co
 INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
   sinks = sinks < T ? sinks : T;
-  const Plan plan = plan_keys(B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal != 0);
+  const Plan plan = plan_keys(32, B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal != 0);
   return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * plan.chunks * sinks * 2 * D +
          (plan.splits > 1 ? (long)plan.splits * B * Hk * T * 2 * D : 0);
 }
