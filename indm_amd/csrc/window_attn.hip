@@ -44,10 +44,10 @@ struct WAttnArgs {
   void *out, *dq, *dk, *dv;         // dense
   float* lse;                       // [B, H, T]: log2 of the sum of exponentials, in units of the exp2 argument
   float* delta;                     // [B, H, T]: <dO, o>
-  float* part;                      // sink partials [B Hk][chunks][sinks][2][D]
+  float* part;                      // sink partials [B Hk][chunks, without splits + 1][sinks][2][D]
   float* split;                     // partial dk, dv [splits][B Hk][T][2][D]
   const int* lengths;               // [B] or NULL
-  int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks, splits;
+  int B, T, H, Hk, D, left, right, sinks, causal, tiles, chunks, splits, sunk;
   float c, scale;                   // scale * log2(e), scale
 };
 
@@ -312,7 +312,9 @@ struct Join {
   }
 };
 
-// workgroup -> work item, so that neighbouring items (which share most of their tiles) run on one XCD's L2
+// workgroup -> work item, so that neighbouring items (which share most of their tiles) run on one XCD's L2.  (Items run over a head's
+// blocks, then the sequences, then the heads: every XCD gets all sequences, whatever their lengths.  Five sequences, one of them empty,
+// 1543 x 8 heads of 128: forward 43 -> 39 us, dk / dv 96 -> 82 us against all heads of a sequence together.)
 __device__ __forceinline__ int xcd_item(int id, int total) {
   const int x = id & 7, per = total >> 3, rem = total & 7;
   return x * per + (x < rem ? x : rem) + (id >> 3);
@@ -357,7 +359,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<T, DP> at(lane);
   const int item = xcd_item(blockIdx.x, gridDim.x);
-  const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.H, b = bh / p.H;
+  const int tile = item % p.tiles, bh = item / p.tiles, h = bh / p.B, b = bh % p.B;
   const int n = seq_len(p, b);
   char* smem = smem_all + (SHARE ? wave * 4 * G::TILE : 0);
   const int q0 = tile * OWN, qw = q0 + (SHARE ? 0 : wave * 32), i = qw + at.l31;
@@ -564,24 +566,26 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
 }
 
 // ---------------------------------------------------------------------------------------------- owner = keys: dk, dv
-// The queries of every head of the group stream past the key.  WHOLE: the window's part of all keys.  SPLIT: the same where there are
-// few key blocks, their queries shared by p.splits workgroups that leave fp32 partial sums.  SINK: what the sink keys get from queries
-// whose window they are outside of -- a few keys against all queries, shared by p.chunks workgroups.  Partial sums are added up in
-// order (no atomics).
-enum { WHOLE = 0, SPLIT = 1, SINKS = 2 };
-template <typename T, int DP, int WV, bool SHARE, int MODE>
+// The queries of every head of the group stream past the key.  There are two kinds of workgroups: the last p.sunk ones gather what the
+// sink keys get from queries whose window they are outside of -- a few keys against all queries, shared by p.chunks workgroups a block of
+// them --, the others the window's part of all keys (SPLIT: where there are few key blocks, each one's queries shared by p.splits
+// workgroups).  What several workgroups contribute to goes to fp32 partial sums that a last kernel adds up in order (no atomics).
+// (WHO spares the launches of one kind the other's tests: 62 instead of 67 us.)
+enum { KEYS = 1, SINKS = 2, BOTH = 3 };
+template <typename T, int DP, int WV, bool SHARE, bool SPLIT, int WHO>
 __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) void wattn_key_kernel(WAttnArgs p) {
   using G = Geo<T, DP>;
   using O = Op<T>;
   typedef typename O::frag frag;
-  constexpr bool SINK = MODE == SINKS;
   constexpr int OWN = SHARE ? 32 : WV * 32, STEP = SHARE ? WV : 1, BUF = 2 * G::TILE + 2 * G::BN * (int)sizeof(float);
   extern __shared__ __attribute__((aligned(16))) char smem_all[];   // [2 buffers][Q tile, dO tile, lse, delta], SHARE: for each wavefront
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Lane<T, DP> at(lane);
-  const int item = xcd_item(blockIdx.x, gridDim.x);
-  const int shares = SINK ? p.chunks : MODE == SPLIT ? p.splits : 1, per = p.tiles * shares;
-  const int bh = item / per, hk = bh % p.Hk, b = bh / p.Hk;
+  const int blocks = gridDim.x - p.sunk;
+  const bool sink = WHO == SINKS || (WHO == BOTH && (int)blockIdx.x >= blocks);
+  const int item = sink ? xcd_item(blockIdx.x - blocks, p.sunk) : xcd_item(blockIdx.x, blocks);
+  const int shares = sink ? p.chunks : SPLIT ? p.splits : 1, per = (sink ? (p.sinks + OWN - 1) / OWN : p.tiles) * shares;
+  const int hk = item / per / p.B, b = item / per % p.B, bh = b * p.Hk + hk;
   const int share = item % per % shares, tile = item % per / shares;
   const int n = seq_len(p, b), group = p.H / p.Hk;
   char* smem = smem_all + (SHARE ? wave * 2 * BUF : 0);
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
   const bool live = j < n;
   // tiles of queries: i0 .. i1 of each head of the group, one after the other, of which this workgroup takes its share
   int i0, i1;
-  if constexpr (SINK) {
+  if (sink) {
     i0 = p.causal ? j0 : 0;
     i1 = n - 1;
   } else {
@@ -629,7 +633,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
   load_owner<T, DP>((const T*)p.v + b * p.vb + (long)j * p.vt + hk * p.vh, live, p.D, at.lhi, vf);
   // the lane's queries.  window: lo .. hi.  sinks: up to last, outside of lo .. hi
   int lo = p.causal ? j : j - p.right, hi = j + p.left, last = n - 1;
-  if constexpr (SINK) {
+  if (sink) {
     if (p.causal) lo = -(1 << 30);
     if (j >= p.sinks || !live) last = -1;
   } else {
@@ -661,7 +665,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
     for (int y = 0; y < G::NY; ++y) {
       const int ia = first + 32 * y, ib = ia + 31;   // (wave-uniform tests, as in the other kernel)
       bool any, all;
-      if constexpr (SINK) {
+      if (sink) {
         any = jw < p.sinks && jw < n && ia < n && (ib > jw + p.left || (!p.causal && ia < jw + 31 - p.right));
         all = false;
       } else {
@@ -683,11 +687,13 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
       if (!all) {
         asm volatile("" ::: "memory");   // (keeps the masks behind the branch)
         const unsigned at0 = (unsigned)(ia + 4 * at.lhi - lo);
+        if (sink) {
+          const int room = last - ia - 4 * at.lhi;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = 8 * (r >> 2) + (r & 3);
-          if constexpr (SINK) P[r] = ia + 4 * at.lhi + i <= last && at0 + i > span ? P[r] : 0.f;
-          else P[r] = at0 + i <= span ? P[r] : 0.f;
+          for (int r = 0; r < 16; ++r) P[r] = 8 * (r >> 2) + (r & 3) <= room && at0 + 8 * (r >> 2) + (r & 3) > span ? P[r] : 0.f;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) P[r] = at0 + 8 * (r >> 2) + (r & 3) <= span ? P[r] : 0.f;
         }
       }
 #pragma unroll
@@ -714,32 +720,24 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
     if (it + STEP < to) put(side ^ 1);
     staged<SHARE>();
   }
+  // a sink's partial sums: the chunks', and without splits one more from the window
+  float* part = p.part + (((long)bh * (p.chunks + (SPLIT ? 0 : 1)) + (sink ? share : p.chunks)) * p.sinks + j) * 2 * p.D;
   const bool sunk = p.chunks > 0 && jw < p.sinks, ends = jw + 31 >= n;   // (wave-uniform)
   auto emit = [&](int u, float (&v)[8]) {   // a half: of dk, then of dv
     const bool first = u < 2 * G::DB;
     const int d0 = 16 * (first ? u : u - 2 * G::DB), at0 = first ? 0 : p.D;
-    if constexpr (SINK) {
-      store_half<float>(p.part + ((((long)bh * p.chunks + share) * p.sinks + j) * 2) * p.D + at0, v, 1.f, j < p.sinks, d0, p.D, at.lhi);
-    } else if constexpr (MODE == SPLIT) {
+    if (sink) {
+      store_half<float>(part + at0, v, 1.f, j < p.sinks, d0, p.D, at.lhi);
+    } else if constexpr (SPLIT) {
       store_half<float>(p.split + ((((long)share * p.B * p.Hk + bh) * p.T + j) * 2) * p.D + at0, v, 1.f, live, d0, p.D, at.lhi);
     } else {
-      if (sunk) {   // add what the sink kernel gathered
-        const float* gathered = p.part + ((long)bh * p.chunks * p.sinks + j) * 2 * p.D + at0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int d = d0 + 8 * h + 4 * at.lhi;
-          if (d < p.D && j < p.sinks) {
-            const f32x4 more = *(const f32x4*)(gathered + d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * h + e] += more[e];
-          }
-        }
-      }
       if (ends && !live) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
       }
-      store_half<T>((T*)(first ? p.dk : p.dv) + (((long)b * p.T + j) * p.Hk + hk) * p.D, v, first ? p.scale : 1.f, j < p.T, d0, p.D, at.lhi);
+      if (sunk) store_half<float>(part + at0, v, 1.f, j < p.sinks, d0, p.D, at.lhi);
+      store_half<T>((T*)(first ? p.dk : p.dv) + (((long)b * p.T + j) * p.Hk + hk) * p.D, v, first ? p.scale : 1.f,
+                    j < p.T && !(sunk && j < p.sinks), d0, p.D, at.lhi);
     }
   };
   if constexpr (SHARE) {
@@ -768,20 +766,36 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
   }
 }
 
-// the sink partials of each (sequence, key head) added up over the chunks, in order, into chunk 0: a workgroup's lanes own 64 of the
-// n = sinks x 2 D values, its wavefronts a quarter of the chunks each
-__global__ __launch_bounds__(256) void wattn_join_kernel(float* part, int chunks, int n) {
-  __shared__ float sh[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-  float* base = part + (long)blockIdx.y * chunks * n + col;
-  float s = 0.f;
-  if (col < n) {
+// dk, dv of the sinks: their partial sums in order (without splits).  A workgroup's lanes own 64 of the n = sinks x 2 D values of a
+// (sequence, key head), its wavefronts a sixteenth of the partial sums each.
+template <typename T>
+__global__ __launch_bounds__(1024) void wattn_sinks_kernel(WAttnArgs p) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slots = p.chunks + 1;
+  const long n = (long)p.sinks * 2 * p.D, cols = (n + 63) / 64, groups = (long)p.B * p.Hk * cols;
+  for (long g = blockIdx.x; g < groups; g += gridDim.x) {
+    const long bh = g / cols, col = (g - bh * cols) * 64 + lane;
+    const float* src = p.part + bh * slots * n + col;
+    float s = 0.f;
+    if (col < n) {
 #pragma unroll 4
-    for (int c = chunks * wave / 4; c < chunks * (wave + 1) / 4; ++c) s += base[(long)c * n];
+      for (int c = slots * wave / 16; c < slots * (wave + 1) / 16; ++c) s += src[c * n];
+    }
+    sh[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < n) {
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) s += sh[w][lane];
+      const long jw = col / p.D, j = jw >> 1, b = bh / p.Hk, hk = bh - b * p.Hk;
+      if (j >= seq_len(p, (int)b)) s = 0.f;
+      T* out = (T*)(jw & 1 ? p.dv : p.dk) + ((b * p.T + j) * p.Hk + hk) * p.D + (col - jw * p.D);
+      if (!(jw & 1)) s *= p.scale;
+      if constexpr (sizeof(T) == 2) *out = __builtin_bit_cast(u16, (__bf16)s);
+      else *out = s;
+    }
+    __syncthreads();
   }
-  sh[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && col < n) base[0] = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
 }
 
 // dk, dv = the splits' partial sums, in order, and the sinks' -- four elements a thread
@@ -799,7 +813,11 @@ __global__ __launch_bounds__(256) void wattn_sum_kernel(WAttnArgs p) {
     if (j < seq_len(p, (int)b)) {
       const float* src = p.split + (((b * p.Hk + hk) * p.T + j) * 2 + which) * p.D + d;
       for (int c = 0; c < p.splits; ++c) s += *(const f32x4*)(src + (long)c * p.B * p.Hk * p.T * 2 * p.D);
-      if (p.chunks > 0 && j < p.sinks) s += *(const f32x4*)(p.part + (((b * p.Hk + hk) * p.chunks * p.sinks + j) * 2 + which) * p.D + d);
+      if (j < p.sinks) {
+        const float* part = p.part + (((b * p.Hk + hk) * p.chunks * p.sinks + j) * 2 + which) * p.D + d;
+#pragma unroll 4
+        for (int c = 0; c < p.chunks; ++c) s += *(const f32x4*)(part + (long)c * p.sinks * 2 * p.D);
+      }
       if (which == 0) s *= p.scale;
     }
     T* out = (T*)(which == 0 ? p.dk : p.dv) + k * p.D + d;
@@ -829,18 +847,22 @@ int run_query(WAttnArgs p, hipStream_t st) {
   return launch<wattn_query_kernel<T, DP, WV, SHARE, BWD>>(p, (long)p.tiles * p.H * p.B, WV * 64,
                                                            (SHARE ? WV : 1) * 4 * (size_t)Geo<T, DP>::TILE, st);
 }
-template <typename T, int DP, bool SHARE, int MODE>
+// the window's part of all keys, the sinks' from all queries, or both
+template <typename T, int DP, bool SHARE, bool SPLIT, int WHO>
 int run_key(WAttnArgs p, hipStream_t st) {
   using G = Geo<T, DP>;
-  constexpr int WV = SHARE ? share_waves<T, DP>() : 4;
-  p.tiles = cdiv(MODE == SINKS ? p.sinks : p.T, SHARE ? 32 : WV * 32);
-  return launch<wattn_key_kernel<T, DP, WV, SHARE, MODE>>(
-      p, (long)p.tiles * (MODE == SINKS ? p.chunks : MODE == SPLIT ? p.splits : 1) * p.Hk * p.B, WV * 64,
-      (SHARE ? WV : 1) * 2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
+  constexpr int WV = SHARE ? share_waves<T, DP>() : 4, OWN = SHARE ? 32 : WV * 32;
+  p.tiles = cdiv(p.T, OWN);
+  const long heads = (long)p.Hk * p.B, sunk = WHO & SINKS ? cdiv(p.sinks, OWN) * p.chunks * heads : 0;
+  if (sunk > 0x7fffffffL) return INDM_E_SHAPE;
+  p.sunk = (int)sunk;
+  return launch<wattn_key_kernel<T, DP, WV, SHARE, SPLIT, WHO>>(p, sunk + (WHO & KEYS ? (long)p.tiles * (SPLIT ? p.splits : 1) * heads : 0), WV * 64,
+                                                                (SHARE ? WV : 1) * 2 * (2 * (size_t)G::TILE + 2 * G::BN * sizeof(float)), st);
 }
-inline int run_join(const WAttnArgs& p, hipStream_t st) {
-  const int n = p.sinks * 2 * p.D;   // (several chunks only for up to 128 sink blocks of all heads: few rows of few values)
-  hipLaunchKernelGGL(wattn_join_kernel, dim3(cdiv(n, 64), p.B * p.Hk), dim3(256), 0, st, p.part, p.chunks, n);
+template <typename T>
+int run_sinks(const WAttnArgs& p, hipStream_t st) {
+  const long groups = (long)p.B * p.Hk * (((long)p.sinks * 2 * p.D + 63) / 64);
+  hipLaunchKernelGGL(wattn_sinks_kernel<T>, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20)), dim3(1024), 0, st, p);
   return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
 }
 template <typename T>
@@ -856,27 +878,37 @@ constexpr long SHARE_BELOW = 128;
 struct Plan {
   int chunks, splits;   // workgroups that share a sink block's queries (0: the sinks reach nothing), and a key block's
   bool share;           // a key block's wavefronts share 32 keys
+  bool apart;           // the sinks' workgroups are a launch of their own (and share 32 keys)
 };
 inline Plan plan_keys(int tile, int B, int T, int H, int Hk, int left, int right, int sinks, int causal) {
-  Plan r = {0, 1, false};
-  // do the sinks reach queries outside of the window?
-  if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
-    const long rows = (long)B * Hk * cdiv(sinks, 32), tiles = (long)(H / Hk) * cdiv(T, tile);
-    long c = 256 / rows;                    // one workgroup a compute unit, each of its wavefronts a tile at least
-    if (c > (tiles + 3) / 4) c = (tiles + 3) / 4;
-    r.chunks = (int)(c < 1 ? 1 : c);
-  }
-  // few key blocks: share each one's queries among workgroups, as long as that leaves each about four tiles (of all heads of the group)
-  const long blocks = (long)cdiv(T, 128) * Hk * B;
+  Plan r = {0, 1, false, false};
+  // few key blocks: share each one's queries among workgroups, as long as that leaves each about four tiles of 64 (of all heads of the group)
+  const long blocks = (long)cdiv(T, 128) * Hk * B, group = H / Hk;
+  const long reach = (long)(left < T ? left : T) + (causal ? 0 : (right < T ? right : T)) + 128, span = reach < T ? reach : T;
   if (blocks < 384) {
-    const long reach = (long)(left < T ? left : T) + (causal ? 0 : (right < T ? right : T)) + 128;
-    const long tiles = (long)(H / Hk) * cdiv(reach < T ? reach : T, 64);
+    const long tiles = group * cdiv(span, 64);
     long s = (512 + blocks - 1) / blocks;
     if (s > tiles / 4) s = tiles / 4;
     r.splits = s < 1 ? 1 : (int)s;
     r.share = blocks * r.splits <= SHARE_BELOW;
   }
+  // Do the sinks reach queries outside of the window?  Then all queries of a block of them are shared by so many workgroups that a
+  // wavefront which streams by itself has one tile and a workgroup that streams together eight, up to one or two a compute unit (16 MB
+  // of partial sums at most).  Where the key blocks leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens,
+  // 8 heads of 128 on 2: 97 us together, 113 apart; 2 x 1021 fp32 tokens, 4 heads of 40: 29 us, 31); where they fill it, it is a launch
+  // before (8 x 4096 tokens, 4 heads of 64: 80 us apart, 89 together).
+  if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
+    r.apart = r.splits == 1 && !r.share;
+    const bool alone = r.share || r.apart;
+    const long rows = (long)B * Hk * cdiv(sinks, alone ? 32 : 128), tiles = group * cdiv(T, tile), mine = alone ? 4 : 8, most = alone ? 256 : 512;
+    long c = (tiles + mine - 1) / mine;
+    if (c > most / rows) c = most / rows;
+    r.chunks = (int)(c < 1 ? 1 : c);
+  }
   return r;
+}
+inline long part_floats(const Plan& plan, int B, int Hk, int sinks, int D) {
+  return plan.chunks == 0 ? 0 : (long)B * Hk * (plan.chunks + (plan.splits > 1 ? 0 : 1)) * sinks * 2 * D;
 }
 inline bool share_queries(int B, int T, int H) { return (long)cdiv(T, 128) * H * B <= SHARE_BELOW; }
 
@@ -923,14 +955,15 @@ int fwd(WAttnArgs p, const long* strides, void* o, void* olo, float* lse, hipStr
 }
 
 template <typename T, int DP>
-int bwd_dp(const WAttnArgs& p, bool share, hipStream_t st) {
+int bwd_dp(const WAttnArgs& p, const Plan& plan, hipStream_t st) {
   int r = share_queries(p.B, p.T, p.H) ? run_query<T, DP, true, true>(p, st) : run_query<T, DP, false, true>(p, st);   // dq; delta for the others
-  if (r == INDM_OK && p.chunks > 0) r = run_key<T, DP, true, SINKS>(p, st);
-  if (r == INDM_OK && p.chunks > 1) r = run_join(p, st);
+  const bool sinks = p.chunks > 0;
+  if (r == INDM_OK && sinks && plan.apart) r = run_key<T, DP, true, false, SINKS>(p, st);
   if (r == INDM_OK)
-    r = p.splits > 1 ? (share ? run_key<T, DP, true, SPLIT>(p, st) : run_key<T, DP, false, SPLIT>(p, st))
-                     : (share ? run_key<T, DP, true, WHOLE>(p, st) : run_key<T, DP, false, WHOLE>(p, st));
+    r = p.splits > 1 ? (plan.share ? run_key<T, DP, true, true, BOTH>(p, st) : run_key<T, DP, false, true, BOTH>(p, st))
+                     : (plan.share ? run_key<T, DP, true, false, BOTH>(p, st) : run_key<T, DP, false, false, KEYS>(p, st));
   if (r == INDM_OK && p.splits > 1) r = run_sum<T>(p, st);
+  else if (r == INDM_OK && sinks) r = run_sinks<T>(p, st);
   return r;
 }
 template <typename T>
@@ -946,8 +979,8 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
   p.chunks = plan.chunks;
   p.splits = plan.splits;
   p.part = ws + ((long)p.B * p.H * p.T + 3) / 4 * 4;
-  p.split = p.part + (long)p.B * p.Hk * p.chunks * p.sinks * 2 * p.D;
-#define WA_BWD(DP) bwd_dp<T, DP>(p, plan.share, st)
+  p.split = p.part + part_floats(plan, p.B, p.Hk, p.sinks, p.D);
+#define WA_BWD(DP) bwd_dp<T, DP>(p, plan, st)
   WA_DISPATCH(WA_BWD)
 }
 
@@ -969,9 +1002,15 @@ INDM_API int indm_wattn_fwd_bf16(const void* q, const void* k, const void* v, co
 INDM_API long indm_wattn_bwd_ws_floats(int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
   sinks = sinks < T ? sinks : T;
-  const Plan plan = plan_keys(32, B, T, H, Hk, left < T ? left : T, right < T ? right : T, sinks, causal != 0);
-  return ((long)B * H * T + 3) / 4 * 4 + (long)B * Hk * plan.chunks * sinks * 2 * D +
-         (plan.splits > 1 ? (long)plan.splits * B * Hk * T * 2 * D : 0);
+  left = left < T ? left : T;
+  right = right < T ? right : T;
+  long most = 0;
+  for (int tile = 32; tile <= 64; tile *= 2) {   // (whichever type needs more)
+    const Plan plan = plan_keys(tile, B, T, H, Hk, left, right, sinks, causal != 0);
+    const long n = part_floats(plan, B, Hk, sinks, D) + (plan.splits > 1 ? (long)plan.splits * B * Hk * T * 2 * D : 0);
+    most = n > most ? n : most;
+  }
+  return ((long)B * H * T + 3) / 4 * 4 + most;
 }
 INDM_API int indm_wattn_bwd_f32(const float* q, const float* k, const float* v, const long* strides, const float* o, const void*,
                                 const float* dO, const float* lse, const int* lengths, float* dq, float* dk, float* dv, float* ws, int B, int T, int H,

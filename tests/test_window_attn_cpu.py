@@ -73,4 +73,4 @@ def test_c_entry_points_refuse_and_ignore_empty_work():
     assert ws(1, 0, 2, 1, 16, 1, 1, 0, 0) == 0 and ws(1, 4, 3, 2, 16, 1, 1, 0, 0) == 0
     assert ws(2, 5, 4, 2, 16, 1, 1, 0, 0) == 40                  # <dO, o> of every query
     assert ws(2, 5, 4, 2, 16, 5, 5, 3, 0) == 40                  # windows that see everything: the sinks add nothing
-    assert ws(1, 64, 1, 1, 16, 5, 5, 3, 0) == 64 + 3 * 2 * 16    # one tile of queries: one share of the three sinks' dk, dv
+    assert ws(1, 64, 1, 1, 16, 5, 5, 3, 0) == 64 + 2 * 3 * 2 * 16    # the three sinks' dk, dv: one share from all queries, one from the window

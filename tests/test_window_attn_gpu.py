@@ -138,6 +138,21 @@ def test_sizes_and_windows(guards, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,T,H,Hk,D,left,right,sinks", [
+    (40, 300, 4, 4, 32, 30, 20, 5),       # key blocks that fill the chip: the sinks' queries in a launch of their own
+    (40, 300, 4, 4, 32, 3, 2, 200),       # the same with several blocks of sinks
+    (5, 600, 8, 2, 64, 300, 100, 16),     # key blocks whose queries are split, the sinks' workgroups behind them
+    (5, 600, 8, 2, 64, 300, 100, 290)])
+def test_workgroup_layouts(guards, dtype, causal, B, T, H, Hk, D, left, right, sinks):
+    """the backward pass' layouts that small cases do not reach, with sequences that end among the sinks and an empty one"""
+    q, k, v, do = (randn((B, T, h, D), 130 + i, dtype) for i, h in enumerate((H, Hk, Hk, H)))
+    lengths = torch.tensor([T, 0, sinks // 2, T - 1, 129] * (B // 5), dtype=torch.int32, device=DEV)
+    check(q, k, v, do, left, right, sinks, causal, lengths)
+    assert guards.broken_guards() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [8, 16, 32, 48, 64, 80, 96, 112, 120, 128])
 def test_head_widths(guards, dtype, D):
     q, k, v, do = (randn((1, 150, h, D), 10 + i, dtype) for i, h in enumerate((2, 1, 1, 2)))
