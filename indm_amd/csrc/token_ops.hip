@@ -111,6 +111,9 @@ __device__ __forceinline__ void load_param(const float* p, int n, float fill, fl
 // ------------------------------------------------------------------------------------------------ layer norm
 // A team of L lanes owns a row and keeps it in registers (NV vectors a lane), so the statistics are the two-pass ones -- the
 // mean, then the sum of squared differences from it -- and x is read from HBM once.  L < 64: several rows a wavefront.
+// HBM-bound.  131072 rows of 256, bf16: forward 24 us (5.6 TB/s, a copy's rate), backward 39 us (5.1 TB/s) and 4 us for the parameters'
+// sums; 4099 rows of 1153, fp32, out of wider rows: 10 us, 16.5 us and 4 us; 256 rows: 2.7 us, a launch.  Rows that start on odd bf16
+// elements cost the backward pass half its rate (2.4 TB/s: the memory pipe splits those accesses).
 // Sum over the team; every lane gets the same bits (each step adds a pair, whichever order).  Within a wavefront all steps are
 // vector instructions: lanes 1, 2, then mirrored quads and halves of a row of 16, then rows and halves of the wavefront traded.
 template <int CTRL>
