@@ -16,8 +16,9 @@
 //                                          <-> y = 8 (t >> 2) + 4 lhi + (t & 3)); A is read transposed out of the same tile
 //                                          (ds_read_b64_tr_b16 on bf16), and out keeps the owner in the lane: rescaling is in-lane
 // On fp32 the same operands are 8 values a lane and a product is 8 v_mfma_f32_32x32x2_f32 (their k order differs from the bf16
-// instruction's, the same way on both sides).  P and dS are rounded to bf16 as operands of the second product on bf16 tensors: each
-// term is then off by half a step like the result itself, and the terms' errors average out in the sum.
+// instruction's, the same way on both sides).  P and dS enter the second product on bf16 tensors as two operands, their rounding and what
+// it left: o and every gradient then have the error of one rounding, 1.66e-3 of their norm (with one operand the gradients had 2.4e-3; the
+// rest's products cost dq 58 -> 68 us and dk / dv 66 -> 85 us in the first case below).
 // The softmax is exp2 with a running maximum that is raised only when a new logit exceeds it by 8 (P <= 256 then: no digit is lost,
 // and the accumulators are rescaled once or twice a row instead of once a tile).
 //
@@ -78,10 +79,12 @@ struct Geo {
 };
 
 // wavefronts a SIMD that the register allocation aims at (kind 0: forward, 1: dq, 2: dk / dv): 512 registers a SIMD lane over 4, 3, 2 or
-// 1, what fits without spilling.  Workgroups that share an owner block fill a compute unit's LDS: one wavefront a SIMD.
+// 1, so that nothing in a loop spills (the compiler reports 12 bytes of scratch for the forward kernel of bf16 heads of 49 to 64, none for any
+// other).  bf16 dk / dv of heads of more than 96: 85 to 93 registers spill at two wavefronts (8 x 4096 tokens, 4 heads of 128: 267 us, at one
+// 195 us).  Workgroups that share an owner block fill a compute unit's LDS: one wavefront a SIMD.
 constexpr int waves_per_simd(int size, int DP, int kind, bool share) {
   if (share) return 1;
-  if (size == 2) return DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : 2;
+  if (size == 2) return DP <= 64 ? (kind == 0 ? 4 : kind == 1 ? 3 : 2) : DP > 96 && kind == 2 ? 1 : 2;
   return DP <= 32 ? 3 : DP <= 64 ? (kind == 0 ? 3 : 2) : DP <= 96 && kind == 0 ? 2 : 1;
 }
 // wavefronts of a workgroup that shares an owner block: each streams tiles of its own, 128 KB of LDS together
@@ -205,6 +208,27 @@ struct Lane {
     }
   }
 };
+
+// out^T += Z^T W of 32 streamed tokens (rows row0 .. of the tile).  On bf16 W goes in as two operands, its rounding and what that left: W
+// then is off by 2^-16 of itself, and the result by its own rounding alone.
+template <typename T, int DP>
+__device__ __forceinline__ void gather(const Lane<T, DP>& at, const char* tile, int row0, const f32x16& W, f32x16 (&out)[Geo<T, DP>::DB]) {
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const Frag<T> w = Op<T>::pack(W, 8 * a);
+    if constexpr (sizeof(T) == 2) {
+      const Frag<T> rest = Op<T>::pack_rest(W, w, 8 * a);
+#pragma unroll
+      for (int d = 0; d < Geo<T, DP>::DB; ++d) {
+        const Frag<T> z = at.transposed(tile, row0 + 16 * a, d);
+        out[d] = Op<T>::mma(z, rest, Op<T>::mma(z, w, out[d]));
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < Geo<T, DP>::DB; ++d) out[d] = Op<T>::mma(at.transposed(tile, row0 + 16 * a, d), w, out[d]);
+    }
+  }
+}
 
 // rows first .. first + BN - 1 of a head -> a tile in LDS, by direct copies of 16 bytes a lane (1 KB a wave-instruction, the swizzle is
 // on the source side).  A whole tile of whole rows needs no vector arithmetic in the loop: a scalar base plus the lane's byte offsets,
@@ -491,22 +515,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
         for (int r = 0; r < 16; ++r)
           S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, -lse)) * (dP[r] - delta);   // dS / scale
       }
-      const char* zb = BWD ? kb : vb;
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const frag w = O::pack(S, 8 * a);
-        if constexpr (!BWD && sizeof(T) == 2) {
-          const frag rest = O::pack_rest(S, w, 8 * a);
-#pragma unroll
-          for (int d = 0; d < G::DB; ++d) {
-            const frag z = at.transposed(zb, 32 * y + 16 * a, d);
-            acc[d] = O::mma(z, rest, O::mma(z, w, acc[d]));
-          }
-        } else {
-#pragma unroll
-          for (int d = 0; d < G::DB; ++d) acc[d] = O::mma(at.transposed(zb, 32 * y + 16 * a, d), w, acc[d]);
-        }
-      }
+      gather<T, DP>(at, BWD ? kb : vb, 32 * y, S, acc);
     }
     staged<SHARE>();
   }
@@ -703,12 +712,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
           for (int r = 0; r < 16; ++r) P[r] = at0 + 8 * (r >> 2) + (r & 3) <= span ? P[r] : 0.f;
         }
       }
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const frag w = O::pack(P, 8 * a);
-#pragma unroll
-        for (int d = 0; d < G::DB; ++d) dv[d] = O::mma(at.transposed(db, 32 * y + 16 * a, d), w, dv[d]);
-      }
+      gather<T, DP>(at, db, 32 * y, P, dv);
 #pragma unroll
       for (int kk = 0; kk < G::KK; ++kk) dP = O::mma(at.rowwise(db, y, kk), vf[kk], dP);
 #pragma unroll
@@ -717,12 +721,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) v
 #pragma unroll
         for (int e = 0; e < 4; ++e) P[4 * a + e] *= dP[4 * a + e] - d4[e];
       }
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const frag w = O::pack(P, 8 * a);
-#pragma unroll
-        for (int d = 0; d < G::DB; ++d) dk[d] = O::mma(at.transposed(qb, 32 * y + 16 * a, d), w, dk[d]);
-      }
+      gather<T, DP>(at, qb, 32 * y, P, dk);
     }
     if (it + STEP < to) put(side ^ 1);
     staged<SHARE>();
