@@ -7,6 +7,7 @@
 // loaded library (indm_amd/hip.py), nothing is linked.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
@@ -66,6 +67,13 @@ bool tracked(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// What these functions cannot carry through is refused, not dropped: the tangent of a forward-mode derivative (a dual tensor need not
+// require grad), and the call itself under torch.jit.trace, which would record an allocation in its place.
+void carries(const char* op, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined()) REFUSE(op, ": forward-mode derivatives are not computed");
+  if (torch::jit::tracer::isTracing()) REFUSE(op, ": cannot be traced by torch.jit.trace");
 }
 // which entry point: 0 float32, 1 bfloat16
 int type_of(const char* op, const Tensor& x) {
@@ -213,6 +221,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 Tensor layer_norm(const Tensor& x, const Maybe& gamma_, const Maybe& beta_, double eps) {
   const Tensor gamma = plain(gamma_), beta = plain(beta_);
+  carries("layer_norm", {&x, &gamma, &beta});
   layer_norm_check(x, gamma, beta, eps);
   return tracked({&x, &gamma, &beta}) ? LayerNorm::apply(x, gamma_, beta_, eps) : layer_norm_run(x, gamma, beta, eps, false).first;
 }
@@ -248,6 +257,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& res_, const Maybe& seed_dev_) {
   const Tensor res = plain(res_), seed_dev = plain(seed_dev_);
+  carries("dropout", {&x, &res});
   type_of("dropout", x);
   if (!(p >= 0. && p <= 1.)) REFUSE("dropout: 0 <= p <= 1, got ", p);
   if (res.defined() && (res.sizes() != x.sizes() || res.scalar_type() != x.scalar_type()))
@@ -331,6 +341,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k_, const Tensor& pos, const Tensor& freqs, const std::vector<int64_t>& sections,
                                 bool interleaved) {
   const Tensor k = plain(k_);
+  carries("rotary", {&q, &k, &pos, &freqs});
   rotary_check(q, k, pos, freqs, sections);
   Tensor yq, yk;
   if (tracked({&q, &k})) {
@@ -438,6 +449,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
                         double scale) {
   const Tensor lengths = plain(lengths_);
   const Window w = {left, right, sinks, causal, scale};
+  carries("window_attention", {&q, &k, &v});
   window_check(q, k, v, w, lengths);
   return tracked({&q, &k, &v}) ? WindowAttention::apply(q, k, v, left, right, sinks, causal, lengths_, scale) : window_run(q, k, v, w, lengths, false).o;
 }

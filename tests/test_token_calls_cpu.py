@@ -1,0 +1,39 @@
+"""Ways of calling the token operators that they refuse rather than answer wrongly, whatever device the tensors are on."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from indm_amd import ops
+
+X, G, POS, FREQS = torch.ones(2, 3, 2, 8), torch.ones(8), torch.zeros(3, 1), ops.rotary_freqs((8,))
+CALLS = {
+    "layer_norm": (lambda x: ops.layer_norm(x), X),
+    "layer_norm gamma": (lambda g: ops.layer_norm(X, g), G),
+    "layer_norm beta": (lambda b: ops.layer_norm(X, None, b), G),
+    "dropout": (lambda x: ops.dropout(x, 0.5, 1), X),
+    "dropout res": (lambda r: ops.dropout(X, 0.5, 1, res=r), X),
+    "rotary": (lambda q: ops.rotary(q, None, POS, FREQS, (8,))[0], X),
+    "rotary k": (lambda k: ops.rotary(X, k, POS, FREQS, (8,))[1], X),
+    "rotary pos": (lambda p: ops.rotary(X, None, p, FREQS, (8,))[0], POS),
+    "rotary freqs": (lambda f: ops.rotary(X, None, POS, f, (8,))[0], FREQS),
+    "window_attention q": (lambda q: ops.window_attention(q, X, X, 1), X),
+    "window_attention k": (lambda k: ops.window_attention(X, k, X, 1), X),
+    "window_attention v": (lambda v: ops.window_attention(X, X, v, 1), X),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(name, grad):
+    """a dual tensor does not require grad: its tangent would be lost without a word"""
+    call, x = CALLS[name]
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "rotary", "window_attention q"])
+def test_tracing_is_refused(name):
+    call, x = CALLS[name]
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, (x.clone(),), check_trace=False)
