@@ -61,7 +61,10 @@ void ok(int status, const char* name) {
   TORCH_CHECK(status == 0, name, " failed: ", what);
 }
 bool given(const Maybe& t) { return t.has_value() && t->defined(); }
-Tensor plain(const Maybe& t) { return given(t) ? *t : Tensor(); }
+// The tensor with the values it stands for in memory: a view may be lazily negated (the imaginary part of a conjugate), and a tensor of
+// zeros that autograd made may have no memory at all.  Differentiable.
+Tensor whole(const Tensor& t) { return t.defined() && (t.is_neg() || t._is_zerotensor()) ? t.clone() : t; }
+Tensor plain(const Maybe& t) { return given(t) ? whole(*t) : Tensor(); }
 bool tracked(std::initializer_list<const Tensor*> ts) {
   if (!c10::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -208,7 +211,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor &x = saved[0], &stats = saved[2];
     const int64_t want = ctx->saved_data["want"].toInt(), C = x.size(-1);
     const c10::DeviceGuard guard(x.device());
-    const Tensor gamma = dense(saved[1]), dy = grads[0].contiguous();
+    const Tensor gamma = dense(saved[1]), dy = whole(grads[0]).contiguous();
     const Rows r = rows_of(x);
     Tensor dx = dense_like(x), dgamma = want & 2 ? floats(C, x) : Tensor(), dbeta = want & 4 ? floats(C, x) : Tensor(), ws;
     // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
@@ -219,11 +222,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return once({dx, dgamma, dbeta, Tensor()});
   }
 };
-Tensor layer_norm(const Tensor& x, const Maybe& gamma_, const Maybe& beta_, double eps) {
-  const Tensor gamma = plain(gamma_), beta = plain(beta_);
+Tensor layer_norm(const Tensor& x_, const Maybe& gamma_, const Maybe& beta_, double eps) {
+  const Tensor x = whole(x_), gamma = plain(gamma_), beta = plain(beta_);
   carries("layer_norm", {&x, &gamma, &beta});
   layer_norm_check(x, gamma, beta, eps);
-  return tracked({&x, &gamma, &beta}) ? LayerNorm::apply(x, gamma_, beta_, eps) : layer_norm_run(x, gamma, beta, eps, false).first;
+  return tracked({&x, &gamma, &beta}) ? LayerNorm::apply(x, Maybe(gamma), Maybe(beta), eps) : layer_norm_run(x, gamma, beta, eps, false).first;
 }
 
 // ---------------------------------------------------------------------------------------------- dropout
@@ -249,14 +252,14 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const auto at = ctx->saved_data.find("seed_dev");
     Tensor dx;
     if (want & 1)
-      dx = dropout_run(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), Tensor(),
+      dx = dropout_run(whole(grads[0]), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), Tensor(),
                        at == ctx->saved_data.end() ? Tensor() : at->second.toTensor());
     variable_list out = once({dx});
     return {out[0], want & 2 ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
-Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& res_, const Maybe& seed_dev_) {
-  const Tensor res = plain(res_), seed_dev = plain(seed_dev_);
+Tensor dropout(const Tensor& x_, double p, uint64_t seed, const Maybe& res_, const Maybe& seed_dev_) {
+  const Tensor x = whole(x_), res = plain(res_), seed_dev = plain(seed_dev_);
   carries("dropout", {&x, &res});
   type_of("dropout", x);
   if (!(p >= 0. && p <= 1.)) REFUSE("dropout: 0 <= p <= 1, got ", p);
@@ -264,7 +267,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const Maybe& res_, cons
     REFUSE("dropout: res is ", x.sizes(), " ", x.scalar_type(), ", got ", res.sizes(), " ", res.scalar_type());
   if (seed_dev.defined() && (seed_dev.scalar_type() != at::kLong || seed_dev.numel() != 1)) REFUSE("dropout: seed_dev is one int64 on the device");
   on_one_gpu("dropout", {&x, &res, &seed_dev});
-  return tracked({&x, &res}) ? Dropout::apply(x, res_, p, (int64_t)seed, seed_dev_) : dropout_run(x, p, seed, res, seed_dev);
+  return tracked({&x, &res}) ? Dropout::apply(x, Maybe(res), p, (int64_t)seed, Maybe(seed_dev)) : dropout_run(x, p, seed, res, seed_dev);
 }
 
 // ---------------------------------------------------------------------------------------------- rotary positions
@@ -331,21 +334,21 @@ struct Rotary : torch::autograd::Function<Rotary> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const int64_t want = ctx->saved_data["want"].toInt();
-    const Tensor dq = want & 1 ? grads[0] : Tensor(), dk = want & 2 && grads.size() > 1 ? grads[1] : Tensor();
+    const Tensor dq = want & 1 ? whole(grads[0]) : Tensor(), dk = want & 2 && grads.size() > 1 ? whole(grads[1]) : Tensor();
     std::pair<Tensor, Tensor> g;
     if (dq.defined() || dk.defined())
       g = rotary_run(dq, dk, saved[0], saved[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
     return once({g.first, g.second, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
-std::pair<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k_, const Tensor& pos, const Tensor& freqs, const std::vector<int64_t>& sections,
+std::pair<Tensor, Maybe> rotary(const Tensor& q_, const Maybe& k_, const Tensor& pos_, const Tensor& freqs_, const std::vector<int64_t>& sections,
                                 bool interleaved) {
-  const Tensor k = plain(k_);
+  const Tensor q = whole(q_), k = plain(k_), pos = whole(pos_), freqs = whole(freqs_);
   carries("rotary", {&q, &k, &pos, &freqs});
   rotary_check(q, k, pos, freqs, sections);
   Tensor yq, yk;
   if (tracked({&q, &k})) {
-    const variable_list y = Rotary::apply(q, k_, pos, freqs, at::IntArrayRef(sections), interleaved);
+    const variable_list y = Rotary::apply(q, Maybe(k), pos, freqs, at::IntArrayRef(sections), interleaved);
     yq = y[0];
     if (y.size() > 1) yk = y[1];
   } else {
@@ -429,7 +432,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5];
     const c10::DeviceGuard guard(q.device());
     const Tensor lengths = dense(saved[6]);
-    Tensor dout = grads[0].contiguous();
+    Tensor dout = whole(grads[0]).contiguous();
     if (reinterpret_cast<uintptr_t>(dout.data_ptr()) & 15) dout = dout.clone();
     const std::vector<int64_t> w = ctx->saved_data["window"].toIntVector();
     const int64_t T = q.size(1);
@@ -445,13 +448,13 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
-Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, int64_t right, int64_t sinks, bool causal, const Maybe& lengths_,
+Tensor window_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t left, int64_t right, int64_t sinks, bool causal, const Maybe& lengths_,
                         double scale) {
-  const Tensor lengths = plain(lengths_);
+  const Tensor q = whole(q_), k = whole(k_), v = whole(v_), lengths = plain(lengths_);
   const Window w = {left, right, sinks, causal, scale};
   carries("window_attention", {&q, &k, &v});
   window_check(q, k, v, w, lengths);
-  return tracked({&q, &k, &v}) ? WindowAttention::apply(q, k, v, left, right, sinks, causal, lengths_, scale) : window_run(q, k, v, w, lengths, false).o;
+  return tracked({&q, &k, &v}) ? WindowAttention::apply(q, k, v, left, right, sinks, causal, Maybe(lengths), scale) : window_run(q, k, v, w, lengths, false).o;
 }
 
 }  // namespace

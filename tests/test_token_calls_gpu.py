@@ -1,0 +1,82 @@
+"""Ways of calling the token operators that ask more of them than dense tensors do: lazily negated views, tensors of zeros without
+memory, tensors that are not all on one device."""
+import pytest
+import torch
+
+from indm_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+SECTIONS = (8,)
+NAMES = ["layer_norm", "dropout", "dropout res", "rotary", "rotary k", "q", "k", "v"]
+
+
+def positions(T):
+    return torch.arange(T, device=DEV)[:, None]
+
+
+def operators(T=6, H=2, D=16):
+    freqs, pos = ops.rotary_freqs(SECTIONS, device=DEV), positions(T)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    other = torch.randn((2, T, H, D), generator=g, device=DEV)
+    gamma = torch.randn((D,), generator=g, device=DEV)
+    return {"layer_norm": lambda x: ops.layer_norm(x, gamma), "dropout": lambda x: ops.dropout(x, 0.4, 5), "dropout res": lambda x: ops.dropout(other, 0.4, 5, res=x),
+            "rotary": lambda x: ops.rotary(x, None, pos, freqs, SECTIONS)[0], "rotary k": lambda x: ops.rotary(other, x, pos, freqs, SECTIONS)[1],
+            "q": lambda x: ops.window_attention(x, other, other, 2), "k": lambda x: ops.window_attention(other, x, other, 2),
+            "v": lambda x: ops.window_attention(other, other, x, 2)}
+
+
+def negated(seed, shape=(2, 6, 2, 16)):
+    """a view whose memory holds the negative of its values"""
+    z = torch.randn(shape, dtype=torch.complex64, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).conj().imag
+    assert z.is_neg()
+    return z
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_negated_views_and_gradients(name):
+    call, x, dy = operators()[name], negated(2), negated(3)
+    plain = x.clone().requires_grad_()
+    want = call(plain)
+    (dwant,) = torch.autograd.grad(want, plain, dy.clone())
+    with torch.no_grad():
+        assert torch.equal(call(x), want)
+    z = torch.complex(torch.zeros_like(plain), -plain.detach()).requires_grad_()
+    view = z.conj().imag
+    assert view.is_neg()
+    got = call(view)
+    (dz,) = torch.autograd.grad(got, z, dy)
+    assert torch.equal(got, want) and torch.equal(dz.imag, -dwant)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_zeros_without_memory(name):
+    call = operators()[name]
+    zero = torch._efficientzerotensor((2, 6, 2, 16), device=DEV)
+    x = torch.zeros((2, 6, 2, 16), device=DEV)
+    with torch.no_grad():
+        assert torch.equal(call(zero), call(x))
+    leaf = torch.randn((2, 6, 2, 16), device=DEV).requires_grad_()
+    (g,) = torch.autograd.grad(call(leaf), leaf, zero)
+    assert torch.equal(g, x)
+
+
+def test_negated_parameters():
+    x, p, n = negated(4).clone(), negated(5, (16,)), positions(6).to(torch.float32)
+    neg_pos = torch.complex(torch.zeros_like(n), -n).conj().imag
+    freqs = ops.rotary_freqs(SECTIONS, device=DEV)
+    neg_freqs = torch.complex(torch.zeros_like(freqs), -freqs).conj().imag
+    assert neg_pos.is_neg() and neg_freqs.is_neg()
+    assert torch.equal(ops.layer_norm(x, p, p), ops.layer_norm(x, p.clone(), p.clone()))
+    assert torch.equal(ops.rotary(x, None, neg_pos, neg_freqs, SECTIONS)[0], ops.rotary(x, None, n, freqs, SECTIONS)[0])
+
+
+def test_tensors_left_on_the_host_are_refused():
+    """a parameter, a residual, positions, lengths left on the host"""
+    x, freqs, pos = torch.ones((2, 6, 2, 16), device=DEV), ops.rotary_freqs(SECTIONS, device=DEV), positions(6)
+    for call in (lambda: ops.layer_norm(x, torch.ones(16)), lambda: ops.layer_norm(x, None, torch.ones(16)), lambda: ops.dropout(x, 0.5, 1, res=x.cpu()),
+                 lambda: ops.rotary(x, x.cpu(), pos, freqs, SECTIONS), lambda: ops.rotary(x, None, pos.cpu(), freqs, SECTIONS),
+                 lambda: ops.rotary(x, None, pos, freqs.cpu(), SECTIONS), lambda: ops.window_attention(x, x.cpu(), x, 2),
+                 lambda: ops.window_attention(x, x, x, 2, lengths=torch.tensor([6, 6], dtype=torch.int32))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
