@@ -265,16 +265,23 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_bwd_kernel(const 
     for (int k = 0; k < RPT; ++k) {
       s1[k] = s2[k] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) xh[k][j][i] = (xh[k][j][i] - m[k]) * rs[k];
+        const int n = C - (j * L + lane) * V;
+        if (n < V) {   // (places behind the row have d = 0, but -m rs may have overflowed there)
+#pragma unroll
+          for (int i = 0; i < V; ++i) xh[k][j][i] = i < n ? xh[k][j][i] : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          xh[k][j][i] = (xh[k][j][i] - m[k]) * rs[k];   // (places behind the row have d = 0: they add nothing below)
           const float h = d[k][j][i] * g[j][i];
           dg[j][i] += d[k][j][i] * xh[k][j][i];
           db[j][i] += d[k][j][i];
           s1[k] += h;
           s2[k] += h * xh[k][j][i];
         }
+      }
     }
 #pragma unroll
     for (int k = 0; k < RPT; ++k) {

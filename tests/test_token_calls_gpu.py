@@ -80,3 +80,21 @@ def test_tensors_left_on_the_host_are_refused():
                  lambda: ops.window_attention(x, x, x, 2, lengths=torch.tensor([6, 6], dtype=torch.int32))):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+@pytest.mark.parametrize("C", [1, 3, 5, 64, 130, 300])
+def test_layer_norm_of_large_constant_rows(C):
+    """Rows of 2^119: -mean / sd overflows (2^119 / sqrt(1e-6) > 2^128) in the places behind a row that fill its last vector, and nothing of that
+    may reach a gradient.  The sums are exact (up to 300 x 2^119 < 2^128); where C is a power of two the mean is, too: y = beta, dgamma = 0,
+    dx = (h - mean h) / sqrt(eps).  Elsewhere the mean may be off by a step of 2^95, whose square overflows: sd is infinite, y = beta."""
+    x = torch.full((4, C), 2.0 ** 119, device=DEV).requires_grad_()
+    gamma, beta = torch.ones(C, device=DEV).requires_grad_(), torch.full((C,), 0.25, device=DEV).requires_grad_()
+    dy = torch.randn((4, C), generator=torch.Generator(device=DEV).manual_seed(6), device=DEV)
+    y = ops.layer_norm(x, gamma, beta)
+    dx, dg, db = torch.autograd.grad(y, (x, gamma, beta), dy)
+    assert (y == 0.25).all() and all(t.isfinite().all() for t in (dx, dg, db))
+    if C & (C - 1) == 0:
+        assert (dg == 0).all()
+        want = (dy.double() - dy.double().mean(1, keepdim=True)) * 1e3
+        # sums of at most 64 terms, half a step each; eps = 1e-6 in 32 bits, its root and its reciprocal
+        assert ((dx.double() - want).abs() <= 80 * 2.0 ** -24 * 1e3 * dy.double().abs().sum(1, keepdim=True)).all()
