@@ -278,6 +278,8 @@ void rotary_check(const Tensor& q, const Tensor& k, const Tensor& pos, const Ten
   if (D > 4096) REFUSE("rotary: heads of up to 4096 entries, got ", D);
   if (k.defined() && (k.scalar_type() != q.scalar_type() || k.dim() != 4 || k.size(0) != B || k.size(1) != T || k.size(3) != D))
     REFUSE("rotary: k is [", B, ", ", T, ", Hk, ", D, "] ", q.scalar_type(), ", got ", k.sizes(), " ", k.scalar_type());
+  for (const Tensor* x : {&q, &k})
+    if (x->defined() && (B > INT32_MAX || x->size(2) > INT32_MAX)) REFUSE("rotary: up to 2^31 - 1 samples and heads, got ", x->sizes());
   int64_t sum = 0;
   bool even = A >= 1 && A <= 8;
   for (int64_t n : sections) {
@@ -312,7 +314,6 @@ std::pair<Tensor, Tensor> rotary_run(const Tensor& q_, const Tensor& k_, const T
   for (size_t i = 0; i < sections.size(); ++i) s[i] = (int)sections[i];
   const int64_t B = any.size(0), T = any.size(1), A = (int64_t)sections.size();
   const auto type = pos.scalar_type();
-  TORCH_CHECK(B <= INT32_MAX && any.size(2) <= INT32_MAX, "indm_amd: rotary: too many samples or heads");
   ok(abi.rotary[type_of("rotary", any)](ptr<void>(q), ptr<void>(k), ptr<void>(yq), ptr<void>(yk), strides, (int)B, T, q.defined() ? (int)q.size(2) : 0,
                                         k.defined() ? (int)k.size(2) : 0, (int)any.size(3), pos.data_ptr(), type == at::kInt ? 0 : type == at::kFloat ? 1 : 2,
                                         pos.dim() == 3 ? T * A : 0, ptr<double>(freqs), s, (int)A, interleaved, inverse, stream_of(any)),

@@ -37,3 +37,13 @@ def test_tracing_is_refused(name):
     call, x = CALLS[name]
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(call, (x.clone(),), check_trace=False)
+
+
+@pytest.mark.parametrize("which", ["q heads", "k heads", "samples"])
+def test_rotary_refuses_what_does_not_fit_32_bits(which):
+    """counts that the kernel holds in 32 bits: a number past them would be taken for a small one"""
+    many = (1 << 32) + 1
+    q = torch.ones(1, 1, 1, 8).expand(many if which == "samples" else 1, 1, many if which == "q heads" else 1, 8)
+    k = torch.ones(1, 1, 1, 8).expand(1, 1, many, 8) if which == "k heads" else None
+    with pytest.raises(RuntimeError, match="samples and heads"):
+        ops.rotary(q, k, torch.zeros(1, 1), FREQS, (8,))
