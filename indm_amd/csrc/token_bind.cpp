@@ -17,6 +17,7 @@
 #include <c10/util/strides.h>
 #include <map>
 #include <mutex>
+#include "indm_hip.h"
 
 namespace {
 
@@ -26,32 +27,33 @@ using torch::autograd::variable_list;
 typedef std::optional<Tensor> Maybe;
 
 // ---------------------------------------------------------------------------------------------- the C ABI (include/indm_hip.h)
+// the entry points' addresses, with the types that the header declares
+#define ENTRIES(X)                                                                                                              \
+  X(layernorm_fwd_f32) X(layernorm_fwd_bf16) X(layernorm_bwd_ws_floats) X(layernorm_bwd_f32) X(layernorm_bwd_bf16)             \
+  X(dropout_f32) X(dropout_bf16) X(rotary_f32) X(rotary_bf16)                                                                  \
+  X(wattn_fwd_f32) X(wattn_fwd_bf16) X(wattn_bwd_ws_floats) X(wattn_bwd_f32) X(wattn_bwd_bf16)
 struct Abi {
-  int (*layernorm_fwd[2])(const void*, long, const float*, const float*, void*, float*, float*, long, int, float, void*);
-  long (*layernorm_bwd_ws_floats)(long, int, int);
-  int (*layernorm_bwd[2])(const void*, const void*, long, const float*, const float*, const float*, void*, float*, float*, float*, long, int, void*);
-  int (*dropout[2])(const void*, const void*, void*, long, float, unsigned long long, const void*, void*);
-  int (*rotary[2])(const void*, const void*, void*, void*, const long*, int, long, int, int, int, const void*, int, long, const double*, const int*, int, int, int, void*);
-  int (*wattn_fwd[2])(const void*, const void*, const void*, const long*, void*, void*, float*, const int*, int, int, int, int, int, int, int, int, int, float, void*);
-  long (*wattn_bwd_ws_floats)(int, int, int, int, int, int, int, int, int);
-  int (*wattn_bwd[2])(const void*, const void*, const void*, const long*, const void*, const void*, const void*, const float*, const int*, void*, void*, void*, float*,
-                      int, int, int, int, int, int, int, int, int, float, void*);
+#define X(name) decltype(&indm_##name) name;
+  ENTRIES(X)
+#undef X
 } abi;
 
 void bind(const std::map<std::string, uint64_t>& at) {
-  auto set = [&](auto& fn, const std::string& name) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(at.at("indm_" + name)); };
-  for (int i = 0; i < 2; ++i) {
-    const std::string t = i == 0 ? "_f32" : "_bf16";
-    set(abi.layernorm_fwd[i], "layernorm_fwd" + t);
-    set(abi.layernorm_bwd[i], "layernorm_bwd" + t);
-    set(abi.dropout[i], "dropout" + t);
-    set(abi.rotary[i], "rotary" + t);
-    set(abi.wattn_fwd[i], "wattn_fwd" + t);
-    set(abi.wattn_bwd[i], "wattn_bwd" + t);
-  }
-  set(abi.layernorm_bwd_ws_floats, "layernorm_bwd_ws_floats");
-  set(abi.wattn_bwd_ws_floats, "wattn_bwd_ws_floats");
+#define X(name) abi.name = reinterpret_cast<decltype(abi.name)>(at.at("indm_" #name));
+  ENTRIES(X)
+#undef X
 }
+// the float32 or the bfloat16 entry point; their tensors' pointers are the only arguments whose types differ
+struct Elements {
+  void* at;
+  template <typename T>
+  operator T*() const { return static_cast<T*>(at); }
+};
+template <typename F32, typename BF16, typename... A>
+int either(int type, F32 f32, BF16 bf16, A... a) {
+  return type == 0 ? f32(a...) : bf16(a...);
+}
+#define CALL(type, name, ...) either(type, abi.name##_f32, abi.name##_bf16, __VA_ARGS__)
 
 // ---------------------------------------------------------------------------------------------- what all of them do
 #define REFUSE(...) TORCH_CHECK(false, "indm_amd: ", __VA_ARGS__)
@@ -132,6 +134,7 @@ template <typename P = float>
 P* ptr(const Tensor& t) {
   return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr;
 }
+Elements elements(const Tensor& t) { return {ptr<void>(t)}; }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 // A backward pass that is itself recorded (create_graph): its results refuse to be differentiated again
@@ -193,8 +196,8 @@ std::pair<Tensor, Tensor> layer_norm_run(const Tensor& x, const Tensor& gamma_, 
   const Tensor gamma = dense(gamma_), beta = dense(beta_);
   const Rows r = rows_of(x);
   Tensor y = dense_like(x), st = stats ? floats(2 * r.n, x) : Tensor();
-  ok(abi.layernorm_fwd[type_of("layer_norm", x)](r.x.data_ptr(), r.ld, ptr(gamma), ptr(beta), y.data_ptr(), ptr(st), stats ? ptr(st) + r.n : nullptr, r.n,
-                                                 (int)x.size(-1), (float)eps, stream_of(x)),
+  ok(CALL(type_of("layer_norm", x), layernorm_fwd, elements(r.x), r.ld, ptr(gamma), ptr(beta), elements(y), ptr(st), stats ? ptr(st) + r.n : nullptr, r.n,
+          (int)x.size(-1), (float)eps, stream_of(x)),
      "indm_layernorm_fwd");
   return {y, st};
 }
@@ -216,8 +219,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     Tensor dx = dense_like(x), dgamma = want & 2 ? floats(C, x) : Tensor(), dbeta = want & 4 ? floats(C, x) : Tensor(), ws;
     // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
     if (want & 6) ws = floats(std::max(1L, abi.layernorm_bwd_ws_floats(r.n, (int)C, (int)x.element_size())), x);
-    ok(abi.layernorm_bwd[type_of("layer_norm", x)](dy.data_ptr(), r.x.data_ptr(), r.ld, ptr(gamma), ptr(stats), ptr(stats) + r.n, dx.data_ptr(), ptr(dgamma),
-                                                   ptr(dbeta), ptr(ws), r.n, (int)C, stream_of(x)),
+    ok(CALL(type_of("layer_norm", x), layernorm_bwd, elements(dy), elements(r.x), r.ld, ptr(gamma), ptr(stats), ptr(stats) + r.n, elements(dx), ptr(dgamma),
+            ptr(dbeta), ptr(ws), r.n, (int)C, stream_of(x)),
        "indm_layernorm_bwd");
     return once({dx, dgamma, dbeta, Tensor()});
   }
@@ -234,7 +237,7 @@ Tensor dropout_run(const Tensor& x_, double p, uint64_t seed, const Tensor& res_
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = dense(x_), res = dense(res_);
   Tensor y = dense_like(x);
-  ok(abi.dropout[type_of("dropout", x)](x.data_ptr(), ptr<void>(res), y.data_ptr(), x.numel(), (float)p, seed, ptr<void>(seed_dev), stream_of(x)),
+  ok(CALL(type_of("dropout", x), dropout, elements(x), elements(res), elements(y), x.numel(), (float)p, seed, ptr<void>(seed_dev), stream_of(x)),
      "indm_dropout");
   return y;
 }
@@ -314,9 +317,9 @@ std::pair<Tensor, Tensor> rotary_run(const Tensor& q_, const Tensor& k_, const T
   for (size_t i = 0; i < sections.size(); ++i) s[i] = (int)sections[i];
   const int64_t B = any.size(0), T = any.size(1), A = (int64_t)sections.size();
   const auto type = pos.scalar_type();
-  ok(abi.rotary[type_of("rotary", any)](ptr<void>(q), ptr<void>(k), ptr<void>(yq), ptr<void>(yk), strides, (int)B, T, q.defined() ? (int)q.size(2) : 0,
-                                        k.defined() ? (int)k.size(2) : 0, (int)any.size(3), pos.data_ptr(), type == at::kInt ? 0 : type == at::kFloat ? 1 : 2,
-                                        pos.dim() == 3 ? T * A : 0, ptr<double>(freqs), s, (int)A, interleaved, inverse, stream_of(any)),
+  ok(CALL(type_of("rotary", any), rotary, elements(q), elements(k), elements(yq), elements(yk), strides, (int)B, T, q.defined() ? (int)q.size(2) : 0,
+          k.defined() ? (int)k.size(2) : 0, (int)any.size(3), pos.data_ptr(), type == at::kInt ? 0 : type == at::kFloat ? 1 : 2, pos.dim() == 3 ? T * A : 0,
+          ptr<double>(freqs), s, (int)A, interleaved, inverse, stream_of(any)),
      "indm_rotary");
   return {yq, yk};
 }
@@ -412,9 +415,10 @@ WindowOut window_run(const Tensor& q_, const Tensor& k_, const Tensor& v_, const
     r.lse = floats(B * H * T, r.q);
     if (r.q.scalar_type() == at::kBFloat16) r.rest = dense_like(r.q);
   }
-  ok(abi.wattn_fwd[type_of("window_attention", r.q)](r.q.data_ptr(), r.k.data_ptr(), r.v.data_ptr(), Heads(r.q, r.k, r.v).strides, r.o.data_ptr(), ptr<void>(r.rest), ptr(r.lse),
-                                                     ptr<int>(lengths), (int)B, (int)T, (int)H, (int)r.k.size(2), (int)D, (int)std::min(w.left, T), (int)std::min(w.right, T),
-                                                     (int)std::min(w.sinks, T), w.causal, (float)w.scale, stream_of(r.q)),
+  const Heads heads(r.q, r.k, r.v);
+  ok(CALL(type_of("window_attention", r.q), wattn_fwd, elements(r.q), elements(r.k), elements(r.v), heads.strides, elements(r.o), ptr<void>(r.rest), ptr(r.lse),
+          ptr<int>(lengths), (int)B, (int)T, (int)H, (int)r.k.size(2), (int)D, (int)std::min(w.left, T), (int)std::min(w.right, T), (int)std::min(w.sinks, T),
+          (int)w.causal, (float)w.scale, stream_of(r.q)),
      "indm_wattn_fwd");
   return r;
 }
@@ -442,9 +446,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     Tensor dq = dense_like(q), dk = dense_like(k), dv = dense_like(v);
     // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
     Tensor ws = floats(std::max(1L, abi.wattn_bwd_ws_floats(B, (int)T, H, Hk, D, left, right, sinks, causal)), q);
-    ok(abi.wattn_bwd[type_of("window_attention", q)](q.data_ptr(), k.data_ptr(), v.data_ptr(), Heads(q, k, v).strides, o.data_ptr(), ptr<void>(rest), dout.data_ptr(), ptr(lse),
-                                                     ptr<int>(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(ws), B, (int)T, H, Hk, D, left, right, sinks, causal,
-                                                     (float)ctx->saved_data["scale"].toDouble(), stream_of(q)),
+    const Heads heads(q, k, v);
+    ok(CALL(type_of("window_attention", q), wattn_bwd, elements(q), elements(k), elements(v), heads.strides, elements(o), ptr<void>(rest), elements(dout), ptr(lse),
+            ptr<int>(lengths), elements(dq), elements(dk), elements(dv), ptr(ws), B, (int)T, H, Hk, D, left, right, sinks, causal,
+            (float)ctx->saved_data["scale"].toDouble(), stream_of(q)),
        "indm_wattn_bwd");
     return once({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
