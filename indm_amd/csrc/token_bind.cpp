@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 #include <c10/util/accumulate.h>
 #include <c10/util/strides.h>
+#include <atomic>
 #include <map>
 #include <mutex>
 #include "indm_hip.h"
@@ -96,36 +97,42 @@ void on_one_gpu(const char* op, std::initializer_list<const Tensor*> ts) {
 }
 void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
 // Every tensor that a kernel writes comes from here.  guard(bytes) pads them with bands of that many bytes of a pattern on both sides
-// (a debugging mode, like POISON_WS: a store outside of a tensor that hits a free block would go unseen), broken_guards() counts the
-// bands that were written to and forgets the tensors.
+// (a debugging mode, like POISON_WS: a store outside of a tensor that hits a free block would go unseen).  The padded tensors are kept until
+// broken_guards() counts the bands that were written to and forgets them; each remembers its bands, whatever guard() says by then.
+struct Guarded {
+  Tensor raw;
+  int64_t band;
+};
 struct Guards {
-  int64_t bytes = 0;
-  std::vector<Tensor> raw;
+  std::atomic<int64_t> band{0};   // (calls on other threads read it while guard() sets it: once each)
   std::mutex lock;
+  std::vector<Guarded> kept;
 } guards;
 constexpr uint8_t GUARD = 0xA5;
 Tensor fresh(at::IntArrayRef sizes, const at::TensorOptions& opt) {
-  if (guards.bytes == 0) return at::empty(sizes, opt);
+  const int64_t band = guards.band.load(std::memory_order_relaxed);
+  if (band == 0) return at::empty(sizes, opt);
   const int64_t n = c10::multiply_integers(sizes), e = (int64_t)opt.dtype().itemsize();
-  Tensor raw = at::empty({n * e + 2 * guards.bytes}, opt.dtype(at::kByte));
+  Tensor raw = at::empty({n * e + 2 * band}, opt.dtype(at::kByte));
   raw.fill_(GUARD);
-  Tensor t = at::empty({0}, opt).set_(raw.storage(), guards.bytes / e, sizes, c10::contiguous_strides(sizes));
+  Tensor t = at::empty({0}, opt).set_(raw.storage(), band / e, sizes, c10::contiguous_strides(sizes));
   const std::lock_guard<std::mutex> hold(guards.lock);
-  guards.raw.push_back(raw);
+  guards.kept.push_back({raw, band});
   return t;
 }
-void guard(int64_t bytes) { guards.bytes = bytes / 256 * 256; }
+void guard(int64_t bytes) {
+  if (bytes < 0) REFUSE("guard: bands of 0 bytes or more, got ", bytes);
+  guards.band = (bytes + 255) / 256 * 256;
+}
 int64_t broken_guards() {
-  std::vector<Tensor> raw;
+  std::vector<Guarded> kept;
   {
     const std::lock_guard<std::mutex> hold(guards.lock);
-    raw.swap(guards.raw);
+    kept.swap(guards.kept);
   }
   int64_t broken = 0;
-  for (const Tensor& r : raw) {
-    const int64_t g = guards.bytes;
-    broken += r.narrow(0, 0, g).ne(GUARD).any().item<bool>() + r.narrow(0, r.size(0) - g, g).ne(GUARD).any().item<bool>();
-  }
+  for (const Guarded& g : kept)
+    for (const int64_t at : {(int64_t)0, g.raw.size(0) - g.band}) broken += g.raw.narrow(0, at, g.band).ne(GUARD).any().item<bool>();
   return broken;
 }
 Tensor dense_like(const Tensor& x) { return fresh(x.sizes(), x.options()); }

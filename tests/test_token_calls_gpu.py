@@ -3,7 +3,7 @@ memory, tensors that are not all on one device."""
 import pytest
 import torch
 
-from indm_amd import ops
+from indm_amd import hip, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -98,3 +98,54 @@ def test_layer_norm_of_large_constant_rows(C):
         want = (dy.double() - dy.double().mean(1, keepdim=True)) * 1e3
         # sums of at most 64 terms, half a step each; eps = 1e-6 in 32 bits, its root and its reciprocal
         assert ((dx.double() - want).abs() <= 80 * 2.0 ** -24 * 1e3 * dy.double().abs().sum(1, keepdim=True)).all()
+
+
+def test_guard_bands_keep_their_own_size():
+    """bands set anew, or switched off, between the call that made a tensor and the count: each tensor is counted by its own"""
+    ext, x = hip.token_ops(), torch.ones(1000, device=DEV)
+    try:
+        for then in (1 << 16, 0):
+            ext.guard(512)
+            y = ops.dropout(x, 0.5, 1)
+            ext.guard(then)
+            assert ext.broken_guards() == 0
+            ext.guard(512)
+            y = ops.dropout(x, 0.5, 1)
+            y.as_strided((1,), (1,), y.storage_offset() - 128).fill_(2.0)     # the first of the 128 floats in front of it
+            ext.guard(then)
+            assert ext.broken_guards() == 1 and ext.broken_guards() == 0
+    finally:
+        ext.broken_guards()
+        ext.guard(0)
+
+
+def test_guard_bands_while_other_threads_call():
+    """calls on four threads, forward and backward, while the bands change: none is lost, none is counted by another's size"""
+    import threading
+    ext, bad = hip.token_ops(), []
+    x = torch.randn((64, 96), device=DEV)
+    want = ops.layer_norm(x)
+
+    def work():
+        try:
+            for _ in range(50):
+                leaf = x.clone().requires_grad_()
+                y = ops.layer_norm(leaf)
+                torch.autograd.grad(y, leaf, x)
+                if not torch.equal(y, want):
+                    bad.append("result")
+        except Exception as e:   # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    try:
+        for t in threads:
+            t.start()
+        for i in range(200):
+            ext.guard((0, 256, 1 << 14)[i % 3])
+        for t in threads:
+            t.join()
+        assert not bad and ext.broken_guards() == 0
+    finally:
+        ext.broken_guards()
+        ext.guard(0)
