@@ -667,6 +667,11 @@ int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, const long*
                         const float* lse, const int* lengths, void* dq, void* dk, void* dv, float* ws, int B, int T, int H, int Hk,
                         int D, int left, int right, int sinks, int causal, float scale, void* stream);
 
+/* How the entry points above lay a call's work out (host only; for tests and for reading a trace): bit 0: a workgroup's wavefronts share 32
+ * queries (forward, dq); bit 1: 32 keys (dk / dv); bit 2: the sinks' workgroups are a launch of their own; bits 4 - 15: the workgroups that
+ * share a key block's queries; bits 16 - 30: those that share a sink block's (0: the sinks reach nothing beyond the window). */
+int indm_wattn_layout(int elem_bytes, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1031,3 +1031,10 @@ INDM_API int indm_wattn_bwd_bf16(const void* q, const void* k, const void* v, co
   return bwd<u16>(pack_args(q, k, v, strides, lengths, B, T, H, Hk, D, left, right, sinks, causal, scale), strides, o, o_lo, dO, lse, dq, dk,
                   dv, ws, (hipStream_t)stream);
 }
+
+INDM_API int indm_wattn_layout(int elem_bytes, int B, int T, int H, int Hk, int D, int left, int right, int sinks, int causal) {
+  if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0 || left < 0 || right < 0 || sinks < 0 || (elem_bytes != 2 && elem_bytes != 4)) return INDM_E_SHAPE;
+  const Plan plan = plan_keys(elem_bytes == 2 ? Geo<u16, 32>::BN : Geo<float, 32>::BN, B, T, H, Hk, left < T ? left : T, right < T ? right : T,
+                              sinks < T ? sinks : T, causal != 0);
+  return (share_queries(B, T, H) ? 1 : 0) | (plan.share ? 2 : 0) | (plan.apart ? 4 : 0) | plan.splits << 4 | plan.chunks << 16;
+}

@@ -174,6 +174,7 @@ _SIGS = {
     "indm_wattn_fwd_f32": [c_p] * 8 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_fwd_bf16": [c_p] * 8 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_bwd_ws_floats": [c_i] * 9,
+    "indm_wattn_layout": [c_i] * 10,
     "indm_wattn_bwd_f32": [c_p] * 13 + [c_i] * 9 + [c_f, c_p],
     "indm_wattn_bwd_bf16": [c_p] * 13 + [c_i] * 9 + [c_f, c_p],
     "indm_timer_create": [c_i, c_p],

@@ -8,6 +8,8 @@ import subprocess
 
 import pytest
 
+from indm_amd import hip
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "indm_amd", "csrc")
 HEADER = os.path.join("..", "..", "include", "indm_hip.h")
@@ -42,3 +44,14 @@ def test_a_changed_signature_does_not_compile(tmp_path, change):
     run = subprocess.run(cmd, cwd=CSRC, capture_output=True, text=True, timeout=300)
     assert (run.returncode == 0) == (change is None), run.stderr[-2000:]
     assert change is None or "error" in run.stderr
+
+
+def test_layout_query():
+    """few blocks are shared, many are not; bad sizes are refused"""
+    f = hip.lib().indm_wattn_layout
+    assert f(2, 1, 256, 4, 4, 64, 64, 64, 1, 0) == 1 | 2 | 1 << 4 | 1 << 16      # 8 key blocks; a sink block's 4 tiles of queries: one workgroup
+    assert f(2, 8, 4096, 4, 4, 64, 256, 256, 0, 0) == 1 << 4                     # 1024 blocks of queries and of keys: nothing is shared
+    assert f(2, 8, 4096, 4, 4, 64, 256, 256, 4, 0) & 0xffff == 4 | 1 << 4        # the sinks apart
+    for bad in ((3, 1, 8, 1, 1), (2, 1, 8, 3, 2), (2, 0, 8, 1, 1), (2, 1, 0, 1, 1), (2, 1, 8, 0, 0)):
+        assert f(*bad, 32, 1, 1, 0, 0) == -1
+    assert f(2, 1, 8, 1, 1, 32, -1, 1, 0, 0) == f(2, 1, 8, 1, 1, 32, 1, 1, -1, 0) == f(2, 1, 8, 1, 1, 0, 1, 1, 0, 0) == -1
