@@ -613,7 +613,7 @@ int indm_layernorm_fwd_f32(const float* x, long ldx, const float* gamma, const f
                            long R, int C, float eps, void* stream);
 int indm_layernorm_fwd_bf16(const void* x, long ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd, long R,
                             int C, float eps, void* stream);
-/* Its backward: dx (dense) and, where the pointers are given, dgamma = sum_r dy xh and dbeta = sum_r dy (fp32 [C]) in one pass over
+/* Its backward: where the pointers are given, dx (dense), dgamma = sum_r dy xh and dbeta = sum_r dy (fp32 [C]) in one pass over
  * dy [R, C] and x; the column sums are joined over workgroups in a fixed order through ws (indm_layernorm_bwd_ws_floats floats,
  * elem_bytes 4 or 2; NULL when neither gradient is wanted).  R = 0 writes zeros to dgamma / dbeta. */
 long indm_layernorm_bwd_ws_floats(long R, int C, int elem_bytes);

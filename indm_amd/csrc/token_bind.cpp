@@ -223,7 +223,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const c10::DeviceGuard guard(x.device());
     const Tensor gamma = dense(saved[1]), dy = whole(grads[0]).contiguous();
     const Rows r = rows_of(x);
-    Tensor dx = dense_like(x), dgamma = want & 2 ? floats(C, x) : Tensor(), dbeta = want & 4 ? floats(C, x) : Tensor(), ws;
+    Tensor dx = want & 1 ? dense_like(x) : Tensor(), dgamma = want & 2 ? floats(C, x) : Tensor(), dbeta = want & 4 ? floats(C, x) : Tensor(), ws;
     // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
     if (want & 6) ws = floats(std::max(1L, abi.layernorm_bwd_ws_floats(r.n, (int)C, (int)x.element_size())), x);
     ok(CALL(type_of("layer_norm", x), layernorm_bwd, elements(dy), elements(r.x), r.ld, ptr(gamma), ptr(stats), ptr(stats) + r.n, elements(dx), ptr(dgamma),

@@ -222,7 +222,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_fwd_kernel(const 
   }
 }
 
-// dx = rstd (h - mean(h) - xh mean(h xh)),  h = dy gamma,  xh = (x - mean) rstd;  per-workgroup partial sums of
+// dx = rstd (h - mean(h) - xh mean(h xh)),  h = dy gamma,  xh = (x - mean) rstd  (dx may be NULL);  per-workgroup partial sums of
 // dgamma = sum dy xh and dbeta = sum dy in registers over the workgroup's rows, folded over its teams in a fixed order and
 // written to part[workgroup][2][C] (layernorm_param_kernel adds those up: no atomics, the same bits every time).
 template <typename T, int L, int NV, int RPT>
@@ -283,6 +283,7 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void layernorm_bwd_kernel(const 
         }
       }
     }
+    if (dx == nullptr) continue;   // (the same for all: the parameters' gradients alone are wanted)
 #pragma unroll
     for (int k = 0; k < RPT; ++k) {
       s1[k] = team_sum<L>(s1[k], sh) * inv;
@@ -471,7 +472,8 @@ int ln_bwd(const T* dy, const T* x, long ldx, const float* gamma, const float* m
     hipLaunchKernelGGL(layernorm_param_kernel, dim3(cdiv(2L * C, 32)), dim3(1024), 0, st, ws, dgamma, dbeta, 0, C);
     return hipGetLastError() == hipSuccess ? INDM_OK : INDM_E_LAUNCH;
   }
-  if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || dx == nullptr) return INDM_E_ARG;
+  if (dx == nullptr && dgamma == nullptr && dbeta == nullptr) return INDM_OK;
+  if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr) return INDM_E_ARG;
   if ((dgamma != nullptr || dbeta != nullptr) && ws == nullptr) return INDM_E_ARG;
 #define LN_BWD(L, NV) launch_ln_bwd<T, L, NV>(dy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, ws, R, C, st)
   LN_DISPATCH_BWD(LN_BWD)

@@ -1,9 +1,11 @@
 """Ways of calling the token operators that they refuse rather than answer wrongly, whatever device the tensors are on."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from indm_amd import ops
+from indm_amd import hip, ops
 
 X, G, POS, FREQS = torch.ones(2, 3, 2, 8), torch.ones(8), torch.zeros(3, 1), ops.rotary_freqs((8,))
 CALLS = {
@@ -47,3 +49,13 @@ def test_rotary_refuses_what_does_not_fit_32_bits(which):
     k = torch.ones(1, 1, 1, 8).expand(1, 1, many, 8) if which == "k heads" else None
     with pytest.raises(RuntimeError, match="samples and heads"):
         ops.rotary(q, k, torch.zeros(1, 1), FREQS, (8,))
+
+
+def test_gradients_that_are_not_wanted():
+    """the C entry points: no gradient wanted is no work"""
+    buf = (ctypes.c_char * 512)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    for suf in ("f32", "bf16"):
+        norm = getattr(hip.lib(), "indm_layernorm_bwd_" + suf)
+        assert norm(p, p, 8, None, p, p, None, None, None, None, 4, 8, None) == 0
+        assert norm(p, p, 8, None, p, p, None, p, None, None, 4, 8, None) == -4      # (the parameters' gradients need the scratch)

@@ -149,3 +149,22 @@ def test_guard_bands_while_other_threads_call():
     finally:
         ext.broken_guards()
         ext.guard(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,C", [(50, 96), (9000, 256), (300, 1153), (40, 9000)])
+def test_layer_norm_parameters_alone(dtype, R, C):
+    """x frozen: no gradient of it is made, and the parameters' are the same numbers"""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x, dy = (torch.randn((R, C), generator=g, device=DEV).to(dtype) for _ in range(2))
+    gamma, beta = (torch.randn((C,), generator=g, device=DEV).requires_grad_() for _ in range(2))
+    leaf = x.clone().requires_grad_()
+    want = torch.autograd.grad(ops.layer_norm(leaf, gamma, beta), (gamma, beta), dy)
+    y = ops.layer_norm(x, gamma, beta)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = torch.autograd.grad(y, (gamma, beta), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if R * C > 1 << 21:     # (its partial sums take 16 bytes a column of up to 1024 workgroups' rows)
+        assert torch.cuda.max_memory_allocated() - before < x.numel() * x.element_size() + 8 * C * min(R, 1024)
