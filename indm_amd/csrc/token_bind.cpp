@@ -436,6 +436,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     WindowOut r = window_run(q, k, v, {left, right, sinks, causal, scale}, lengths, true);
     ctx->save_for_backward({r.q, r.k, r.v, r.o, r.rest, r.lse, lengths});
     ctx->saved_data["window"] = std::vector<int64_t>{left, right, sinks, causal};
+    ctx->saved_data["want"] = (int64_t)((q.requires_grad() ? 1 : 0) | (k.requires_grad() || v.requires_grad() ? 2 : 0));   // (dk and dv come together)
     ctx->saved_data["scale"] = scale;
     return r.o;
   }
@@ -450,7 +451,8 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const int64_t T = q.size(1);
     const int B = (int)q.size(0), H = (int)q.size(2), Hk = (int)k.size(2), D = (int)q.size(3);
     const int left = (int)std::min(w[0], T), right = (int)std::min(w[1], T), sinks = (int)std::min(w[2], T), causal = (int)w[3];
-    Tensor dq = dense_like(q), dk = dense_like(k), dv = dense_like(v);
+    const int64_t want = ctx->saved_data["want"].toInt();
+    Tensor dq = want & 1 ? dense_like(q) : Tensor(), dk = want & 2 ? dense_like(k) : Tensor(), dv = want & 2 ? dense_like(v) : Tensor();
     // (the scratch is an allocation of its own: calls on other streams and in other captured graphs share nothing)
     Tensor ws = floats(std::max(1L, abi.wattn_bwd_ws_floats(B, (int)T, H, Hk, D, left, right, sinks, causal)), q);
     const Heads heads(q, k, v);

@@ -399,7 +399,8 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
   const T* V = (const T*)p.v + b * p.vb + hk * p.vh;
   const long orow = (((long)b * p.T + i) * p.H + h) * p.D, srow = ((long)b * p.H + h) * p.T + i;
   const bool live = i < n;
-  const KeyTiles kt = key_tiles(p, q0, q0 + OWN - 1, n, G::BN);
+  const bool wanted = !BWD || p.dq != nullptr;   // (dq not wanted: <dO, o> alone, for the other kernels)
+  const KeyTiles kt = key_tiles(p, q0, q0 + OWN - 1, wanted ? n : 0, G::BN);
   auto first_of = [&](int it) { return (it < kt.ns ? it : kt.t0 + it - kt.ns) * G::BN; };
   const int swave = SHARE ? 0 : wave, it0 = SHARE ? wave : 0;
   const Stager<T, DP, SHARE ? 1 : WV> ks(p.kt, swave, lane), vs(p.vt, swave, lane);
@@ -520,6 +521,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
     staged<SHARE>();
   }
 
+  if (!wanted) return;
   if constexpr (!BWD) sum = half_sum(sum);
   float inv = sum > 0.f ? 1.f / sum : 0.f;
   auto emit = [&](int u, float (&v)[8]) {   // a half of the result, before the division by the sum
@@ -965,7 +967,8 @@ template <typename T, int DP>
 int bwd_dp(const WAttnArgs& p, const Plan& plan, hipStream_t st) {
   int r = share_queries(p.B, p.T, p.H) ? run_query<T, DP, true, true>(p, st) : run_query<T, DP, false, true>(p, st);   // dq; delta for the others
   const bool sinks = p.chunks > 0;
-  if (r == INDM_OK && sinks && plan.apart) r = run_key<T, DP, true, false, SINKS>(p, st);
+  if (r != INDM_OK || p.dk == nullptr) return r;
+  if (sinks && plan.apart) r = run_key<T, DP, true, false, SINKS>(p, st);
   if (r == INDM_OK)
     r = p.splits > 1 ? (plan.share ? run_key<T, DP, true, true, BOTH>(p, st) : run_key<T, DP, false, true, BOTH>(p, st))
                      : (plan.share ? run_key<T, DP, true, false, BOTH>(p, st) : run_key<T, DP, false, false, KEYS>(p, st));
@@ -978,7 +981,9 @@ int bwd(WAttnArgs p, const long* strides, const void* o, const void* olo, const 
         hipStream_t st) {
   const int r = check<T>(p, strides);
   if (r <= 0) return r;
-  if (o == nullptr || dO == nullptr || lse == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || ws == nullptr ||
+  if ((dk == nullptr) != (dv == nullptr)) return INDM_E_ARG;
+  if (dq == nullptr && dk == nullptr) return INDM_OK;
+  if (o == nullptr || dO == nullptr || lse == nullptr || ws == nullptr ||
       (((uintptr_t)o | (uintptr_t)olo | (uintptr_t)dO | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)) return INDM_E_ARG;
   p.o = o; p.olo = const_cast<void*>(olo); p.dO = dO; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = ws;

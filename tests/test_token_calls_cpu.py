@@ -52,10 +52,16 @@ def test_rotary_refuses_what_does_not_fit_32_bits(which):
 
 
 def test_gradients_that_are_not_wanted():
-    """the C entry points: no gradient wanted is no work"""
+    """the C entry points: no gradient wanted is no work, dk and dv come together"""
     buf = (ctypes.c_char * 512)()
     p = (ctypes.addressof(buf) + 63) // 64 * 64
+    strides = (ctypes.c_long * 9)(*[64] * 9)
     for suf in ("f32", "bf16"):
-        norm = getattr(hip.lib(), "indm_layernorm_bwd_" + suf)
+        norm, attn = getattr(hip.lib(), "indm_layernorm_bwd_" + suf), getattr(hip.lib(), "indm_wattn_bwd_" + suf)
         assert norm(p, p, 8, None, p, p, None, None, None, None, 4, 8, None) == 0
         assert norm(p, p, 8, None, p, p, None, p, None, None, 4, 8, None) == -4      # (the parameters' gradients need the scratch)
+
+        def f(dq, dk, dv):
+            return attn(p, p, p, strides, p, None, p, p, None, dq, dk, dv, p, 1, 4, 2, 1, 16, 1, 1, 0, 0, 1.0, None)
+
+        assert f(None, None, None) == 0 and f(p, p, None) == f(p, None, p) == f(None, p, None) == f(p + 4, None, None) == -4

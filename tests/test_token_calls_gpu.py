@@ -152,6 +152,25 @@ def test_guard_bands_while_other_threads_call():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,H,Hk", [(1, 90, 2, 1), (1, 500, 8, 2), (5, 600, 8, 2), (40, 300, 4, 4)])     # (each layout of the key kernels)
+def test_window_attention_wanted_gradients_only(dtype, B, T, H, Hk):
+    """some of q, k, v frozen: the others' gradients are the same numbers"""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    xs = [torch.randn((B, T, h, 32), generator=g, device=DEV).to(dtype) for h in (H, Hk, Hk)]
+    do = torch.randn((B, T, H, 32), generator=g, device=DEV).to(dtype)
+    lengths = torch.tensor([T - b % 3 * 17 for b in range(B)], dtype=torch.int32, device=DEV)
+
+    def grads(keep):
+        leaves = [x.clone().requires_grad_(i in keep) for i, x in enumerate(xs)]
+        o = ops.window_attention(*leaves, 200, sinks=3, lengths=lengths)
+        return torch.autograd.grad(o, [leaves[i] for i in keep], do)
+
+    want = grads((0, 1, 2))
+    for keep in ((0,), (1,), (2,), (0, 1), (1, 2), (0, 2)):
+        assert all(torch.equal(a, want[i]) for a, i in zip(grads(keep), keep)), keep
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("R,C", [(50, 96), (9000, 256), (300, 1153), (40, 9000)])
 def test_layer_norm_parameters_alone(dtype, R, C):
     """x frozen: no gradient of it is made, and the parameters' are the same numbers"""
