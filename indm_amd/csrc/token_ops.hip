@@ -112,7 +112,8 @@ __device__ __forceinline__ void load_param(const float* p, int n, float fill, fl
 // A team of L lanes owns a row and keeps it in registers (NV vectors a lane), so the statistics are the two-pass ones -- the
 // mean, then the sum of squared differences from it -- and x is read from HBM once.  L < 64: several rows a wavefront.
 // HBM-bound.  131072 rows of 256, bf16: forward 24 us (5.6 TB/s, a copy's rate), backward 39 us (5.1 TB/s) and 4 us for the parameters'
-// sums; 4099 rows of 1153, fp32, out of wider rows: 10 us, 16.5 us and 4 us; 256 rows: 2.7 us, a launch.  Rows that start on odd bf16
+// sums; 4099 rows of 1153, fp32, out of wider rows: 10 us, 16.5 us and 4 us (384 and 512 slots for the 289 vectors of a row, and backward
+// four barriers a row); 256 rows: 2.8 us, a launch.  Rows that start on odd bf16
 // elements cost the backward pass half its rate (2.4 TB/s: the memory pipe splits those accesses).
 // Sum over the team; every lane gets the same bits (each step adds a pair, whichever order).  Within a wavefront all steps are
 // vector instructions: lanes 1, 2, then mirrored quads and halves of a row of 16, then rows and halves of the wavefront traded.
@@ -404,7 +405,8 @@ constexpr int ln_rpt(int V, int NV, int L) { return L > 256 ? 1 : NV * V <= 8 ? 
 constexpr int ln_bwd_rpt(int V, int NV, int L) { return L <= 64 && NV * V <= 8 ? 2 : 1; }
 
 // workgroups of the backward pass: enough to fill the chip, but few enough that the partial sums (16 C bytes a workgroup, written and
-// read) stay a sixth of the rows' 3 R C elem bytes
+// read) stay a sixth of the rows' 3 R C elem bytes, from 4096 rows of bf16 or 2048 of fp32 on.  Fewer rows still have up to 256 workgroups, whose
+// partial sums may be more than the rows themselves (256 rows of 8192 bf16: 33 MB next to 12.6 MB).
 inline int ln_bwd_blocks(long R, int teams, int elem) {
   const long rows = (R + teams - 1) / teams;
   long nb = R * elem / 32;

@@ -18,16 +18,17 @@
 // On fp32 the same operands are 8 values a lane and a product is 8 v_mfma_f32_32x32x2_f32 (their k order differs from the bf16
 // instruction's, the same way on both sides).  P and dS enter the second product on bf16 tensors as two operands, their rounding and what
 // it left: o and every gradient then have the error of one rounding, 1.66e-3 of their norm (with one operand the gradients had 2.4e-3; the
-// rest's products cost dq 58 -> 68 us and dk / dv 66 -> 85 us in the first case below).
+// rest's products cost dq 57 -> 67 us and dk / dv 65 -> 82 us in the first case below).
 // The softmax is exp2 with a running maximum that is raised only when a new logit exceeds it by 8 (P <= 256 then: no digit is lost,
 // and the accumulators are rescaled once or twice a row instead of once a tile).
 //
 // What bounds the kernels is neither HBM nor the matrix instructions alone but the chain product -> exponential -> product of the
 // few wavefronts that the registers allow, on vector instructions and LDS reads in turn.  8 sequences of 4096 tokens, 4 heads of 64, 256
-// tokens of window to each side, 4 sinks (bf16): forward 48 us (4 wavefronts a SIMD, vector unit busy 62 %, matrix unit 29 %; 360
-// TFLOP/s of the formula's two products), dq 55 us, the sinks' part 13.5 + 5 us, dk / dv 61 us (2 wavefronts a SIMD, 42 % and 27 %).  5 ragged
-// sequences of 1543, 8 heads of 128 on 2, causal: 39, 42, 85 + 12 us.  2 x 1021 fp32 tokens, 4 heads of 40: 11.7, 14, 25 + 4 us.  256
-// tokens, 4 heads of 64: 6.1 us.
+// tokens of window to each side, 4 sinks (bf16; medians of a kernel trace): forward 52 us (4 wavefronts a SIMD, vector unit busy 61 %, matrix
+// unit 29 %; 330 TFLOP/s of the formula's two products), dq 67 us (48 % and 30 %), the sinks' part 15 + 5 us, dk / dv 82 us (2 wavefronts a
+// SIMD, 45 % and 34 %).  5 ragged sequences of 1543, 8 heads of 128 on 2, causal: 39, 48, 93 + 12 us.  2 x 1021 fp32 tokens, 4 heads of 40: 12, 14,
+// 25 + 4 us.  256 tokens, 4 heads of 64: 6.3 us.  Every token of 8 x 4096, 4 heads of 64: bf16 267 us (510 TFLOP/s), 321, 479; fp32 1168 us
+// (118 TFLOP/s), 1640, 2135.
 #include "indm_common.h"
 #pragma clang diagnostic ignored "-Winline-asm"
 
@@ -902,8 +903,9 @@ inline Plan plan_keys(int tile, int B, int T, int H, int Hk, int left, int right
     r.share = blocks * r.splits <= SHARE_BELOW;
   }
   // Do the sinks reach queries outside of the window?  Then all queries of a block of them are shared by so many workgroups that a
-  // wavefront which streams by itself has one tile and a workgroup that streams together eight, up to one or two a compute unit (16 MB
-  // of partial sums at most).  Where the key blocks leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens,
+  // wavefront which streams by itself has one tile and a workgroup that streams together eight, up to one or two a compute unit: 256
+  // partial sums of 32 sinks or 512 of 128, 8 or 64 MB at 128 entries.  More blocks of sinks than that have one workgroup each, and the partial
+  // sums then are as large as two fp32 copies of the sinks' dk and dv (one, where key blocks are split).  Where the key blocks leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens,
   // 8 heads of 128 on 2: 97 us together, 113 apart; 2 x 1021 fp32 tokens, 4 heads of 40: 29 us, 31); where they fill it, it is a launch
   // before (8 x 4096 tokens, 4 heads of 64: 80 us apart, 89 together).
   if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
