@@ -75,7 +75,8 @@ bool tracked(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 // What these functions cannot carry through is refused, not dropped: the tangent of a forward-mode derivative (a dual tensor need not
-// require grad), and the call itself under torch.jit.trace, which would record an allocation in its place.
+// require grad; the gradient that a backward pass is given may have one), and the call itself under torch.jit.trace, which would record an
+// allocation in its place.
 void carries(const char* op, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->_fw_grad(/*level=*/0).defined()) REFUSE(op, ": forward-mode derivatives are not computed");
@@ -219,6 +220,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &stats = saved[2];
+    carries("layer_norm", {&grads[0]});
     const int64_t want = ctx->saved_data["want"].toInt(), C = x.size(-1);
     const c10::DeviceGuard guard(x.device());
     const Tensor gamma = dense(saved[1]), dy = whole(grads[0]).contiguous();
@@ -261,6 +263,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const int64_t want = ctx->saved_data["want"].toInt();
     const auto at = ctx->saved_data.find("seed_dev");
     Tensor dx;
+    if (want & 1) carries("dropout", {&grads[0]});
     if (want & 1)
       dx = dropout_run(whole(grads[0]), ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(), Tensor(),
                        at == ctx->saved_data.end() ? Tensor() : at->second.toTensor());
@@ -347,6 +350,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const int64_t want = ctx->saved_data["want"].toInt();
     const Tensor dq = want & 1 ? whole(grads[0]) : Tensor(), dk = want & 2 && grads.size() > 1 ? whole(grads[1]) : Tensor();
     std::pair<Tensor, Tensor> g;
+    carries("rotary", {&dq, &dk});
     if (dq.defined() || dk.defined())
       g = rotary_run(dq, dk, saved[0], saved[1], ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
     return once({g.first, g.second, Tensor(), Tensor(), Tensor(), Tensor()});
@@ -445,6 +449,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &rest = saved[4], &lse = saved[5];
     const c10::DeviceGuard guard(q.device());
     const Tensor lengths = dense(saved[6]);
+    carries("window_attention", {&grads[0]});
     Tensor dout = whole(grads[0]).contiguous();
     if (reinterpret_cast<uintptr_t>(dout.data_ptr()) & 15) dout = dout.clone();
     const std::vector<int64_t> w = ctx->saved_data["window"].toIntVector();

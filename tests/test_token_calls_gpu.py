@@ -2,6 +2,7 @@
 memory, tensors that are not all on one device."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from indm_amd import hip, ops
 
@@ -187,3 +188,20 @@ def test_layer_norm_parameters_alone(dtype, R, C):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     if R * C > 1 << 21:     # (its partial sums take 16 bytes a column of up to 1024 workgroups' rows)
         assert torch.cuda.max_memory_allocated() - before < x.numel() * x.element_size() + 8 * C * min(R, 1024)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_through_a_backward_pass_is_refused(name):
+    """a gradient with a tangent: that of the result would be lost without a word"""
+    call, leaf, dy = operators()[name], torch.randn((2, 6, 2, 16), device=DEV).requires_grad_(), torch.randn((2, 6, 2, 16), device=DEV)
+    y = call(leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(dy, dy)
+        if name == "dropout res":      # (its gradient is the one that came in, with its tangent)
+            (g,) = torch.autograd.grad(y, leaf, dual, retain_graph=True)
+            assert torch.equal(forward_ad.unpack_dual(g).tangent, dy)
+        else:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, dual, retain_graph=True)
+    (g,) = torch.autograd.grad(y, leaf, dy)
+    assert g.isfinite().all()
