@@ -652,7 +652,7 @@ int indm_rotary_bf16(const void* q, const void* k, void* yq, void* yk, const lon
  * q, k, v (a HOST array); D contiguous, D % 8 == 0, D <= 128; rows on 16 bytes (bases and strides),
  * strides not negative, token strides and H D up to 2^22.  o dense.  o_lo (bf16, as o, or NULL; fp32: not used): what rounding o to bf16
  * left; the backward's <dO, o> then is as exact as its other terms.  lse fp32 [B, H, T] for
- * the backward (log2 of the sum of exponentials; +inf for rows >= n), or NULL.  left, right, sinks >= 0, scale > 0.
+ * the backward (log2 of the sum of exponentials; +inf for rows >= n), or NULL.  left, right, sinks >= 0, 0 < scale < 2e38.
  * Backward: dq (or NULL), dk and dv (or both NULL) dense from dense o, dO and lse; ws: indm_wattn_bwd_ws_floats floats, 16-byte aligned.  The queries' heads that
  * share a key are summed in a fixed order, the sinks' long sums are split over workgroups and joined in a fixed order. */
 int indm_wattn_fwd_f32(const float* q, const float* k, const float* v, const long* strides, float* o, void* o_lo, float* lse,

@@ -390,7 +390,7 @@ void window_check(const Tensor& q, const Tensor& k, const Tensor& v, const Windo
   if (D % 8 || D < 8 || D > 128) REFUSE("window_attention: heads of 8, 16, ... 128 entries, got ", D);
   if (T > (1 << 28) || B > INT32_MAX || H * D > (1 << 22)) REFUSE("window_attention: up to ", 1 << 28, " tokens of ", 1 << 22, " entries, got ", T, " of ", H * D);
   if (w.left < 0 || w.right < 0 || w.sinks < 0) REFUSE("window_attention: window and sinks >= 0, got (", w.left, ", ", w.right, "), ", w.sinks);
-  if (!(w.scale > 0. && (float)w.scale < INFINITY && (float)w.scale > 0.f)) REFUSE("window_attention: scale > 0, got ", w.scale);
+  if (!((float)w.scale > 0.f && w.scale < 2e38)) REFUSE("window_attention: scale > 0 and below 2e38, got ", w.scale);
   if (lengths.defined() && (lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B))
     REFUSE("window_attention: lengths is int32 [", B, "], got ", lengths.sizes(), " ", lengths.scalar_type());
   on_one_gpu("window_attention", {&q, &k, &v, &lengths});

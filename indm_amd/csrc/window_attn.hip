@@ -934,7 +934,7 @@ inline bool share_queries(int B, int T, int H) { return (long)cdiv(T, 128) * H *
 template <typename T>
 int check(const WAttnArgs& p, const long* strides) {
   if (p.B < 0 || p.T < 0 || p.T > (1 << 28) || p.H <= 0 || p.Hk <= 0 || p.H % p.Hk || p.D <= 0 || p.D > 128 || p.D % 8) return INDM_E_SHAPE;
-  if (p.left < 0 || p.right < 0 || p.sinks < 0 || strides == nullptr || !(p.scale > 0.f && p.scale < INFINITY)) return INDM_E_ARG;
+  if (p.left < 0 || p.right < 0 || p.sinks < 0 || strides == nullptr || !(p.scale > 0.f && p.scale < 2e38f)) return INDM_E_ARG;   // (p.c is finite)
   if (p.B == 0 || p.T == 0) return INDM_OK;
   if (p.q == nullptr || p.k == nullptr || p.v == nullptr || (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15)) return INDM_E_ARG;
   for (int i = 0; i < 9; ++i)

@@ -65,3 +65,15 @@ def test_gradients_that_are_not_wanted():
             return attn(p, p, p, strides, p, None, p, p, None, dq, dk, dv, p, 1, 4, 2, 1, 16, 1, 1, 0, 0, 1.0, None)
 
         assert f(None, None, None) == 0 and f(p, p, None) == f(p, None, p) == f(None, p, None) == f(p + 4, None, None) == -4
+
+
+def test_window_attention_refuses_a_scale_that_overflows():
+    """in units of the kernels' powers of two the scale is 1.44 times larger: past 2.36e38 that is infinite, and every logit NaN"""
+    with pytest.raises(RuntimeError, match="scale > 0"):
+        ops.window_attention(X, X, X, 1, scale=2.5e38)
+    buf = (ctypes.c_char * 512)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    for suf in ("f32", "bf16"):
+        f = getattr(hip.lib(), "indm_wattn_fwd_" + suf)
+        strides = (ctypes.c_long * 9)(*[64] * 9)
+        assert f(p, p, p, strides, p, None, None, None, 1, 4, 2, 1, 16, 1, 1, 0, 0, 2.5e38, None) == -4
