@@ -904,10 +904,11 @@ inline Plan plan_keys(int tile, int B, int T, int H, int Hk, int left, int right
   }
   // Do the sinks reach queries outside of the window?  Then all queries of a block of them are shared by so many workgroups that a
   // wavefront which streams by itself has one tile and a workgroup that streams together eight, up to one or two a compute unit: 256
-  // partial sums of 32 sinks or 512 of 128, 8 or 64 MB at 128 entries.  More blocks of sinks than that have one workgroup each, and the partial
-  // sums then are as large as two fp32 copies of the sinks' dk and dv (one, where key blocks are split).  Where the key blocks leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens,
-  // 8 heads of 128 on 2: 97 us together, 113 apart; 2 x 1021 fp32 tokens, 4 heads of 40: 29 us, 31); where they fill it, it is a launch
-  // before (8 x 4096 tokens, 4 heads of 64: 80 us apart, 89 together).
+  // partial sums of 32 sinks or 512 of 128, 8 or 64 MB at 128 entries.  More blocks of sinks than that have one workgroup each, and the
+  // partial sums then are as large as two fp32 copies of the sinks' dk and dv (one, where key blocks are split).  Where the key blocks
+  // leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens, 8 heads of 128 on 2: 97 us together, 113 apart;
+  // 2 x 1021 fp32 tokens, 4 heads of 40: 29 us, 31); where they fill it, it is a launch before (8 x 4096 tokens, 4 heads of 64: 80 us
+  // apart, 89 together).
   if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
     r.apart = r.splits == 1 && !r.share;
     const bool alone = r.share || r.apart;
