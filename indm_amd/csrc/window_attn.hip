@@ -346,7 +346,7 @@ struct Join {
 
 // workgroup -> work item, so that neighbouring items (which share most of their tiles) run on one XCD's L2.  (Items run over a head's
 // blocks, then the sequences, then the heads: every XCD gets all sequences, whatever their lengths.  Five sequences, one of them empty,
-// 1543 x 8 heads of 128: forward 43 -> 39 us, dk / dv 96 -> 82 us against all heads of a sequence together.)
+// 1543 x 8 heads of 128: forward 44 -> 39 us, dk / dv 122 -> 94 us against all heads of a sequence together.)
 __device__ __forceinline__ int xcd_item(int id, int total) {
   const int x = id & 7, per = total >> 3, rem = total & 7;
   return x * per + (x < rem ? x : rem) + (id >> 3);
@@ -589,7 +589,7 @@ __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, BWD ? 1 : 0,
 // sink keys get from queries whose window they are outside of -- a few keys against all queries, shared by p.chunks workgroups a block of
 // them --, the others the window's part of all keys (SPLIT: where there are few key blocks, each one's queries shared by p.splits
 // workgroups).  What several workgroups contribute to goes to fp32 partial sums that a last kernel adds up in order (no atomics).
-// (WHO spares the launches of one kind the other's tests: 62 instead of 67 us.)
+// (WHO spares the launches of one kind the other's tests: 8 x 4096 tokens, 4 heads of 64, window 256 + 256 without sinks: 79 instead of 83 us.)
 enum { KEYS = 1, SINKS = 2, BOTH = 3 };
 template <typename T, int DP, int WV, bool SHARE, bool SPLIT, int WHO>
 __global__ __launch_bounds__(WV * 64, waves_per_simd(sizeof(T), DP, 2, SHARE)) void wattn_key_kernel(WAttnArgs p) {
@@ -906,9 +906,9 @@ inline Plan plan_keys(int tile, int B, int T, int H, int Hk, int left, int right
   // wavefront which streams by itself has one tile and a workgroup that streams together eight, up to one or two a compute unit: 256
   // partial sums of 32 sinks or 512 of 128, 8 or 64 MB at 128 entries.  More blocks of sinks than that have one workgroup each, and the
   // partial sums then are as large as two fp32 copies of the sinks' dk and dv (one, where key blocks are split).  Where the key blocks
-  // leave the chip room, these workgroups follow them in the same launch (5 x 1543 tokens, 8 heads of 128 on 2: 97 us together, 113 apart;
-  // 2 x 1021 fp32 tokens, 4 heads of 40: 29 us, 31); where they fill it, it is a launch before (8 x 4096 tokens, 4 heads of 64: 80 us
-  // apart, 89 together).
+  // leave the chip room, these workgroups follow them in the same launch (the sinks' and the keys' part and the last sums: 5 x 1543
+  // tokens, 8 heads of 128 on 2: 106 us together, 120 apart; 2 x 1021 fp32 tokens, 4 heads of 40: 29 us either way, a launch less); where
+  // they fill it, it is a launch before (8 x 4096 tokens, 4 heads of 64: 103 us apart, 109 together).
   if (sinks > 0 && (T - 1 > left || (!causal && sinks - 1 > right))) {
     r.apart = r.splits == 1 && !r.share;
     const bool alone = r.share || r.apart;
